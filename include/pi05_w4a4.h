@@ -452,6 +452,65 @@ int pi05w4a4_quantize_e3m2_k16384_warm(const void* x_fp16, int64_t m, void* q6, 
 int pi05w4a4_gemm_e3m2_rows(const void* q6, const float* sa, int64_t m, int32_t k, const int32_t* w6, int32_t n,
                             const void* residual_fp16, void* y_fp16, void* stream);
 
+/*
+ * 8-bit operators: int8 codes in [-127, 127] with fp32 scales, on fp16 or bf16 data
+ * (elem: PI05W4A4_FP16 or PI05W4A4_BF16).  No counterpart in the reference, which has no
+ * 8-bit path and leaves the cache to its caller's framework.
+ *
+ * pi05w4a4_int8_rows: rows of K elements (K % 8 == 0, K <= 32768) to codes q [M, K] and
+ *   scales [M]; x has row stride ldx (elements, % 8 == 0, 16-byte aligned rows).
+ *     norm_w == NULL: y = x.  Otherwise y = h * g / sqrt(mean(h^2) + eps), g = 1 + w
+ *     (unit_offset) or w, with h = x, or, with a residual (row stride ldr), h = x + residual
+ *     rounded to the element type and written to h_out [M, K].
+ *     scale = max|y| / 127 + 1e-12, q = rint(y / scale).  A row with a NaN or an infinity:
+ *     scale NaN, codes 0.
+ * pi05w4a4_int8_gemm: y[m, n] = (sum_k q[m, k] w[n, k]) * sq[m] * sw[n] + bias[n] +
+ *   residual[m, n], in fp32 with one rounding; bias and residual may be null.  q and w have
+ *   row strides ldq, ldw (bytes, % 16 == 0; rows 16-byte aligned), K % 16 == 0, K <= 65536;
+ *   y is [M, N] contiguous, 16-byte aligned; the residual has row stride ldr (elements).
+ *   Needs pi05w4a4_int8_gemm_workspace_bytes(M, N, K) bytes (0 for most sizes).
+ *
+ * KV cache: pages of 64 tokens.  k_cache int8 [pages, KVH, 64, D], v_cache int8 [pages, KVH,
+ *   D, 64] (transposed within the page), k_scale and v_scale fp32 [pages, KVH]; D is 64, 128
+ *   or 256.  Token i of sequence b is row i % 64 of page table[b * table_stride + i / 64].
+ *   Table entries outside [0, pages) name no page: tokens there are neither written nor read.
+ *
+ * pi05w4a4_int8_kv_append: writes tokens lens[b] .. lens[b] + counts[b] - 1 (counts null: all
+ *   t) of every sequence; k, v [B, T, KVH, D] with strides {batch, token, head} in elements
+ *   (% 8 == 0), 16-byte aligned.  The scale of a page is the largest that its tokens needed,
+ *   max|.| / 127 + 1e-12; where it grows, the page's earlier codes are rounded to it.  A page
+ *   whose first token is new is written whole, zeros behind the last token.  Tokens past
+ *   table_pages * 64 are dropped.  lens is read only.  A page may be written for one sequence
+ *   at a time.
+ * pi05w4a4_int8_kv_attention: out [B, T, H, D] = softmax(scaling q K^T) V over the tokens that
+ *   query i of sequence b sees: with ql = q_lens[b] (null: T), the first lens[b] - ql + i + 1
+ *   when causal, else lens[b]; none for i >= ql.  lens counts the new tokens too.  A query
+ *   that sees none gets zeros.  lse, when not null, fp32 [B, T, H]: the natural log of the sum
+ *   of exp(scaling q k) (-inf where none is seen).  Query head h reads KV head h / (H / KVH).
+ *   Needs pi05w4a4_int8_kv_attention_workspace_bytes(...) bytes (0 without a split).
+ */
+#define PI05W4A4_FP16 0
+#define PI05W4A4_BF16 1
+int pi05w4a4_int8_rows(const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* norm_w, float eps,
+                       int32_t unit_offset, int32_t elem, int64_t m, int32_t k, void* q, float* scale, void* h_out,
+                       void* stream);
+size_t pi05w4a4_int8_gemm_workspace_bytes(int64_t m, int32_t n, int32_t k);
+int pi05w4a4_int8_gemm(const void* q, int64_t ldq, const float* sq, int64_t m, int32_t k, const void* w, int64_t ldw,
+                       const float* sw, int32_t n, const void* bias, const void* residual, int64_t ldr, int32_t elem,
+                       void* y, void* workspace, size_t workspace_bytes, void* stream);
+int pi05w4a4_int8_kv_append(const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides, int32_t elem,
+                            int32_t b, int32_t t, int32_t kvh, int32_t d, void* k_cache, void* v_cache, float* k_scale,
+                            float* v_scale, int32_t pages, const int32_t* table, int64_t table_stride,
+                            int32_t table_pages, const int32_t* lens, const int32_t* counts, void* stream);
+size_t pi05w4a4_int8_kv_attention_workspace_bytes(int32_t b, int32_t t, int32_t h, int32_t kvh, int32_t d,
+                                                  int32_t table_pages);
+int pi05w4a4_int8_kv_attention(const void* q, const int64_t* q_strides, int32_t elem, int32_t b, int32_t t, int32_t h,
+                               int32_t kvh, int32_t d, const void* k_cache, const void* v_cache, const float* k_scale,
+                               const float* v_scale, int32_t pages, const int32_t* table, int64_t table_stride,
+                               int32_t table_pages, const int32_t* lens, const int32_t* q_lens, float scaling,
+                               int32_t causal, void* out, float* lse, void* workspace, size_t workspace_bytes,
+                               void* stream);
+
 #ifdef __cplusplus
 }
 #endif

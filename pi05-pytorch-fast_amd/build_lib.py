@@ -33,7 +33,8 @@ from pathlib import Path
 
 PKG_ROOT = Path(__file__).resolve().parent
 CSRC = PKG_ROOT / "csrc"
-SOURCES = ["quant_rot.hip", "repack.hip", "gemm.hip", "rmsnorm.hip", "attention.hip", "capi.hip"]
+SOURCES = ["quant_rot.hip", "repack.hip", "gemm.hip", "rmsnorm.hip", "attention.hip", "capi.hip",
+           "int8_rows.hip", "int8_gemm.hip", "kv_int8.hip", "capi_int8.hip"]
 OUT = PKG_ROOT / "pi05_fast" / "w4a4" / "_lib" / "libpi05_w4a4.so"
 DEFAULT_ARCH = "gfx950"
 

@@ -1145,3 +1145,17 @@ extern "C" int pi05w4a4_int4_gemm_noalloc(const void* x_fp16, int64_t m, int32_t
   // words), and every split-K slice writes all of its partials before the reduce reads them.
   return pi05w4a4_int4_gemm(x_fp16, m, k, w_mfma, n, y_fp16, q, sa, ws, ws_bytes, stream);
 }
+
+// The same error text for the entry points of the other translation units.
+namespace w4a4 {
+int capi_fail(int code, const char* fmt, ...) {
+  char buf[512];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof(buf), fmt, ap);
+  va_end(ap);
+  return fail(code, "%s", buf);
+}
+int capi_ok() { return ok(); }
+int capi_hip(hipError_t e, const char* what) { return hip_status(e, what); }
+}  // namespace w4a4

@@ -146,6 +146,17 @@ def load_int4_gemm():
         "pi05w4a4_quantize_e3m2_k16384_warm": (
             ctypes.c_int, [vp, i64, vp, vp, ctypes.POINTER(vp), ctypes.POINTER(sz), i32, vp]),
         "pi05w4a4_gemm_e3m2_rows": (ctypes.c_int, [vp, vp, i64, i32, vp, i32, vp, vp, vp]),
+        "pi05w4a4_int8_rows": (
+            ctypes.c_int, [vp, i64, vp, i64, vp, ctypes.c_float, i32, i32, i64, i32, vp, vp, vp, vp]),
+        "pi05w4a4_int8_gemm_workspace_bytes": (sz, [i64, i32, i32]),
+        "pi05w4a4_int8_gemm": (
+            ctypes.c_int, [vp, i64, vp, i64, i32, vp, i64, vp, i32, vp, vp, i64, i32, vp, vp, sz, vp]),
+        "pi05w4a4_int8_kv_append": (
+            ctypes.c_int, [vp, vp, vp, vp, i32, i32, i32, i32, i32, vp, vp, vp, vp, i32, vp, i64, i32, vp, vp, vp]),
+        "pi05w4a4_int8_kv_attention_workspace_bytes": (sz, [i32, i32, i32, i32, i32, i32]),
+        "pi05w4a4_int8_kv_attention": (
+            ctypes.c_int, [vp, vp, i32, i32, i32, i32, i32, i32, vp, vp, vp, vp, i32, vp, i64, i32, vp, vp,
+                           ctypes.c_float, i32, vp, vp, vp, sz, vp]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)
