@@ -95,7 +95,7 @@ extern "C" int pi05w4a4_int8_gemm(const void* q, int64_t ldq, const float* sq, i
     return capi_fail(PI05W4A4_EINVAL, "row strides of q and w must be multiples of 16 bytes of at most 2^23, got %lld and %lld",
                      (long long)ldq, (long long)ldw);
   if (residual != nullptr && ldr < 0) return capi_fail(PI05W4A4_EINVAL, "the residual's row stride must be >= 0");
-  if (((m + 63) / 64) * ((n + 63LL) / 64) > 0x7fffffffLL)
+  if (((m + 63) / 64) * ((n + 31LL) / 32) > 0x7fffffffLL / 16)
     return capi_fail(PI05W4A4_EINVAL, "M=%lld N=%d is more tiles than one launch holds", (long long)m, n);
   const Int8GemmPlan plan = int8_gemm_plan(m, n, k, device_cu_count());
   const size_t need = plan.ksplit > 1 ? static_cast<size_t>(plan.ksplit) * m * n * sizeof(int32_t) : 0;

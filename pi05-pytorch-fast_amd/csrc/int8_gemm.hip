@@ -9,11 +9,11 @@
 // The weights are MFMA operand A, so that a lane ends with four consecutive columns of one row.
 // In a 64-deep step lane L holds k = 16 (L / 16) .. + 15 of row L % 16 of either operand.
 //
-// Two kernels:
-//   int8_tile_kernel    BM x BN tiles through LDS, for everything but few rows: bound by the MFMAs
-//                       (many rows) or by latency (few tiles);
-//   int8_stream_kernel  up to 64 rows: the weights stream from memory straight into registers,
-//                       the waves of a workgroup split K.
+// Three kernels:
+//   int8_stream_kernel  up to 16 rows: the weights stream from memory straight into registers,
+//                       the waves of a workgroup split K;
+//   int8_tile_kernel    64 x 64 and 128 x 64 tiles through LDS, with K slices where tiles are few;
+//   int8_big_kernel     256 x 256 tiles, for what fills the CUs with them.
 
 #include "direct_load.h"
 #include "int8_internal.h"
@@ -22,12 +22,13 @@ namespace w4a4 {
 namespace {
 
 typedef int v4i __attribute__((ext_vector_type(4)));
+typedef int v16i __attribute__((ext_vector_type(16)));
 template <typename T>
 using vec4 = T __attribute__((ext_vector_type(4)));
 
-// y[row, col .. col + 3] of one accumulator quad, with the bias and the residual: fp32, one
-// rounding.  `whole`: four columns inside N whose loads are aligned.
-template <typename T>
+// y[row, col .. col + 3] of one accumulator quad, with the bias and (RES) the residual: fp32, one
+// rounding.
+template <typename T, bool RES = true>
 struct Epilogue {
   const Int8GemmParams& p;
   bool res_vec;  // residual quads can be read as one aligned load
@@ -45,7 +46,7 @@ struct Epilogue {
   __device__ __forceinline__ vec4<T> operator()(const v4i acc, float sq, const float (&sw)[4], const float (&bias)[4],
                                                 int64_t row, int64_t col) const {
     float res[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (p.res != nullptr && row < p.m) {
+    if (RES && p.res != nullptr && row < p.m) {
       const T* const rp = static_cast<const T*>(p.res) + row * p.ldr + col;
       if (res_vec) {
         if (col < p.n) {
@@ -61,54 +62,87 @@ struct Epilogue {
     }
     vec4<T> o;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) o[r] = static_cast<T>((static_cast<float>(acc[r]) * sq) * sw[r] + bias[r] + res[r]);
+    for (int r = 0; r < 4; ++r) {
+      const float v = fmaf(static_cast<float>(acc[r]) * sq, sw[r], bias[r]);
+      o[r] = static_cast<T>(RES ? v + res[r] : v);
+    }
     return o;
   }
 };
 
+// The sums of columns col .. col + 3 of a K slice, to its plane of partial sums.
+__device__ __forceinline__ void store_partial(const Int8GemmParams& p, const v4i s, int split, int64_t row, int64_t col) {
+  if (row >= p.m) return;
+  int32_t* const o = p.partial + (split * p.m + row) * p.n + col;
+  if ((p.n & 3) == 0) {
+    if (col < p.n) *reinterpret_cast<v4i*>(o) = s;
+  } else {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (col + r < p.n) o[r] = s[r];
+  }
+}
+
 // ------------------------------------------------------------------ LDS tiles
-// Stage: BM rows of q, then BN rows of w, 128 bytes of K each.  A 1 KB direct load brings 8 rows;
-// 16-byte chunk c of row r is kept at chunk c ^ (r % 8), so that eight rows read at one chunk
-// meet eight different bank groups.
-template <int BM, int BN, int WM, int WN, int ST>
+// BM x BN tiles of waves that each hold 64 x 64 of it and one KW-th of every 128-byte stage, on
+// v_mfma_i32_32x32x32_i8: one wave a SIMD feeds it at its full rate (16 x 16 x 64: 28 clocks
+// for 16), and the K split gives small tiles enough waves without more LDS reads.  A wave then
+// owns 4 / KW of the four 32 x 32 blocks of its position, sums the other waves' parts of them
+// through LDS and finishes them.
+// Stage: BM rows of q, then BN rows of w, 128 bytes of K each, in a ring of ST.  A 1 KB direct
+// load brings 8 rows; 16-byte chunk c of row r is kept at chunk c ^ (r % 8), so that eight rows
+// read at one chunk meet eight different bank groups.
+template <int BM, int BN, int KW, int ST>
 struct Int8Tile {
-  static constexpr int kWaves = (BM / WM) * (BN / WN);
-  static constexpr int MI = WM / 16, NI = WN / 16;
+  static constexpr int kPos = (BM / 64) * (BN / 64);
+  static constexpr int kWaves = kPos * KW;
   static constexpr int kStage = (BM + BN) * 128;
   static constexpr int kPA = BM / 8 / kWaves, kPB = BN / 8 / kWaves;  // pieces of a wave
-  static constexpr int kOutStride = WN + 8;                           // staged output row, elements
-  static constexpr int kLds = ST * kStage;
+  static constexpr int kOwn = 4 / KW;                                 // blocks that a wave finishes
+  static constexpr int kOutStride = 32 + 8;                           // staged output row, elements
+  static constexpr int kBlock = KW > 1 ? (KW - 1) * 4096 : 4096;       // LDS of a block: its sums, then its output rows
+  static constexpr int kLds = ST * kStage > kPos * 4 * kBlock ? ST * kStage : kPos * 4 * kBlock;
+  static_assert(32 * kOutStride * 2 <= kBlock, "a block's output rows fit where its sums were");
   static_assert(BM % (8 * kWaves) == 0 && BN % (8 * kWaves) == 0, "pieces are dealt evenly");
-  static_assert(kWaves * 16 * kOutStride * 2 <= kLds, "the output rows are staged in the ring");
 };
 
-template <typename T, int BM, int BN, int WM, int WN, int ST>
-__global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void int8_tile_kernel(Int8GemmParams p) {
-  using C = Int8Tile<BM, BN, WM, WN, ST>;
-  constexpr int MI = C::MI, NI = C::NI;
-  __shared__ __align__(1024) char lds[C::kLds];
+// Two waves a SIMD in the bounds: the accumulators then stay in ordinary registers (given twice as
+// many, the compiler moves them to the accumulation registers and back in every step).
+// Measured (us, 2048 deep, 2560 columns): 100 rows 8.5, 776 rows 14; a 64 x 64 step of a CU costs
+// 0.25 us, a 128 x 64 step 0.36, where its MFMAs alone take 0.07 and 0.13: the steps are bound by the
+// issue of their loads and reads.
+template <typename T, int BM, int BN, int KW, int ST>
+__global__ __launch_bounds__(64 * (BM / 64) * (BN / 64) * KW, 2) void int8_tile_kernel(Int8GemmParams p) {
+  using C = Int8Tile<BM, BN, KW, ST>;
+  extern __shared__ __align__(1024) char lds[];
   const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)lds));
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wm = wave / (BN / WN), wn = wave % (BN / WN);
+  const int kg = wave % KW, pos = wave / KW;
+  const int wm = pos / (BN / 64), wn = pos % (BN / 64);
 
   // XCD x = b % 8 owns a contiguous run of the tiles, which walk the m-tiles of a group of 8 under
   // each n-tile: the tiles that run together on an XCD share operands in its L2.
-  int mt, nt;
+  int mt, nt, split;
   {
-    const int total = p.mtiles * p.ntiles;
+    const int tiles = p.mtiles * p.ntiles, total = tiles * p.ksplit;
     const int xcd = blockIdx.x & 7, q8 = total >> 3, r8 = total & 7;
-    const int t = xcd * q8 + min(xcd, r8) + (static_cast<int>(blockIdx.x) >> 3);
+    const int s = xcd * q8 + min(xcd, r8) + (static_cast<int>(blockIdx.x) >> 3);
+    split = __builtin_amdgcn_readfirstlane(s / tiles);
+    const int t = s - split * tiles;
     const int full = 8 * p.ntiles;
     const int g = t / full, rem = t - g * full;
     const int size = min(8, p.mtiles - 8 * g);
-    nt = rem / size;
-    mt = 8 * g + (rem - nt * size);
+    nt = __builtin_amdgcn_readfirstlane(rem / size);  // uniform, and to be held in scalar registers
+    mt = __builtin_amdgcn_readfirstlane(8 * g + (rem - nt * size));
   }
   const int64_t m0 = static_cast<int64_t>(mt) * BM;
   const int n0 = nt * BN;
-  const int nkb = (p.k + 127) >> 7;
-  const bool ragged = (p.k & 127) != 0;
+  // The 128-byte blocks of this K slice; only the last slice ends inside one.
+  const int blocks = (p.k + 127) >> 7;
+  const int kb0 = static_cast<int>(static_cast<int64_t>(blocks) * split / p.ksplit);
+  const int nkb = static_cast<int>(static_cast<int64_t>(blocks) * (split + 1) / p.ksplit) - kb0;
+  const bool ragged = (p.k & 127) != 0 && split == p.ksplit - 1;
 
   // Rows past the matrix are clamped to its last one (their results are not stored).
   const int rchunk = (lane & 7) ^ (lane >> 3);
@@ -123,131 +157,397 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void int8_tile_kernel(I
     const int r = min(8 * (wave + C::kWaves * j) + (lane >> 3), p.n - 1 - n0);
     vb[j] = static_cast<uint32_t>(r) * static_cast<uint32_t>(p.ldw) + rchunk * 16;
   }
-  const char* const abase = reinterpret_cast<const char*>(p.q) + m0 * p.ldq;
-  const char* const bbase = reinterpret_cast<const char*>(p.w) + static_cast<int64_t>(n0) * p.ldw;
-  auto issue = [&](int kb, int slot) {
+  const char* const abase = reinterpret_cast<const char*>(p.q) + m0 * p.ldq + static_cast<int64_t>(kb0) * 128;
+  const char* const bbase = reinterpret_cast<const char*>(p.w) + static_cast<int64_t>(n0) * p.ldw + static_cast<int64_t>(kb0) * 128;
+  constexpr int kPieces = C::kPA + C::kPB;
+  auto issue = [&](int kb, int slot, int j) {  // piece j of this wave
     // The last block of a K that is no multiple of 128: chunks past the row's end read its last one.
     const uint32_t back = ragged && kb == nkb - 1 ? 16u * max(0, rchunk - ((p.k & 127) / 16 - 1)) : 0u;
     const uint32_t dst = lds0 + slot * C::kStage + wave * 1024;
-#pragma unroll
-    for (int j = 0; j < C::kPA; ++j) load_lds_1k(abase + static_cast<int64_t>(kb) * 128, va[j] - back, dst + j * C::kWaves * 1024);
-#pragma unroll
-    for (int j = 0; j < C::kPB; ++j)
-      load_lds_1k(bbase + static_cast<int64_t>(kb) * 128, vb[j] - back, dst + BM * 128 + j * C::kWaves * 1024);
+    if (j < C::kPA) load_lds_1k(abase + static_cast<int64_t>(kb) * 128, va[j] - back, dst + j * C::kWaves * 1024);
+    else load_lds_1k(bbase + static_cast<int64_t>(kb) * 128, vb[j - C::kPA] - back, dst + BM * 128 + (j - C::kPA) * C::kWaves * 1024);
   };
 
-  v4i acc[MI][NI];
+  v16i acc[2][2];
 #pragma unroll
-  for (int i = 0; i < MI; ++i)
+  for (int i = 0; i < 2; ++i)
 #pragma unroll
-    for (int j = 0; j < NI; ++j) acc[i][j] = v4i{0, 0, 0, 0};
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0;
 
-  // Lane L reads row L % 16 at chunk 4 kk + L / 16 of a 16-row fragment.
-  const int roff = (lane & 15) * 128 + (((lane >> 4) ^ (lane & 7)) * 16);
-  const int aoff = wm * WM * 128 + roff, boff = BM * 128 + wn * WN * 128 + roff;
+  // Lane L of a 32-deep MFMA holds k = 16 (L / 32) .. + 15 of row L % 32 of either operand: chunk
+  // 2 kk + L / 32 of its row.
+  const int roff = (lane & 31) * 128 + (((lane >> 5) ^ (lane & 7)) * 16);
+  const int aoff = wm * 64 * 128 + roff, boff = BM * 128 + wn * 64 * 128 + roff;
 
-#pragma unroll
-  for (int s = 0; s < ST - 1; ++s)
-    if (s < nkb) issue(s, s);
-  int slot = 0;
-  for (int kb = 0; kb < nkb; ++kb) {
-    // Younger than this stage's loads: those of the ST - 2 stages after it, where they exist.
-    if (ST > 2 && kb + ST - 2 < nkb) wait_vm<(ST - 2) * (C::kPA + C::kPB)>();
-    else wait_vm<0>();
-    lds_done_barrier();  // all waves' loads of this stage have landed; all reads of the one before are done
-    if (kb + ST - 1 < nkb) issue(kb + ST - 1, slot == 0 ? ST - 1 : slot - 1);
+  // The fragments of a stage are read one stage ahead of their MFMAs.  Reads and loads go out among
+  // the MFMAs, the reads in the first half of a step and the loads in the second: in a bunch, each
+  // holds a wave up until the one before is taken (128 x 128 tiles, a step of K = 8192 at 100 rows:
+  // 0.27 us of MFMAs and 0.30 of reads and loads took 0.48).
+  constexpr int kParts = 4 / KW, kMfmas = 4 * kParts;
+  v4i a0[2 * kParts], b0[2 * kParts], a1[2 * kParts], b1[2 * kParts];
+  auto read = [&](int slot, v4i (&a)[2 * kParts], v4i (&b)[2 * kParts], int f) {  // in the order of their use
     const char* const st = lds + slot * C::kStage;
-#pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-      v4i a[MI], b[NI];
-#pragma unroll
-      for (int i = 0; i < MI; ++i) a[i] = *reinterpret_cast<const v4i*>(st + ((aoff + i * 2048) ^ (kk * 64)));
-#pragma unroll
-      for (int j = 0; j < NI; ++j) b[j] = *reinterpret_cast<const v4i*>(st + ((boff + j * 2048) ^ (kk * 64)));
-      if (ragged && kb == nkb - 1 && kk * 64 + (lane >> 4) * 16 >= (p.k & 127)) {
-#pragma unroll
-        for (int i = 0; i < MI; ++i) a[i] = v4i{0, 0, 0, 0};
-      }
-#pragma unroll
-      for (int i = 0; i < MI; ++i)
-#pragma unroll
-        for (int j = 0; j < NI; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(b[j], a[i], acc[i][j], 0, 0, 0);
+    const int k4 = f >> 2, i = f & 1, kk = kg * kParts + k4;
+    if (f & 2) a[2 * k4 + i] = *reinterpret_cast<const v4i*>(st + ((aoff + i * 4096) ^ (kk * 32)));
+    else b[2 * k4 + i] = *reinterpret_cast<const v4i*>(st + ((boff + i * 4096) ^ (kk * 32)));
+  };
+  auto mfma = [&](const v4i (&a)[2 * kParts], const v4i (&b)[2 * kParts], int f) {
+    const int k4 = f >> 2, i = (f >> 1) & 1, j = f & 1;
+    acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(b[2 * k4 + j], a[2 * k4 + i], acc[i][j], 0, 0, 0);
+  };
+  int slot = 0;  // of the stage that is multiplied
+  auto step = [&](int kb, v4i (&a)[2 * kParts], v4i (&b)[2 * kParts], v4i (&an)[2 * kParts], v4i (&bn)[2 * kParts]) {
+    const int next = slot == ST - 1 ? 0 : slot + 1;
+    if (kb + 1 < nkb) {
+      // Younger than the next stage's loads: those of the ST - 2 stages after it, where they exist.
+      if (ST > 2 && kb + ST - 1 < nkb) wait_vm<(ST - 2) * kPieces>();
+      else wait_vm<0>();
+      lds_done_barrier();  // the next stage has landed for all waves, which hold this one in registers
     }
-    slot = slot == ST - 1 ? 0 : slot + 1;
-  }
-  lds_done_barrier();  // the ring becomes the staging of the output rows
-
-  const Epilogue<T> epi(p);
-  const int lrow = lane & 15, lcol = (lane >> 4) * 4;
-  const int64_t mw = m0 + wm * WM;
-  const int nw = n0 + wn * WN;
-  float sw[NI][4], bias[NI][4];
+    if (ragged && kb == nkb - 1) {  // the activations past K count as zeros
 #pragma unroll
-  for (int j = 0; j < NI; ++j) epi.scales(nw + j * 16 + lcol, sw[j], bias[j]);
-  T* const stage = reinterpret_cast<T*>(lds) + wave * 16 * C::kOutStride;
+      for (int k4 = 0; k4 < kParts; ++k4)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          if ((kg * kParts + k4) * 32 + (lane >> 5) * 16 >= (p.k & 127)) a[2 * k4 + i] = v4i{0, 0, 0, 0};
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int f = 0; f < kMfmas / 2; ++f) {
+      mfma(a, b, f);
+      read(next, an, bn, 2 * f);  // past the last stage: an old one's, not used
+      read(next, an, bn, 2 * f + 1);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    const bool more = kb + ST < nkb;
+#pragma unroll
+    for (int f = 0; f < kMfmas / 2; ++f) {
+      mfma(a, b, kMfmas / 2 + f);
+      if (more) {
+#pragma unroll
+        for (int j = f * kPieces / (kMfmas / 2); j < (f + 1) * kPieces / (kMfmas / 2); ++j) issue(kb + ST, slot, j);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    slot = next;
+  };
+
+#pragma unroll
+  for (int s = 0; s < ST; ++s)
+    if (s < nkb) {
+#pragma unroll
+      for (int j = 0; j < kPieces; ++j) issue(s, s, j);
+    }
+  if (nkb >= ST) wait_vm<(ST - 1) * kPieces>();
+  else wait_vm<0>();
+  lds_done_barrier();
+#pragma unroll
+  for (int f = 0; f < 4 * kParts; ++f) read(0, a0, b0, f);
+#pragma unroll 1
+  for (int kb = 0; kb < nkb; kb += 2) {
+    step(kb, a0, b0, a1, b1);
+    if (kb + 1 < nkb) step(kb + 1, a1, b1, a0, b0);
+  }
+  lds_done_barrier();  // the ring becomes the waves' sums and the staging of the output rows
+
+  if constexpr (KW > 1) {
+    // Block f = 2 i + j of a position belongs to K group f / kOwn; part q of it is that of group q
+    // (q + 1 from the owner on).
+#pragma unroll
+    for (int f = 0; f < 4; ++f) {
+      const int owner = f / C::kOwn;
+      if (kg == owner) continue;
+      const int part = kg - (kg > owner);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const v16i v = acc[f >> 1][f & 1];
+        reinterpret_cast<v4i*>(lds + (pos * 4 + f) * C::kBlock + part * 4096)[r * 64 + lane] =
+            v4i{v[4 * r], v[4 * r + 1], v[4 * r + 2], v[4 * r + 3]};
+      }
+    }
+    __syncthreads();
+  }
+  const Epilogue<T> epi(p);
   T* const y = static_cast<T*>(p.y);
   const bool wide = (p.n & 7) == 0;
 #pragma unroll
-  for (int i = 0; i < MI; ++i) {
-    const int64_t row = mw + i * 16 + lrow;
+  for (int f = 0; f < 4; ++f) {
+    if (f / C::kOwn != kg) continue;
+    char* const mine = lds + (pos * 4 + f) * C::kBlock;
+    T* const stage = reinterpret_cast<T*>(mine);
+    const int64_t mb = m0 + wm * 64 + (f >> 1) * 32, row = mb + (lane & 31);
+    const int nb = n0 + wn * 64 + (f & 1) * 32;
     const float sq = p.sq[min(row, p.m - 1)];
+    v4i sum[4];
 #pragma unroll
-    for (int j = 0; j < NI; ++j)
-      *reinterpret_cast<vec4<T>*>(stage + lrow * C::kOutStride + j * 16 + lcol) =
-          epi(acc[i][j], sq, sw[j], bias[j], row, nw + j * 16 + lcol);
+    for (int t = 0; t < 4; ++t) {  // columns 8 t + 4 (L / 32) .. + 3 of row L % 32
+      const v16i v = acc[f >> 1][f & 1];
+      sum[t] = v4i{v[4 * t], v[4 * t + 1], v[4 * t + 2], v[4 * t + 3]};
+      if constexpr (KW > 1) {
+#pragma unroll
+        for (int q = 0; q < KW - 1; ++q) sum[t] += reinterpret_cast<const v4i*>(mine + q * 4096)[t * 64 + lane];
+      }
+    }
+    if (p.ksplit > 1) {
+#pragma unroll
+      for (int t = 0; t < 4; ++t) store_partial(p, sum[t], split, row, nb + 8 * t + 4 * (lane >> 5));
+      continue;
+    }
+    __builtin_amdgcn_wave_barrier();  // the sums are in registers: the output rows take their place
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const int c = 8 * t + 4 * (lane >> 5);
+      float sw[4], bias[4];
+      epi.scales(nb + c, sw, bias);
+      *reinterpret_cast<vec4<T>*>(stage + (lane & 31) * C::kOutStride + c) = epi(sum[t], sq, sw, bias, row, nb + c);
+    }
     __builtin_amdgcn_wave_barrier();
     if (wide) {
-      constexpr int LPR = WN / 8, RPI = 64 / LPR;  // lanes of a row, rows of one store
 #pragma unroll
-      for (int s = 0; s < 16 / RPI; ++s) {
-        const int r = s * RPI + lane / LPR, c = (lane % LPR) * 8;
-        const int64_t orow = mw + i * 16 + r;
-        if (orow < p.m && nw + c < p.n)
-          *reinterpret_cast<v4i*>(y + orow * p.n + nw + c) = *reinterpret_cast<const v4i*>(stage + r * C::kOutStride + c);
+      for (int s = 0; s < 2; ++s) {
+        const int r = s * 16 + (lane >> 2), c = (lane & 3) * 8;
+        if (mb + r < p.m && nb + c < p.n)
+          *reinterpret_cast<v4i*>(y + (mb + r) * p.n + nb + c) = *reinterpret_cast<const v4i*>(stage + r * C::kOutStride + c);
       }
     } else {
-      for (int e = lane; e < 16 * WN; e += 64) {
-        const int r = e / WN, c = e % WN;
-        const int64_t orow = mw + i * 16 + r;
-        if (orow < p.m && nw + c < p.n) y[orow * p.n + nw + c] = stage[r * C::kOutStride + c];
+      for (int e = lane; e < 32 * 32; e += 64) {
+        const int r = e >> 5, c = e & 31;
+        if (mb + r < p.m && nb + c < p.n) y[(mb + r) * p.n + nb + c] = stage[r * C::kOutStride + c];
       }
     }
     __builtin_amdgcn_wave_barrier();
   }
 }
 
+// ------------------------------------------------------------------ many rows
+// 256 x 256 tiles, eight waves of 64 x 128 (two a SIMD), a ring of two 128-byte stages.  The loads
+// of the next stage go out at the top of a step, before its MFMAs, and have all of them to land:
+// spread among the MFMAs, or as 64-byte stages three steps ahead, they were no faster (8192^3,
+// us: 431 / 469 / 462).
+// The workgroups walk the tiles, one a CU; the loads run on into the next tile, so that its first
+// stage lands during the epilogue, whose scales wait in LDS since the tile's first step.
+// What bounds it: power.  8192^3 takes 395 us with operands of ones and 431-445 with random ones, the
+// clock falling from 2.3 to 1.87 GHz; four waves of 128 x 128 on 32 x 32 x 32 MFMAs need a fifth
+// fewer clocks and run them at 1.62 GHz, in the same time.  MFMAs on random registers alone hold
+// 3450 TOP/s of the 5000 that the matrix units issue.
+// Tiles of 128 x 256 with two workgroups a CU, so that one's epilogue overlaps the other's product,
+// lose more to their operand traffic (6208 x 2048 x 16384: 238 us against 227).
+struct Int8Big {
+  static constexpr int kTile = 256, kWaves = 8, MI = 4, NI = 8;
+  static constexpr int kStage = 2 * kTile * 128;
+  static constexpr int kOutStride = 64 + 8;               // half of a wave's columns at a time
+  static constexpr int kScale = 2 * kStage;               // fp32 sq, sw, bias of the tile
+  static constexpr int kOut = kScale + 3 * kTile * 4;
+  static constexpr int kLds = kOut + kWaves * 16 * kOutStride * 2;
+};
+
+template <typename T, bool RES>
+__global__ __launch_bounds__(512) void int8_big_kernel(Int8GemmParams p) {
+  using C = Int8Big;
+  constexpr int MI = C::MI, NI = C::NI;
+  extern __shared__ __align__(1024) char lds[];
+  const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)lds));
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave >> 1, wn = wave & 1;
+  const int nkb = (p.k + 127) >> 7;
+  const bool ragged = (p.k & 127) != 0;
+
+  // XCD b % 8 owns a contiguous run of the tiles, which its workgroups take in turn; the order
+  // walks the m-tiles of a group of 8 under each n-tile, so that the 32 tiles that run together
+  // on an XCD are 8 x 4 and share their operands in its L2.
+  int t, t_end, t_stride;
+  {
+    const int total = p.ntiles * p.mtiles, grid = gridDim.x, xcd = blockIdx.x & 7;
+    const int q = total >> 3, r = total & 7;
+    const int begin = xcd * q + min(xcd, r);
+    t = begin + (static_cast<int>(blockIdx.x) >> 3);
+    t_end = begin + q + (xcd < r ? 1 : 0);
+    t_stride = (grid >> 3) + (xcd < (grid & 7) ? 1 : 0);
+  }
+  if (t >= t_end) return;
+  struct Tile { int64_t m0; int n0; };
+  auto tile_at = [&](int i) {
+    const int full = 8 * p.ntiles;
+    const int g = i / full, rem = i - g * full;
+    const int size = min(8, p.mtiles - 8 * g);
+    const int nt = __builtin_amdgcn_readfirstlane(rem / size);
+    const int mt = __builtin_amdgcn_readfirstlane(8 * g + (rem - nt * size));
+    return Tile{static_cast<int64_t>(mt) * C::kTile, nt * C::kTile};
+  };
+
+  // Loader: four 1 KB pieces (8 rows) of either operand a wave and stage.  Rows past the matrix are
+  // clamped to its last one, and chunks past K to the row's last one.
+  const int rchunk = (lane & 7) ^ (lane >> 3);
+  uint32_t va[4], vb[4];
+  const char *abase, *bbase;
+  auto load_tile = [&](const Tile& c) {
+    abase = reinterpret_cast<const char*>(p.q) + c.m0 * p.ldq;
+    bbase = reinterpret_cast<const char*>(p.w) + static_cast<int64_t>(c.n0) * p.ldw;
+    const int mlast = static_cast<int>(min(p.m - 1 - c.m0, static_cast<int64_t>(C::kTile - 1))), nlast = min(p.n - 1 - c.n0, C::kTile - 1);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int r = 8 * (wave + 8 * j) + (lane >> 3);
+      va[j] = static_cast<uint32_t>(min(r, mlast)) * static_cast<uint32_t>(p.ldq) + rchunk * 16;
+      vb[j] = static_cast<uint32_t>(min(r, nlast)) * static_cast<uint32_t>(p.ldw) + rchunk * 16;
+    }
+  };
+  auto issue = [&](int kb, int slot) {
+    const uint32_t back = ragged && kb == nkb - 1 ? 16u * max(0, rchunk - ((p.k & 127) / 16 - 1)) : 0u;
+    const uint32_t dst = lds0 + slot + wave * 1024;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) load_lds_1k(abase + static_cast<int64_t>(kb) * 128, va[j] - back, dst + j * 8192);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) load_lds_1k(bbase + static_cast<int64_t>(kb) * 128, vb[j] - back, dst + 32768 + j * 8192);
+  };
+
+  const int roff = (lane & 15) * 128 + (((lane >> 4) ^ (lane & 7)) * 16);
+  const int aoff = wm * 64 * 128 + roff, boff = 32768 + wn * 128 * 128 + roff;
+  const Epilogue<T, RES> epi(p);
+  float* const sc = reinterpret_cast<float*>(lds + C::kScale);
+  const bool wide = (p.n & 7) == 0;
+
+  Tile cur = tile_at(t);
+  load_tile(cur);
+  issue(0, 0);
+  int slot = 0;
+  for (;;) {
+    const bool more = t + t_stride < t_end;
+    // Threads 0..255: a row scale; 256..511: a column's scale and bias.
+    float s0, s1 = 0.0f;
+    if (tid < 256) {
+      s0 = p.sq[min(cur.m0 + tid, p.m - 1)];
+    } else {
+      const int col = min(cur.n0 + tid - 256, p.n - 1);
+      s0 = p.sw[col];
+      if (p.bias != nullptr) s1 = static_cast<float>(static_cast<const T*>(p.bias)[col]);
+    }
+    v4i acc[MI][NI];
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int j = 0; j < NI; ++j) acc[i][j] = v4i{0, 0, 0, 0};
+    Tile nxt = cur;
+    for (int kb = 0; kb < nkb; ++kb) {
+      wait_vm<0>();
+      lds_done_barrier();  // this stage has landed; every wave has read the one before (and the last tile's scales)
+      if (kb + 1 < nkb) {
+        issue(kb + 1, slot ^ C::kStage);
+      } else if (more) {
+        nxt = tile_at(t + t_stride);
+        load_tile(nxt);
+        issue(0, slot ^ C::kStage);
+      }
+      const char* const st = lds + slot;
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk) {
+        v4i a[MI], b[NI];
+#pragma unroll
+        for (int i = 0; i < MI; ++i) a[i] = *reinterpret_cast<const v4i*>(st + ((aoff + i * 2048) ^ (kk * 64)));
+#pragma unroll
+        for (int j = 0; j < NI; ++j) b[j] = *reinterpret_cast<const v4i*>(st + ((boff + j * 2048) ^ (kk * 64)));
+        if (ragged && kb == nkb - 1 && kk * 64 + (lane >> 4) * 16 >= (p.k & 127)) {
+#pragma unroll
+          for (int i = 0; i < MI; ++i) a[i] = v4i{0, 0, 0, 0};
+        }
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+          for (int j = 0; j < NI; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(b[j], a[i], acc[i][j], 0, 0, 0);
+      }
+      if (kb == 0) {
+        sc[tid] = s0;
+        if (tid >= 256) sc[256 + tid] = s1;
+      }
+      slot ^= C::kStage;
+    }
+    if (nkb == 1) lds_done_barrier();  // the scales
+
+    // Epilogue: 16 rows x 64 columns at a time through the wave's own LDS rows to whole lines.
+    const int l = opaque_copy(lane);
+    const int lrow = l & 15, lcol = (l >> 4) * 4;
+    const int64_t mw = cur.m0 + wm * 64;
+    const int nw = cur.n0 + wn * 128;
+    T* const stage = reinterpret_cast<T*>(lds + C::kOut) + wave * 16 * C::kOutStride;
+    T* const y = static_cast<T*>(p.y);
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      float4 sw[4], bias[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float* const s = sc + 256 + wn * 128 + half * 64 + j * 16 + lcol;
+        sw[j] = *reinterpret_cast<const float4*>(s);
+        bias[j] = *reinterpret_cast<const float4*>(s + 256);
+      }
+      const int nh = nw + half * 64;
+#pragma unroll
+      for (int i = 0; i < MI; ++i) {
+        const int64_t row = mw + i * 16 + lrow;
+        const float sq = sc[wm * 64 + i * 16 + lrow];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float w4[4] = {sw[j].x, sw[j].y, sw[j].z, sw[j].w}, b4[4] = {bias[j].x, bias[j].y, bias[j].z, bias[j].w};
+          *reinterpret_cast<vec4<T>*>(stage + lrow * C::kOutStride + j * 16 + lcol) =
+              epi(acc[i][half * 4 + j], sq, w4, b4, row, nh + j * 16 + lcol);
+        }
+        __builtin_amdgcn_wave_barrier();
+        if (wide) {
+#pragma unroll
+          for (int s = 0; s < 2; ++s) {
+            const int r = s * 8 + (l >> 3), c = (l & 7) * 8;
+            const int64_t orow = mw + i * 16 + r;
+            // Past the L2, which the operands need: 248 -> 238 us at 6208 x 2048 x 16384.
+            if (orow < p.m && nh + c < p.n)
+              __builtin_nontemporal_store(*reinterpret_cast<const v4i*>(stage + r * C::kOutStride + c),
+                                          reinterpret_cast<v4i*>(y + orow * p.n + nh + c));
+          }
+        } else {
+          for (int e = l; e < 16 * 64; e += 64) {
+            const int r = e >> 6, c = e & 63;
+            const int64_t orow = mw + i * 16 + r;
+            if (orow < p.m && nh + c < p.n) y[orow * p.n + nh + c] = stage[r * C::kOutStride + c];
+          }
+        }
+        __builtin_amdgcn_wave_barrier();
+      }
+    }
+    if (!more) break;
+    t += t_stride;
+    cur = nxt;
+  }
+}
+
 // ------------------------------------------------------------------ few rows
-// A workgroup holds 16 MI rows and 32 columns; its four waves (and the ksplit workgroups of a
-// tile) each take a run of the 64-deep blocks of K.  The sums of the waves meet in LDS.
+// A workgroup holds 16 rows and 32 columns; its four waves (and the ksplit workgroups of a tile)
+// each take a run of the 64-deep blocks of K, eight blocks in flight.  Both operands go straight
+// into registers; the sums of the waves meet in LDS.
 constexpr int kStreamCols = 32;
 
-template <typename T, int MI>
+template <typename T>
 __global__ __launch_bounds__(256) void int8_stream_kernel(Int8GemmParams p) {
-  constexpr int NI = kStreamCols / 16, U = 4;
-  __shared__ v4i sums[3][MI * NI * 64];
+  constexpr int NI = kStreamCols / 16, U = 8;
+  __shared__ v4i sums[3][NI * 64];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n0 = blockIdx.x * kStreamCols;
-  const int64_t m0 = static_cast<int64_t>(blockIdx.z) * (16 * MI);
+  const int64_t m0 = static_cast<int64_t>(blockIdx.z) * 16;
   const int split = blockIdx.y;
   const int blocks = (p.k + 63) >> 6, parts = 4 * p.ksplit, part = 4 * split + wave;
   const int begin = static_cast<int>(static_cast<int64_t>(blocks) * part / parts);
   const int end = static_cast<int>(static_cast<int64_t>(blocks) * (part + 1) / parts);
   const int kl = (lane >> 4) * 16;  // this lane's k in a block
-  const int8_t* ap[MI];
+  const int8_t* const ap = p.q + min(m0 + (lane & 15), p.m - 1) * p.ldq;
   const int8_t* bp[NI];
 #pragma unroll
-  for (int i = 0; i < MI; ++i) ap[i] = p.q + min(m0 + i * 16 + (lane & 15), p.m - 1) * p.ldq;
-#pragma unroll
   for (int j = 0; j < NI; ++j) bp[j] = p.w + static_cast<int64_t>(min(n0 + j * 16 + (lane & 15), p.n - 1)) * p.ldw;
-  v4i acc[MI][NI];
+  v4i acc[NI];
 #pragma unroll
-  for (int i = 0; i < MI; ++i)
-#pragma unroll
-    for (int j = 0; j < NI; ++j) acc[i][j] = v4i{0, 0, 0, 0};
+  for (int j = 0; j < NI; ++j) acc[j] = v4i{0, 0, 0, 0};
 
   for (int kb = begin; kb < end; kb += U) {
-    v4i a[U][MI], b[U][NI];
+    v4i a[U], b[U][NI];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       // Blocks past the wave's last one, and chunks past K, read the row's last chunk; their
@@ -255,43 +555,33 @@ __global__ __launch_bounds__(256) void int8_stream_kernel(Int8GemmParams p) {
       const int k = min((kb + u) * 64 + kl, p.k - 16);
 #pragma unroll
       for (int j = 0; j < NI; ++j) b[u][j] = *reinterpret_cast<const v4i*>(bp[j] + k);
-#pragma unroll
-      for (int i = 0; i < MI; ++i) a[u][i] = *reinterpret_cast<const v4i*>(ap[i] + k);
+      a[u] = *reinterpret_cast<const v4i*>(ap + k);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const bool in = kb + u < end && (kb + u) * 64 + kl < p.k;
+      const v4i ai = in ? a[u] : v4i{0, 0, 0, 0};
 #pragma unroll
-      for (int i = 0; i < MI; ++i) {
-        const v4i ai = in ? a[u][i] : v4i{0, 0, 0, 0};
-#pragma unroll
-        for (int j = 0; j < NI; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(b[u][j], ai, acc[i][j], 0, 0, 0);
-      }
+      for (int j = 0; j < NI; ++j) acc[j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(b[u][j], ai, acc[j], 0, 0, 0);
     }
   }
   if (wave > 0) {
 #pragma unroll
-    for (int i = 0; i < MI; ++i)
-#pragma unroll
-      for (int j = 0; j < NI; ++j) sums[wave - 1][(i * NI + j) * 64 + lane] = acc[i][j];
+    for (int j = 0; j < NI; ++j) sums[wave - 1][j * 64 + lane] = acc[j];
   }
   __syncthreads();
+  if (wave != 0) return;
   const Epilogue<T> epi(p);
-  // Fragment f of the tile to wave f % 4; wave 0 holds its own sums in registers.
+  const int64_t row = m0 + (lane & 15);
+  if (row >= p.m) return;
 #pragma unroll
-  for (int f = 0; f < MI * NI; ++f) {
-    if (wave != 0) break;
-    v4i s = acc[f / NI][f % NI];
+  for (int j = 0; j < NI; ++j) {
+    v4i s = acc[j];
 #pragma unroll
-    for (int w = 0; w < 3; ++w) s += sums[w][f * 64 + lane];
-    const int64_t row = m0 + (f / NI) * 16 + (lane & 15);
-    const int64_t col = n0 + (f % NI) * 16 + (lane >> 4) * 4;
-    if (row >= p.m) continue;
+    for (int w = 0; w < 3; ++w) s += sums[w][j * 64 + lane];
+    const int64_t col = n0 + j * 16 + (lane >> 4) * 4;
     if (p.ksplit > 1) {
-      int32_t* const o = p.partial + (static_cast<int64_t>(split) * p.m + row) * p.n + col;
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (col + r < p.n) o[r] = s[r];
+      store_partial(p, s, split, row, col);
     } else {
       float sw[4], bias[4];
       epi.scales(col, sw, bias);
@@ -314,50 +604,76 @@ __global__ __launch_bounds__(256) void int8_reduce_kernel(Int8GemmParams p) {
   const int64_t plane = p.m * p.n;
   const int32_t* const s = p.partial + row * p.n + col;
   v4i acc{0, 0, 0, 0};
-  for (int k = 0; k < p.ksplit; ++k) {
+  if ((p.n & 3) == 0) {
+#pragma unroll 4
+    for (int k = 0; k < p.ksplit; ++k) acc += *reinterpret_cast<const v4i*>(s + k * plane);
+  } else {
+    for (int k = 0; k < p.ksplit; ++k) {
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-      if (col + r < p.n) acc[r] += s[k * plane + r];
+      for (int r = 0; r < 4; ++r)
+        if (col + r < p.n) acc[r] += s[k * plane + r];
+    }
   }
   const Epilogue<T> epi(p);
   float sw[4], bias[4];
   epi.scales(col, sw, bias);
   const vec4<T> o = epi(acc, p.sq[row], sw, bias, row, col);
   T* const y = static_cast<T*>(p.y) + row * p.n + col;
+  if ((p.n & 3) == 0) {
+    *reinterpret_cast<vec4<T>*>(y) = o;
+  } else {
 #pragma unroll
-  for (int r = 0; r < 4; ++r)
-    if (col + r < p.n) y[r] = o[r];
+    for (int r = 0; r < 4; ++r)
+      if (col + r < p.n) y[r] = o[r];
+  }
 }
 
-enum : int { kTile128 = 0, kTile64 = 1, kStream16 = 2, kStream32 = 3, kStream64 = 4 };
+enum : int { kTile128x64, kTile64, kStream, kBig };
 
-template <typename T, int BM, int BN, int WM, int WN, int ST>
+template <typename T>
+void launch_reduce(const Int8GemmParams& p, hipStream_t stream) {
+  if (p.ksplit <= 1) return;
+  const int64_t items = p.m * ((p.n + 3) / 4);
+  int8_reduce_kernel<T><<<dim3(static_cast<unsigned>((items + 255) / 256)), 256, 0, stream>>>(p);
+}
+
+template <typename T, int BM, int BN, int KW, int ST>
 void launch_tile(Int8GemmParams& p, hipStream_t stream) {
+  using C = Int8Tile<BM, BN, KW, ST>;
   p.mtiles = static_cast<int32_t>((p.m + BM - 1) / BM);
   p.ntiles = (p.n + BN - 1) / BN;
-  int8_tile_kernel<T, BM, BN, WM, WN, ST>
-      <<<dim3(static_cast<unsigned>(p.mtiles * p.ntiles)), 64 * Int8Tile<BM, BN, WM, WN, ST>::kWaves, 0, stream>>>(p);
+  int8_tile_kernel<T, BM, BN, KW, ST>
+      <<<dim3(static_cast<unsigned>(p.mtiles * p.ntiles * p.ksplit)), 64 * C::kWaves, C::kLds, stream>>>(p);
+  launch_reduce<T>(p, stream);
 }
 
-template <typename T, int MI>
+template <typename T>
+void launch_big(Int8GemmParams& p, hipStream_t stream) {
+  p.mtiles = static_cast<int32_t>((p.m + Int8Big::kTile - 1) / Int8Big::kTile);
+  p.ntiles = (p.n + Int8Big::kTile - 1) / Int8Big::kTile;
+  const int tiles = p.mtiles * p.ntiles, cus = device_cu_count();
+  const dim3 grid(static_cast<unsigned>(tiles < cus ? tiles : cus));
+  if (p.res != nullptr)
+    int8_big_kernel<T, true><<<grid, 512, Int8Big::kLds, stream>>>(p);
+  else
+    int8_big_kernel<T, false><<<grid, 512, Int8Big::kLds, stream>>>(p);
+}
+
+template <typename T>
 void launch_stream(const Int8GemmParams& p, hipStream_t stream) {
   const dim3 grid(static_cast<unsigned>((p.n + kStreamCols - 1) / kStreamCols), static_cast<unsigned>(p.ksplit),
-                  static_cast<unsigned>((p.m + 16 * MI - 1) / (16 * MI)));
-  int8_stream_kernel<T, MI><<<grid, 256, 0, stream>>>(p);
-  if (p.ksplit > 1) {
-    const int64_t items = p.m * ((p.n + 3) / 4);
-    int8_reduce_kernel<T><<<dim3(static_cast<unsigned>((items + 255) / 256)), 256, 0, stream>>>(p);
-  }
+                  static_cast<unsigned>((p.m + 15) / 16));
+  int8_stream_kernel<T><<<grid, 256, 0, stream>>>(p);
+  launch_reduce<T>(p, stream);
 }
 
 template <typename T>
 void launch(Int8GemmParams& p, const Int8GemmPlan& plan, hipStream_t stream) {
   switch (plan.tile) {
-    case kTile128: launch_tile<T, 128, 128, 64, 64, 2>(p, stream); break;
-    case kTile64: launch_tile<T, 64, 64, 32, 32, 3>(p, stream); break;
-    case kStream16: launch_stream<T, 1>(p, stream); break;
-    case kStream32: launch_stream<T, 2>(p, stream); break;
-    default: launch_stream<T, 4>(p, stream); break;
+    case kTile128x64: launch_tile<T, 128, 64, 2, 3>(p, stream); break;
+    case kBig: launch_big<T>(p, stream); break;
+    case kTile64: launch_tile<T, 64, 64, 4, 3>(p, stream); break;
+    default: launch_stream<T>(p, stream); break;
   }
 }
 
@@ -366,15 +682,40 @@ void launch(Int8GemmParams& p, const Int8GemmPlan& plan, hipStream_t stream) {
 Int8GemmPlan int8_gemm_plan(int64_t m, int32_t n, int32_t k, int cus) {
   Int8GemmPlan plan{};
   plan.ksplit = 1;
-  if (m <= 64) {
-    plan.tile = m <= 16 ? kStream16 : m <= 32 ? kStream32 : kStream64;
-    // K slices until every CU has two workgroups, each wave with at least four 64-deep blocks.
+  if (m <= 16) {
+    // K slices until every CU has a workgroup, each wave at least eight 64-deep blocks (one row, us
+    // with 1 / 2 / 4 / 8 slices: 2048 deep and 2560 columns 5.9 / 6.4 / 7.1 / -, 16384 and 2048 columns
+    // 20.2 / 13.9 / 10.7 / 11.6).  From 17 rows on the 64 x 64 tiles are faster (32 rows 15.3 / 12.8,
+    // 64 rows 20.3 / 13.3 at 16384 deep; 64 rows x 16384 columns 20.7 / 10.7).
+    plan.tile = kStream;
     const int64_t tiles = (n + kStreamCols - 1) / kStreamCols;
-    while (plan.ksplit < 16 && tiles * plan.ksplit < 2 * cus && k / (plan.ksplit * 2) >= 4 * 4 * 64) plan.ksplit *= 2;
+    while (plan.ksplit < 16 && tiles * plan.ksplit < cus && k / (plan.ksplit * 2) >= 4 * 8 * 64) plan.ksplit *= 2;
     return plan;
   }
-  const int64_t big = ((m + 127) / 128) * ((n + 127) / 128);
-  plan.tile = big >= cus ? kTile128 : kTile64;
+  // The least of the times (us, beside a launch) that these measurements give, 128 bytes of K a step
+  // and w workgroups on the CUs: 64 x 64 tiles 0.25 a step and workgroup of a CU (2048 deep, 2560
+  // columns: 200 rows 8.7 us, 1500 rows 20.2), 128 x 64 tiles 0.36 (10.9, 15.7), 256 x 256 tiles 1.4 a
+  // step and round of CUs, and 2 for their longer ends (27.2, 28.0; 776 rows x 16384 columns 31.4 us,
+  // against 54.4 and 49.6).  A K slice shortens the steps and costs the sums' way through memory.
+  const double steps = (k + 127) / 128;
+  double best = 1e30;
+  auto consider = [&](int tile, int64_t w, double step_us, int ks) {
+    const double load = static_cast<double>(w) * ks / cus;
+    const double us = (steps / ks) * step_us * (load < 1 ? 1 : load) +
+                      (ks > 1 ? 3.0 + static_cast<double>(m) * n * (8.0 * ks + 2) / 5e6 : 0.0);
+    if (us < best) {
+      best = us;
+      plan.tile = tile;
+      plan.ksplit = ks;
+    }
+  };
+  for (int ks = 1; ks <= 8; ks *= 2) {
+    if (ks > 1 && steps / ks < 8) break;
+    consider(kTile64, ((m + 63) / 64) * ((n + 63) / 64), 0.25, ks);
+    consider(kTile128x64, ((m + 127) / 128) * ((n + 63) / 64), 0.36, ks);
+  }
+  const int64_t big = ((m + 255) / 256) * ((n + 255) / 256);
+  if (2.0 + steps * 1.4 * static_cast<double>((big + cus - 1) / cus) < best) plan = {kBig, 1};
   return plan;
 }
 
