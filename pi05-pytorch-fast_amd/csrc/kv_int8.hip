@@ -5,8 +5,8 @@
 // attention computes S^T = K Q^T and O^T = V^T P^T on 16-row matrix instructions whose operands
 // are 16-byte loads of consecutive codes of either array: no transposes, no LDS for the cache.
 
+#include "direct_load.h"
 #include "int8_internal.h"
-#include "quant_row.h"
 
 namespace w4a4 {
 namespace {
@@ -34,9 +34,11 @@ __device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) {
 // tokens (lens -> table -> scale, one after the other) and by HBM for prefixes.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void kv_append_kernel(KvAppendParams p) {
-  constexpr int kChunks = kKvPage * D / 8 / 256;  // 8-element chunks of a thread
-  constexpr int kRowChunks = D / 8;
-  constexpr int kStride = kKvPage + 4;            // staged V row (one d), bytes
+  // A thread holds kRows consecutive page rows of eight consecutive dimensions, so that a V row (one
+  // dimension) takes its kRows codes in one LDS write.
+  constexpr int kRows = kKvPage * D / 8 / 256, kRowChunks = D / 8;
+  constexpr int kStride = kKvPage + 8;            // staged V row, bytes
+  constexpr int kGroups = D * 4 / 256;            // 16-token groups of V rows that a thread writes
   __shared__ uint32_t red[4];
   __shared__ __align__(16) char vt[D * kStride];
   const int tid = threadIdx.x;
@@ -46,31 +48,35 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvAppendParams p) {
   const int64_t len = max(p.c.lens[b], 0);
   const int64_t count = min(max(p.counts != nullptr ? p.counts[b] : p.t, 0), p.t);
   const int64_t slot = len / kKvPage + blockIdx.x;
-  const int64_t first = max(len - slot * kKvPage, static_cast<int64_t>(0));  // new tokens: page rows first .. last - 1
-  const int64_t last = min(len + count - slot * kKvPage, static_cast<int64_t>(kKvPage));
-  if (last <= first || slot >= p.c.table_pages) return;
+  const int64_t tok0 = slot * kKvPage - len;  // token of page row 0
+  if (tok0 >= count || slot >= p.c.table_pages) return;
+  const int first = static_cast<int>(max(-tok0, static_cast<int64_t>(0)));  // new tokens: page rows first .. last - 1
+  const int last = static_cast<int>(min(count - tok0, static_cast<int64_t>(kKvPage)));
+  if (last <= first) return;
   const int page = p.c.table[b * p.c.table_stride + slot];
   if (page < 0 || page >= p.c.pages) return;
   const int64_t ph = static_cast<int64_t>(page) * p.c.kvh + head;
   const int64_t* const st = is_v ? p.v_stride : p.k_stride;
   const T* const src = static_cast<const T*>(is_v ? p.v : p.k) + b * st[0] + head * st[2];
-  const int64_t tok0 = slot * kKvPage - len;  // token of page row 0
+  const int row0 = tid / kRowChunks * kRows, d0 = (tid % kRowChunks) * 8;
 
-  vec8<T> x[kChunks];
+  vec8<T> x[kRows];
   uint32_t top = 0;
 #pragma unroll
-  for (int j = 0; j < kChunks; ++j) {
-    const int c = j * 256 + tid, row = c / kRowChunks;
+  for (int j = 0; j < kRows; ++j) {
+    const int row = row0 + j;
     x[j] = vec8<T>{};
-    if (row >= first && row < last) x[j] = *reinterpret_cast<const vec8<T>*>(src + (tok0 + row) * st[1] + (c % kRowChunks) * 8);
+    if (row >= first && row < last) x[j] = *reinterpret_cast<const vec8<T>*>(src + (tok0 + row) * st[1] + d0);
+  }
+  float* const scale = (is_v ? p.c.vs : p.c.ks) + ph;
+  const float s0 = first > 0 ? *scale : 0.0f;
+#pragma unroll
+  for (int j = 0; j < kRows; ++j)
 #pragma unroll
     for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(static_cast<float>(x[j][e])) & 0x7fffffffu);
-  }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), o, 64)));
   if ((tid & 63) == 0) red[tid >> 6] = top;
-  float* const scale = (is_v ? p.c.vs : p.c.ks) + ph;
-  const float s0 = first > 0 ? *scale : 0.0f;
   __syncthreads();  // also: every thread has read the old scale
   top = max(max(red[0], red[1]), max(red[2], red[3]));
   const float amax = __uint_as_float(top);
@@ -83,9 +89,9 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvAppendParams p) {
   const float inv = finite ? 1.0f / s : 0.0f;
   const float ratio = finite && first > 0 ? s0 / s : 0.0f;
 
-  uint32_t code[kChunks][2];
+  uint32_t code[kRows][2];
 #pragma unroll
-  for (int j = 0; j < kChunks; ++j) {
+  for (int j = 0; j < kRows; ++j) {
     float f[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) f[e] = finite ? fmaf(static_cast<float>(x[j][e]), inv, kRintMagic) : kRintMagic;
@@ -98,53 +104,71 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvAppendParams p) {
     for (int e = 0; e < 4; ++e) f[e] = fmaf(static_cast<float>(static_cast<int8_t>(w >> (8 * e))), ratio, kRintMagic);
     return pack4(f[0], f[1], f[2], f[3]);
   };
+  const bool keep = first > 0;  // the page has tokens of before
   if (!is_v) {
-    char* const dst = reinterpret_cast<char*>(p.c.k) + ph * (kKvPage * D);
+    char* const dst = reinterpret_cast<char*>(p.c.k) + ph * (kKvPage * D) + row0 * D + d0;
+    uint2 old[kRows];
 #pragma unroll
-    for (int j = 0; j < kChunks; ++j) {
-      const int c = j * 256 + tid, row = c / kRowChunks;
-      uint2* const d = reinterpret_cast<uint2*>(dst + c * 8);
-      if (row >= first && row < last)
-        *d = uint2{code[j][0], code[j][1]};
-      else if (first == 0)
-        *d = uint2{0u, 0u};
-      else if (grow) {
-        const uint2 o = *d;
-        *d = uint2{rescaled(o.x), rescaled(o.y)};
-      }
+    for (int j = 0; j < kRows; ++j) {
+      const bool fresh = row0 + j >= first && row0 + j < last;
+      old[j] = uint2{0u, 0u};
+      if (!fresh && keep && grow) old[j] = *reinterpret_cast<const uint2*>(dst + j * D);
+    }
+#pragma unroll
+    for (int j = 0; j < kRows; ++j) {
+      const bool fresh = row0 + j >= first && row0 + j < last;
+      if (fresh)
+        *reinterpret_cast<uint2*>(dst + j * D) = uint2{code[j][0], code[j][1]};
+      else if (!keep || grow)
+        *reinterpret_cast<uint2*>(dst + j * D) = keep ? uint2{rescaled(old[j].x), rescaled(old[j].y)} : uint2{0u, 0u};
     }
     return;
   }
-  // V: the new codes are turned in LDS; each thread then owns 16 tokens of one d at a time.
+  // V: the new codes are turned in LDS; each thread then writes 16 tokens of one dimension at a time.
 #pragma unroll
-  for (int j = 0; j < kChunks; ++j) {
-    const int c = j * 256 + tid, row = c / kRowChunks, d0 = (c % kRowChunks) * 8;
+  for (int e = 0; e < 8; ++e) {
+    uint32_t w[2] = {0u, 0u};
 #pragma unroll
-    for (int e = 0; e < 8; ++e) vt[(d0 + e) * kStride + row] = static_cast<char>(code[j][e >> 2] >> (8 * (e & 3)));
+    for (int j = 0; j < kRows; ++j) w[j >> 2] |= ((code[j][e >> 2] >> (8 * (e & 3))) & 0xffu) << (8 * (j & 3));
+    char* const o = vt + (d0 + e) * kStride + row0;
+    if constexpr (kRows == 8) *reinterpret_cast<uint2*>(o) = uint2{w[0], w[1]};
+    else if constexpr (kRows == 4) *reinterpret_cast<uint32_t*>(o) = w[0];
+    else *reinterpret_cast<uint16_t*>(o) = static_cast<uint16_t>(w[0]);
   }
   __syncthreads();
   char* const dst = reinterpret_cast<char*>(p.c.v) + ph * (kKvPage * D);
-  for (int i = tid; i < D * (kKvPage / 4); i += 256) {
-    const int d = i / (kKvPage / 4), t0 = (i % (kKvPage / 4)) * 4;
-    if (!grow && (t0 + 4 <= first || t0 >= last)) continue;
-    uint32_t* const o = reinterpret_cast<uint32_t*>(dst + d * kKvPage + t0);
-    const uint32_t fresh = *reinterpret_cast<const uint32_t*>(vt + d * kStride + t0);
-    uint32_t old = 0;
-    if (first > 0 && (t0 < first || t0 + 4 > last)) old = grow ? rescaled(*o) : *o;
-    uint32_t w = 0;
+  v4i old[kGroups];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const uint32_t m = 0xffu << (8 * e);
-      w |= (t0 + e >= first && t0 + e < last ? fresh : old) & m;
+  for (int i = 0; i < kGroups; ++i) {
+    const int at = i * 256 + tid, t0 = (at & 3) * 16;
+    old[i] = v4i{0, 0, 0, 0};
+    if (keep && (grow || (t0 + 16 > first && t0 < last))) old[i] = *reinterpret_cast<const v4i*>(dst + at * 16);
+  }
+#pragma unroll
+  for (int i = 0; i < kGroups; ++i) {
+    const int at = i * 256 + tid, d = at >> 2, t0 = (at & 3) * 16;
+    if (!grow && (t0 + 16 <= first || t0 >= last)) continue;
+    v4i out;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const uint32_t fresh = *reinterpret_cast<const uint32_t*>(vt + d * kStride + t0 + 4 * q);
+      const uint32_t was = grow && keep ? rescaled(static_cast<uint32_t>(old[i][q])) : static_cast<uint32_t>(old[i][q]);
+      uint32_t m = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (t0 + 4 * q + e >= first && t0 + 4 * q + e < last) m |= 0xffu << (8 * e);
+      out[q] = static_cast<int>((fresh & m) | (was & ~m));
     }
-    *o = w;
+    *reinterpret_cast<v4i*>(dst + at * 16) = out;
   }
 }
 
 // ------------------------------------------------------------------ attention
-// A workgroup holds 16 query rows of one KV head (row = token * (H / KVH) + query head) and a run
-// of the sequence's pages; its four waves take every fourth page of the run, each with a softmax
-// of its own (running maximum and sum), and meet in LDS at the end.
+// Two kernels.  kv_attn_kernel: 16 query rows of one KV head (row = token * (H / KVH) + query
+// head) and a run of the sequence's pages a workgroup, whose eight waves take every eighth page,
+// each with a softmax of its own (running maximum and sum), and meet in LDS at the end: decoded
+// tokens, where the cache is read once and its bytes bound.  kv_attn_wide_kernel: 128 rows, 32 a
+// wave, over pages that the waves share in LDS: chunks of tokens.
 //
 // Q K^T in int8: a query row is held as 16-bit integers v = rint(q / sq), |v| <= 32512, split
 // v = 256 hi + lo into two int8 operands, so that S = sq ks (256 K hi + K lo) is exact but for
@@ -153,19 +177,16 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvAppendParams p) {
 // w = 2^(S log2e + log2 vs - m) with m the running maximum of that sum, so that the weights of
 // all pages share one accumulator and stay at most 1; the sum of the probabilities is that of
 // w / vs.  Sums, maxima and accumulators are fp32; w is rounded to fp16 (2^-11) for the product.
-//
-// Lane L of a 16 x 16 S^T tile holds row L % 16 and four consecutive tile rows 4 (L / 16) ..  Tile
-// t's row 4 a + r is key 16 a + 4 t + r, so that over the four tiles of a page the lane holds
-// keys 16 (L / 16) .. + 15: the 16 bytes that it loads of a V row.
-template <typename T, int D>
-__device__ __forceinline__ void load_query(const T* row, float& sq, v4i (&hi)[D / 64], v4i (&lo)[D / 64], int g) {
-  float f[D / 64][16];
+template <typename T, int D, int STEP>
+__device__ __forceinline__ void load_query(const T* row, float& sq, v4i (&hi)[D / STEP], v4i (&lo)[D / STEP], int g) {
+  // The lane's 16 elements at 16 g of every STEP; the row's lanes are those with the same lane % (1024 / STEP).
+  float f[D / STEP][16];
   uint32_t top = 0;
 #pragma unroll
-  for (int i = 0; i < D / 64; ++i) {
+  for (int i = 0; i < D / STEP; ++i) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const vec8<T> v = *reinterpret_cast<const vec8<T>*>(row + 64 * i + 16 * g + 8 * h);
+      const vec8<T> v = *reinterpret_cast<const vec8<T>*>(row + STEP * i + 16 * g + 8 * h);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         f[i][8 * h + e] = static_cast<float>(v[e]);
@@ -173,31 +194,31 @@ __device__ __forceinline__ void load_query(const T* row, float& sq, v4i (&hi)[D 
       }
     }
   }
-  top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 16, 64)));
+  if constexpr (STEP == 64) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 16, 64)));
   top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 32, 64)));
   const float amax = __uint_as_float(top);
   const bool finite = amax <= 3.4028235e38f;
   sq = finite ? amax / 32512.0f : __builtin_nanf("");
   const float inv = finite && amax >= 1e-30f ? 32512.0f / amax : 0.0f;
+  // v + 1.5 * 2^23 holds v in its low 16 bits: lo is the low byte as it is, hi the next one after adding 128.
 #pragma unroll
-  for (int i = 0; i < D / 64; ++i) {
+  for (int i = 0; i < D / STEP; ++i) {
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      uint32_t ph = 0, pl = 0;
+      uint32_t v[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int v = finite ? static_cast<int>(__builtin_rintf(f[i][4 * w + e] * inv)) : 0;
-        const int h = (v + 128) >> 8;
-        ph |= static_cast<uint32_t>(h & 0xff) << (8 * e);
-        pl |= static_cast<uint32_t>((v - 256 * h) & 0xff) << (8 * e);
-      }
-      hi[i][w] = static_cast<int>(ph);
-      lo[i][w] = static_cast<int>(pl);
+      for (int e = 0; e < 4; ++e) v[e] = __float_as_uint(finite ? fmaf(f[i][4 * w + e], inv, kRintMagic) : kRintMagic);
+      lo[i][w] = static_cast<int>(__builtin_amdgcn_perm(__builtin_amdgcn_perm(v[3], v[2], 0x0c0c0400u),
+                                                        __builtin_amdgcn_perm(v[1], v[0], 0x0c0c0400u), 0x05040100u));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] += 128u;
+      hi[i][w] = static_cast<int>(__builtin_amdgcn_perm(__builtin_amdgcn_perm(v[3], v[2], 0x0c0c0501u),
+                                                        __builtin_amdgcn_perm(v[1], v[0], 0x0c0c0501u), 0x05040100u));
     }
   }
 }
 
-// Four codes as fp16: byte + 128 under the exponent of 1024, less 1152.
+// Eight codes as fp16: byte + 128 under the exponent of 1024, less 1152.
 typedef _Float16 half2 __attribute__((ext_vector_type(2)));
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 __device__ __forceinline__ half8 codes_to_half(int w0, int w1) {
@@ -218,15 +239,76 @@ __device__ __forceinline__ half8 codes_to_half(int w0, int w1) {
 }
 
 constexpr float kNone = -1e30f;  // running maximum before the first visible key
+// The running maximum follows the largest score only when that is 2^kSlack larger: weights are then
+// at most 2^kSlack, well inside fp16, and the accumulators are rescaled once or twice a run.
+constexpr float kSlack = 8.0f;
+
+// A load at a uniform address that nothing in the kernel writes: through the scalar cache, so that
+// no wait for vector loads stands before its use.
+template <typename U>
+__device__ __forceinline__ U scalar_load(const U* p) {
+  return *reinterpret_cast<const __attribute__((address_space(4))) U*>(reinterpret_cast<uintptr_t>(p));
+}
 
 // Partial results of a run: O (unnormalised, fp32), the maximum and the sum of each row.
 __host__ __device__ inline int64_t split_floats(int64_t rows, int d) { return rows * (d + 2); }
 
+// What a workgroup's rows see.  ROWS query rows of a KV head from row0 on; a lane's row is given.
+struct Span {
+  int64_t q_len, len;
+  int causal;
+  __device__ __forceinline__ Span(const KvAttnParams& p, int b) {
+    const int64_t cap = static_cast<int64_t>(p.c.table_pages) * kKvPage;
+    len = p.c.pages > 0 ? min(static_cast<int64_t>(max(p.c.lens[b], 0)), cap) : 0;
+    q_len = min(max(p.q_lens != nullptr ? p.q_lens[b] : p.t, 0), p.t);
+    causal = p.causal;
+  }
+  // Tokens that query `token` sees: none past q_len.
+  __device__ __forceinline__ int64_t seen(int64_t token) const {
+    return token >= q_len ? static_cast<int64_t>(0) : causal ? max(len - q_len + token + 1, static_cast<int64_t>(0)) : len;
+  }
+  // The most that any of the tokens first .. last sees, and what all of them do.
+  __device__ __forceinline__ int64_t most(int64_t first, int64_t last) const { return seen(min(last, max(q_len - 1, first))); }
+  __device__ __forceinline__ int64_t least(int64_t first, int64_t last) const { return last < q_len ? seen(first) : 0; }
+};
+
+// The end of a row: its output, or its part of a run's partial results.  v: columns 4 consecutive from c.
+template <typename T>
+__device__ __forceinline__ void store_quad(const KvAttnParams& p, const v4f v, float inv, int split, int64_t orow, int d, int c) {
+  if (p.nsplit > 1) {
+    const int64_t all_rows = static_cast<int64_t>(p.b) * p.t * p.h;
+    *reinterpret_cast<v4f*>(p.ws + split * split_floats(all_rows, d) + orow * d + c) = v;
+  } else {
+    typedef T tv4 __attribute__((ext_vector_type(4)));
+    tv4 y;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) y[r] = static_cast<T>(inv == 0.0f ? 0.0f : v[r] * inv);
+    *reinterpret_cast<tv4*>(static_cast<T*>(p.out) + orow * d + c) = y;
+  }
+}
+__device__ __forceinline__ void store_sums(const KvAttnParams& p, float m, float l, int split, int64_t orow, int d) {
+  if (p.nsplit > 1) {
+    const int64_t all_rows = static_cast<int64_t>(p.b) * p.t * p.h;
+    float* const ml = p.ws + split * split_floats(all_rows, d) + all_rows * d + orow * 2;
+    ml[0] = m;
+    ml[1] = l;
+  } else if (p.lse != nullptr) {
+    p.lse[orow] = l == 0.0f ? -__builtin_inff() : m / kLog2e + __builtin_logf(l);
+  }
+}
+
+// Lane L of a 16 x 16 S^T tile holds row L % 16 and four consecutive tile rows 4 (L / 16) ..  Tile
+// t's row 4 a + r is key 16 a + 4 t + r, so that over the four tiles of a page the lane holds
+// keys 16 (L / 16) .. + 15: the 16 bytes that it loads of a V row.
+// A page's values are requested before its scores, the next page's keys as the values are used up.
+constexpr int kAttnWaves = 8;
+
 template <typename T, int D>
-__global__ __launch_bounds__(256) void kv_attn_kernel(KvAttnParams p) {
-  constexpr int F = D / 64, DT = D / 16;
-  __shared__ v4f obuf[3][DT * 64];
-  __shared__ float mbuf[4][16], lbuf[4][16];
+__global__ __launch_bounds__(64 * kAttnWaves, 2) void kv_attn_kernel(KvAttnParams p) {
+  constexpr int F = D / 64, DT = D / 16, W = kAttnWaves;
+  static_assert(DT == 4 * F, "a key load for each tile of values");
+  extern __shared__ __align__(16) v4f obuf[];  // [W][DT][64]
+  __shared__ float mbuf[W][16], lbuf[W][16];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, col = lane & 15;
@@ -235,30 +317,22 @@ __global__ __launch_bounds__(256) void kv_attn_kernel(KvAttnParams p) {
   const int tiles = (rows + 15) >> 4;
   const int tile = blockIdx.x % tiles, split = blockIdx.x / tiles;
   const int head = blockIdx.y, b = blockIdx.z;
-  const int64_t cap = static_cast<int64_t>(p.c.table_pages) * kKvPage;
-  const int64_t len = min(static_cast<int64_t>(max(p.c.lens[b], 0)), cap);
-  const int64_t q_len = min(max(p.q_lens != nullptr ? p.q_lens[b] : p.t, 0), p.t);
+  const Span span(p, b);
 
   // This lane's row; rows past the last one, and tokens past q_len, see nothing.
   const int row = tile * 16 + col;
   const int tok = min(row / group, p.t - 1), qh = head * group + row % group;
-  auto visible = [&](int64_t token) {
-    return token >= q_len ? static_cast<int64_t>(0) : p.causal ? max(len - q_len + token + 1, static_cast<int64_t>(0)) : len;
-  };
-  const int64_t seen = row < rows ? visible(row / group) : 0;
-  // Keys that the tile's rows see: those of its last token (of none, if that is past q_len and
-  // so are all the others').
+  const int64_t seen = row < rows ? span.seen(row / group) : 0;
   const int64_t tok_first = tile * 16 / group, tok_last = min(tile * 16 + 15, rows - 1) / group;
-  const int64_t most = visible(min(tok_last, max(q_len - 1, tok_first)));
-  const int64_t least = tile * 16 + 15 < rows && tok_last < q_len ? visible(tok_first) : 0;
-  const int pages = static_cast<int>((most + kKvPage - 1) / kKvPage);
+  const int64_t least = tile * 16 + 15 < rows ? span.least(tok_first, tok_last) : 0;
+  const int pages = static_cast<int>((span.most(tok_first, tok_last) + kKvPage - 1) / kKvPage);
   const int per = (pages + p.nsplit - 1) / p.nsplit;
   const int begin = split * per, end = min(begin + per, pages);
 
   float sq;
   v4i qhi[F], qlo[F];
   const T* const qrow = static_cast<const T*>(p.q) + b * p.q_stride[0] + tok * p.q_stride[1] + qh * p.q_stride[2];
-  load_query<T, D>(qrow, sq, qhi, qlo, g);
+  load_query<T, D, 64>(qrow, sq, qhi, qlo, g);
   const float qfac = sq * p.scaling * kLog2e;
 
   float m = kNone, l = 0.0f;
@@ -266,21 +340,29 @@ __global__ __launch_bounds__(256) void kv_attn_kernel(KvAttnParams p) {
 #pragma unroll
   for (int i = 0; i < DT; ++i) o[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
 
+  // Entries that name no page are read as page 0, whose keys then count as not there.
   const int32_t* const table = p.c.table + b * p.c.table_stride;
-  for (int pg = begin + wave; pg < end; pg += 4) {
-    const int page = table[pg];
-    if (page < 0 || page >= p.c.pages) continue;  // no such page: its keys are not there
-    const int64_t ph = static_cast<int64_t>(page) * p.c.kvh + head;
-    const int8_t* const kp = p.c.k + ph * (kKvPage * D) + (16 * (col >> 2) + (col & 3)) * D + 16 * g;
-    const int8_t* const vp = p.c.v + ph * (kKvPage * D) + col * kKvPage + 16 * g;
-    const float ks = p.c.ks[ph];
-    float vs = p.c.vs[ph];
+  const int64_t koff = (16 * (col >> 2) + (col & 3)) * D + 16 * g, voff = col * kKvPage + 16 * g;
+  auto page_at = [&](int pg) { return pg < end ? scalar_load(table + __builtin_amdgcn_readfirstlane(pg)) : -1; };
+  auto place = [&](int page) {
+    return static_cast<int64_t>(__builtin_amdgcn_readfirstlane(page >= 0 && page < p.c.pages ? page : 0)) * p.c.kvh + head;
+  };
+  v4i kc[4][F];
+  auto load_key = [&](const int8_t* kp, int i) { kc[i / F][i % F] = *reinterpret_cast<const v4i*>(kp + 4 * (i / F) * D + 64 * (i % F)); };
+  int page = page_at(begin + wave);
+  if (begin + wave < end) {
+#pragma unroll
+    for (int i = 0; i < 4 * F; ++i) load_key(p.c.k + place(page) * (kKvPage * D) + koff, i);
+  }
+  for (int pg = begin + wave; pg < end; pg += W) {
+    const int64_t ph = place(page);
+    const bool there = page >= 0 && page < p.c.pages;
+    const int next = page_at(pg + W);
+    const int8_t* const vp = p.c.v + ph * (kKvPage * D) + voff;
+    const float ks = scalar_load(p.c.ks + ph);
+    float vs = scalar_load(p.c.vs + ph);
     if (vs == 0.0f) vs = 1e-30f;  // zeros, whatever the codes: the page still counts in the sum
-    v4i kc[4][F], vc[DT];
-#pragma unroll
-    for (int t = 0; t < 4; ++t)
-#pragma unroll
-      for (int f = 0; f < F; ++f) kc[t][f] = *reinterpret_cast<const v4i*>(kp + 4 * t * D + 64 * f);
+    v4i vc[DT];
 #pragma unroll
     for (int i = 0; i < DT; ++i) vc[i] = *reinterpret_cast<const v4i*>(vp + 16 * i * kKvPage);
 
@@ -295,15 +377,16 @@ __global__ __launch_bounds__(256) void kv_attn_kernel(KvAttnParams p) {
         al = __builtin_amdgcn_mfma_i32_16x16x64_i8(kc[t][f], qlo[f], al, 0, 0, 0);
       }
 #pragma unroll
-      for (int r = 0; r < 4; ++r) s[t][r] = static_cast<float>(256 * ah[r] + al[r]) * fac + lvs;
+      for (int r = 0; r < 4; ++r) s[t][r] = fmaf(static_cast<float>(256 * ah[r] + al[r]), fac, lvs);
     }
     const int64_t key0 = static_cast<int64_t>(pg) * kKvPage;
-    if (key0 + kKvPage > least) {  // some row does not see the whole page
+    const int64_t limit = there ? seen : 0;
+    if (!there || key0 + kKvPage > least) {  // some row does not see the whole page
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          if (key0 + 16 * g + 4 * t + r >= seen) s[t][r] = -__builtin_inff();
+          if (key0 + 16 * g + 4 * t + r >= limit) s[t][r] = -__builtin_inff();
     }
     float top = s[0][0];
 #pragma unroll
@@ -312,78 +395,280 @@ __global__ __launch_bounds__(256) void kv_attn_kernel(KvAttnParams p) {
       for (int r = 0; r < 4; ++r) top = fmaxf(top, s[t][r]);
     top = fmaxf(top, __shfl_xor(top, 16, 64));
     top = fmaxf(top, __shfl_xor(top, 32, 64));
-    const float m1 = fmaxf(m, top);
-    const float alpha = __builtin_amdgcn_exp2f(m - m1);
-    m = m1;
+    if (__any(top > m + kSlack)) {
+      const float m1 = fmaxf(m, top);
+      const float alpha = __builtin_amdgcn_exp2f(m - m1);
+      m = m1;
+      l *= alpha;
+#pragma unroll
+      for (int i = 0; i < DT; ++i) o[i] *= alpha;
+    }
     float sum = 0.0f;
     half8 w[2];
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const float e = __builtin_amdgcn_exp2f(s[t][r] - m1);
+        const float e = __builtin_amdgcn_exp2f(s[t][r] - m);
         sum += e;
         w[t >> 1][4 * (t & 1) + r] = static_cast<_Float16>(e);
       }
     // A row that sees nothing of the page takes nothing from its scale either (it may be NaN).
-    l = l * alpha + (sum != 0.0f ? sum / vs : 0.0f);
+    l += sum != 0.0f ? sum / vs : 0.0f;
+    // The next page's keys take the registers of the values as these are used (past the last page:
+    // this one's again, not used).
+    const int8_t* const kn = p.c.k + (pg + W < end ? place(next) : ph) * (kKvPage * D) + koff;
 #pragma unroll
     for (int i = 0; i < DT; ++i) {
-      o[i] *= alpha;
       o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes_to_half(vc[i][0], vc[i][1]), w[0], o[i], 0, 0, 0);
       o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes_to_half(vc[i][2], vc[i][3]), w[1], o[i], 0, 0, 0);
+      load_key(kn, i);
+      __builtin_amdgcn_sched_barrier(0);
     }
+    page = next;
   }
   l += __shfl_xor(l, 16, 64);
   l += __shfl_xor(l, 32, 64);
 
-  // The four waves' parts: a common maximum, then the sums of the scaled parts.
+  // The waves' parts meet in LDS, scaled to a common maximum; each wave sums and finishes DT / W tiles
+  // of dimensions.
   if (g == 0) {
     mbuf[wave][col] = m;
     lbuf[wave][col] = l;
   }
   __syncthreads();
-  const float mall = fmaxf(fmaxf(mbuf[0][col], mbuf[1][col]), fmaxf(mbuf[2][col], mbuf[3][col]));
+  float mall = mbuf[0][col];
+#pragma unroll
+  for (int w = 1; w < W; ++w) mall = fmaxf(mall, mbuf[w][col]);
   const float mine = __builtin_amdgcn_exp2f(m - mall);
 #pragma unroll
-  for (int i = 0; i < DT; ++i) {
-    o[i] *= mine;
-    if (wave > 0) obuf[wave - 1][i * 64 + lane] = o[i];
-  }
-  __syncthreads();
-  if (wave != 0) return;
+  for (int i = 0; i < DT; ++i) obuf[(wave * DT + i) * 64 + lane] = o[i] * mine;
   float lall = 0.0f;
 #pragma unroll
-  for (int w = 0; w < 4; ++w) lall += lbuf[w][col] * __builtin_amdgcn_exp2f(mbuf[w][col] - mall);
-  const int64_t all_rows = static_cast<int64_t>(p.b) * p.t * p.h;
-  const int64_t orow = (static_cast<int64_t>(b) * p.t + tok) * p.h + qh;
-  const float inv = lall != 0.0f ? 1.0f / lall : 0.0f;
-  const bool empty = lall == 0.0f;  // no visible key (false for NaN)
+  for (int w = 0; w < W; ++w) lall += lbuf[w][col] * __builtin_amdgcn_exp2f(mbuf[w][col] - mall);
+  __syncthreads();
   if (row >= rows) return;
+  const int64_t orow = (static_cast<int64_t>(b) * p.t + tok) * p.h + qh;
+  const float inv = lall != 0.0f ? 1.0f / lall : 0.0f;  // 0: no visible key (NaN stays NaN)
+  for (int i = wave; i < DT; i += W) {
+    v4f v = obuf[i * 64 + lane];
 #pragma unroll
-  for (int i = 0; i < DT; ++i) {
-    v4f v = o[i];
-#pragma unroll
-    for (int w = 0; w < 3; ++w) v += obuf[w][i * 64 + lane];
-    if (p.nsplit > 1) {
-      *reinterpret_cast<v4f*>(p.ws + split * split_floats(all_rows, D) + orow * D + 16 * i + 4 * g) = v;
-    } else {
-      typedef T tv4 __attribute__((ext_vector_type(4)));
-      tv4 y;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) y[r] = static_cast<T>(empty ? 0.0f : v[r] * inv);
-      *reinterpret_cast<tv4*>(static_cast<T*>(p.out) + orow * D + 16 * i + 4 * g) = y;
-    }
+    for (int w = 1; w < W; ++w) v += obuf[(w * DT + i) * 64 + lane];
+    store_quad<T>(p, v, inv, split, orow, D, 16 * i + 4 * g);
   }
-  if (g == 0) {
-    if (p.nsplit > 1) {
-      float* const ml = p.ws + split * split_floats(all_rows, D) + all_rows * D + orow * 2;
-      ml[0] = mall;
-      ml[1] = lall;
-    } else if (p.lse != nullptr) {
-      p.lse[orow] = empty ? -__builtin_inff() : mall / kLog2e + __builtin_logf(lall);
-    }
+  if (wave == 0 && g == 0) store_sums(p, mall, lall, split, orow, D);
+}
+
+// ------------------------------------------------------------------ attention of many rows
+// Four waves of 32 query rows; the pages of the run come through an LDS ring of three by direct
+// loads, each read once for 128 rows.  32 x 32 matrix instructions, which one wave a SIMD feeds at
+// their rate (accumulators 128 registers and queries 64 leave no room for a second one).
+//
+// Lane L holds query row L % 32 and, of a 32-key S^T tile, the tile rows 8 a + 4 (L / 32) + r.  Tile
+// t's row 8 a + 4 h + r is key 32 h + 16 t + 4 a + r, so that the lane holds keys 32 (L / 32) .. + 31,
+// and eight consecutive of them are what it gives to one 16-deep step of P V: 32 bytes of a V row.
+// LDS: 16-byte chunk c of key row k is kept at c ^ swizzle(k), and of a V row likewise, so that
+// eight lanes that read one chunk of their rows meet eight different bank groups.
+typedef int v16i __attribute__((ext_vector_type(16)));
+typedef float v16f __attribute__((ext_vector_type(16)));
+
+template <int D>
+struct WideAttn {
+  static constexpr int kWaves = 4, kRows = 32 * kWaves, kSlots = 3;
+  static constexpr int kSide = kKvPage * D;                   // bytes of a page's keys (or values)
+  static constexpr int kPieces = kSide / 1024 / kWaves;       // 1 KB pieces of a wave and side
+  static constexpr int kLds = kSlots * 2 * kSide;
+  static constexpr int kChunks = D / 16;                      // 16-byte chunks of a key row
+  static constexpr int kPieceRows = 1024 / D;                 // key rows of a piece
+  __device__ static int key_swizzle(int k) {
+    return D >= 128 ? (k & 3) | ((k >> 5) & 1) << 2 : ((k >> 1) & 1) | ((k >> 5) & 1) << 1;
   }
+  __device__ static int value_swizzle(int d) { return (d >> 1) & 3; }
+};
+
+template <typename T, int D>
+__global__ __launch_bounds__(256, 1) void kv_attn_wide_kernel(KvAttnParams p) {
+  using C = WideAttn<D>;
+  constexpr int F = D / 32;  // 32-deep steps of Q K^T, and 32-row tiles of O^T
+  extern __shared__ __align__(1024) char lds[];
+  const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)lds));
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int h = lane >> 5, col = lane & 31;
+  const int group = p.h / p.c.kvh;
+  const int rows = p.t * group;
+  const int tiles = (rows + C::kRows - 1) / C::kRows;
+  const int tile = blockIdx.x % tiles, split = blockIdx.x / tiles;
+  const int head = blockIdx.y, b = blockIdx.z;
+  const Span span(p, b);
+
+  const int row = tile * C::kRows + wave * 32 + col;
+  const int tok = min(row / group, p.t - 1), qh = head * group + row % group;
+  const int64_t seen = row < rows ? span.seen(row / group) : 0;
+  // The pages of the workgroup's rows, and those of this wave's.
+  const int first = tile * C::kRows, last = min(first + C::kRows - 1, rows - 1);
+  const int wfirst = first + wave * 32, wlast = min(wfirst + 31, rows - 1);
+  const int64_t least = wfirst + 31 < rows ? span.least(wfirst / group, wlast / group) : 0;
+  const int64_t wmost = wfirst < rows ? span.most(wfirst / group, wlast / group) : 0;
+  const int pages = static_cast<int>((span.most(first / group, last / group) + kKvPage - 1) / kKvPage);
+  const int per = (pages + p.nsplit - 1) / p.nsplit;
+  const int begin = __builtin_amdgcn_readfirstlane(split * per);
+  const int end = __builtin_amdgcn_readfirstlane(min(begin + per, pages));
+
+  float sq;
+  v4i qhi[F], qlo[F];
+  const T* const qrow = static_cast<const T*>(p.q) + b * p.q_stride[0] + tok * p.q_stride[1] + qh * p.q_stride[2];
+  load_query<T, D, 32>(qrow, sq, qhi, qlo, h);
+  const float qfac = sq * p.scaling * kLog2e;
+
+  // Loader: the wave's pieces of either side (a piece of values is 16 rows of 64 bytes).
+  uint32_t ko[C::kPieces], vo[C::kPieces];
+#pragma unroll
+  for (int j = 0; j < C::kPieces; ++j) {
+    const int pc = wave * C::kPieces + j;
+    const int key = pc * C::kPieceRows + lane / C::kChunks;
+    ko[j] = static_cast<uint32_t>(key * D + ((lane % C::kChunks) ^ C::key_swizzle(key)) * 16);
+    const int d = pc * 16 + (lane >> 2);
+    vo[j] = static_cast<uint32_t>(d * kKvPage + ((lane & 3) ^ C::value_swizzle(d)) * 16);
+  }
+  const int32_t* const table = p.c.table + b * p.c.table_stride;
+  auto place = [&](int page) {  // entries that name no page are read as page 0
+    const int id = __builtin_amdgcn_readfirstlane(page);
+    return static_cast<int64_t>(id >= 0 && id < p.c.pages ? id : 0) * p.c.kvh + head;
+  };
+  auto request = [&](int page, int slot) {
+    const int64_t ph = place(page);
+    const char* const kb = reinterpret_cast<const char*>(p.c.k) + ph * C::kSide;
+    const char* const vb = reinterpret_cast<const char*>(p.c.v) + ph * C::kSide;
+    const uint32_t dst = lds0 + slot * 2 * C::kSide + wave * C::kPieces * 1024;
+#pragma unroll
+    for (int j = 0; j < C::kPieces; ++j) load_lds_1k(kb, ko[j], dst + j * 1024);
+#pragma unroll
+    for (int j = 0; j < C::kPieces; ++j) load_lds_1k(vb, vo[j], dst + C::kSide + j * 1024);
+  };
+
+  float m = kNone, l = 0.0f;
+  v16f o[F];
+#pragma unroll
+  for (int i = 0; i < F; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[i][r] = 0.0f;
+
+  // This lane's key of the first tile (row col of it), and its reads' offsets.
+  const int key = 32 * ((col >> 2) & 1) + 4 * (col >> 3) + (col & 3);  // + 16 for the second: the same swizzle
+  const int kswz = C::key_swizzle(key), vswz = C::value_swizzle(col);
+
+  // Table entries two pages ahead of their use.
+  auto entry = [&](int pg) { return pg < end ? scalar_load(table + pg) : -1; };
+  int page = entry(begin), page1 = entry(begin + 1), page2 = entry(begin + 2);
+  if (begin < end) request(page, 0);
+  if (begin + 1 < end) request(page1, 1);
+  int slot = 0;
+  for (int pg = begin; pg < end; ++pg) {
+    const int64_t ph = place(page);
+    const float ks = scalar_load(p.c.ks + ph);
+    float vs = scalar_load(p.c.vs + ph);
+    if (vs == 0.0f) vs = 1e-30f;  // zeros, whatever the codes: the page still counts in the sum
+    const int page3 = entry(pg + 3);
+    // Younger than this page's loads: the next page's.
+    if (pg + 1 < end) wait_vm<2 * C::kPieces>();
+    else wait_vm<0>();
+    lds_done_barrier();  // every wave's pieces are there, and the slot of the page before is free
+    if (pg + 2 < end) request(page2, slot == 0 ? 2 : slot - 1);
+    const char* const kst = lds + slot * 2 * C::kSide;
+    const char* const vst = kst + C::kSide;
+    const int64_t key0 = static_cast<int64_t>(pg) * kKvPage;
+    if (page >= 0 && page < p.c.pages && key0 < wmost) {  // uniform over the wave
+      const float fac = qfac * ks, lvs = __builtin_log2f(vs);
+      v4i kf[2][F];
+      auto read_keys = [&](int t) {
+#pragma unroll
+        for (int f = 0; f < F; ++f)
+          kf[t][f] = *reinterpret_cast<const v4i*>(kst + (key + 16 * t) * D + (((2 * f + h) ^ kswz) * 16));
+      };
+      read_keys(0);
+      float s[2][16];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        if (t == 0) read_keys(1);
+        __builtin_amdgcn_sched_barrier(0);
+        v16i ah, al;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) ah[r] = al[r] = 0;
+#pragma unroll
+        for (int f = 0; f < F; ++f) {
+          ah = __builtin_amdgcn_mfma_i32_32x32x32_i8(kf[t][f], qhi[f], ah, 0, 0, 0);
+          al = __builtin_amdgcn_mfma_i32_32x32x32_i8(kf[t][f], qlo[f], al, 0, 0, 0);
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[t][r] = fmaf(static_cast<float>(256 * ah[r] + al[r]), fac, lvs);
+      }
+      // The values' first reads pass under the softmax.
+      v4i vf[F][2];
+      auto read_values = [&](int i) {
+        const char* const vrow = vst + (32 * i + col) * kKvPage;  // 32 i: the same swizzle
+        vf[i][0] = *reinterpret_cast<const v4i*>(vrow + (((2 * h) ^ vswz) * 16));
+        vf[i][1] = *reinterpret_cast<const v4i*>(vrow + (((2 * h + 1) ^ vswz) * 16));
+      };
+      read_values(0);
+      read_values(1);
+      if (key0 + kKvPage > least) {  // some row does not see the whole page
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (key0 + 32 * h + 16 * t + r >= seen) s[t][r] = -__builtin_inff();
+      }
+      float top = s[0][0];
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) top = fmaxf(top, s[t][r]);
+      top = fmaxf(top, __shfl_xor(top, 32, 64));
+      if (__any(top > m + kSlack)) {
+        const float m1 = fmaxf(m, top);
+        const float alpha = __builtin_amdgcn_exp2f(m - m1);
+        m = m1;
+        l *= alpha;
+#pragma unroll
+        for (int i = 0; i < F; ++i) o[i] *= alpha;
+      }
+      float sum = 0.0f;
+      half8 w[4];  // 16-deep steps of P V: keys 32 h + 8 step .. + 7
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const float e = __builtin_amdgcn_exp2f(s[t][r] - m);
+          sum += e;
+          w[2 * t + (r >> 3)][r & 7] = static_cast<_Float16>(e);
+        }
+      l += sum != 0.0f ? sum / vs : 0.0f;
+#pragma unroll
+      for (int i = 0; i < F; ++i) {
+        if (i + 2 < F) read_values(i + 2);
+        o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(codes_to_half(vf[i][0][0], vf[i][0][1]), w[0], o[i], 0, 0, 0);
+        o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(codes_to_half(vf[i][0][2], vf[i][0][3]), w[1], o[i], 0, 0, 0);
+        o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(codes_to_half(vf[i][1][0], vf[i][1][1]), w[2], o[i], 0, 0, 0);
+        o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(codes_to_half(vf[i][1][2], vf[i][1][3]), w[3], o[i], 0, 0, 0);
+      }
+    }
+    slot = slot == 2 ? 0 : slot + 1;
+    page = page1;
+    page1 = page2;
+    page2 = page3;
+  }
+  wait_vm<0>();
+  l += __shfl_xor(l, 32, 64);
+  if (row >= rows) return;
+  const int64_t orow = (static_cast<int64_t>(b) * p.t + tok) * p.h + qh;
+  const float inv = l != 0.0f ? 1.0f / l : 0.0f;  // 0: no visible key (NaN stays NaN)
+#pragma unroll
+  for (int i = 0; i < F; ++i)
+#pragma unroll
+    for (int a = 0; a < 4; ++a)
+      store_quad<T>(p, v4f{o[i][4 * a], o[i][4 * a + 1], o[i][4 * a + 2], o[i][4 * a + 3]}, inv, split, orow, D, 32 * i + 8 * a + 4 * h);
+  if (h == 0) store_sums(p, m, l, split, orow, D);
 }
 
 // Joins the runs of a row: one wave a row.
@@ -418,14 +703,23 @@ void launch_append(const KvAppendParams& p, hipStream_t stream) {
   kv_append_kernel<T, D><<<grid, 256, 0, stream>>>(p);
 }
 
+// 32 rows are the fewer and wider tiles' gain: from 33 rows of a KV head on, one workgroup of 128
+// rows in place of several of 16 that read the same pages.
+bool wide_rows(int64_t rows) { return rows > 32; }
+
 template <typename T, int D>
 void launch_attn(const KvAttnParams& p, hipStream_t stream) {
-  const int tiles = (p.t * (p.h / p.c.kvh) + 15) / 16;
-  const dim3 grid(static_cast<unsigned>(tiles * p.nsplit), static_cast<unsigned>(p.c.kvh), static_cast<unsigned>(p.b));
-  kv_attn_kernel<T, D><<<grid, 256, 0, stream>>>(p);
+  const int rows = p.t * (p.h / p.c.kvh);
+  const bool wide = wide_rows(rows);
+  const int tile = wide ? WideAttn<D>::kRows : 16;
+  const dim3 grid(static_cast<unsigned>((rows + tile - 1) / tile * p.nsplit), static_cast<unsigned>(p.c.kvh), static_cast<unsigned>(p.b));
+  if (wide)
+    kv_attn_wide_kernel<T, D><<<grid, 256, WideAttn<D>::kLds, stream>>>(p);
+  else
+    kv_attn_kernel<T, D><<<grid, 64 * kAttnWaves, kAttnWaves * D * 64, stream>>>(p);
   if (p.nsplit > 1) {
-    const int64_t rows = static_cast<int64_t>(p.b) * p.t * p.h;
-    kv_attn_join_kernel<T, D><<<dim3(static_cast<unsigned>((rows + 3) / 4)), 256, 0, stream>>>(p);
+    const int64_t all = static_cast<int64_t>(p.b) * p.t * p.h;
+    kv_attn_join_kernel<T, D><<<dim3(static_cast<unsigned>((all + 3) / 4)), 256, 0, stream>>>(p);
   }
 }
 
@@ -448,14 +742,17 @@ hipError_t launch_kv_append(const KvAppendParams& p, int elem, hipStream_t strea
   return hipGetLastError();
 }
 
-// Runs of pages for each (sequence, KV head, 16-row tile): enough workgroups for two a CU, a run
-// being at least four pages long (one for each wave).
+// Runs of pages for each (sequence, KV head, row tile): as many as give every CU a workgroup, a run
+// being at least eight pages long (one for each wave) or, of the wide kernel, four.
 int kv_attn_splits(int64_t b, int64_t t, int32_t h, int32_t kvh, int32_t d, int64_t table_pages, int cus) {
   (void)d;
-  const int64_t tiles = (t * (h / kvh) + 15) / 16 * b * kvh;
-  if (tiles <= 0) return 1;
-  int64_t n = (2 * cus + tiles - 1) / tiles;
-  n = n < (table_pages + 3) / 4 ? n : (table_pages + 3) / 4;
+  const int64_t rows = t * (h / kvh);
+  const bool wide = wide_rows(rows);
+  const int64_t groups = (wide ? (rows + 127) / 128 : (rows + 15) / 16) * b * kvh;
+  if (groups <= 0) return 1;
+  const int64_t run = wide ? 4 : 8;
+  int64_t n = (cus + groups - 1) / groups;
+  n = n < (table_pages + run - 1) / run ? n : (table_pages + run - 1) / run;
   return static_cast<int>(n < 1 ? 1 : n > 64 ? 64 : n);
 }
 
