@@ -165,9 +165,9 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvAppendParams p) {
 
 // ------------------------------------------------------------------ attention
 // Two kernels.  kv_attn_kernel: 16 query rows of one KV head (row = token * (H / KVH) + query
-// head) and a run of the sequence's pages a workgroup, whose eight waves take every eighth page,
-// each with a softmax of its own (running maximum and sum), and meet in LDS at the end: decoded
-// tokens, where the cache is read once and its bytes bound.  kv_attn_wide_kernel: 128 rows, 32 a
+// head) and a run of the sequence's pages a workgroup, whose W waves take every W-th page, each with a
+// softmax of its own (running maximum and sum), and meet in LDS at the end: decoded tokens, where
+// the cache is read once and its bytes bound.  kv_attn_wide_kernel: 128 rows, 32 a
 // wave, over pages that the waves share in LDS: chunks of tokens.
 //
 // Q K^T in int8: a query row is held as 16-bit integers v = rint(q / sq), |v| <= 32512, split
@@ -301,11 +301,9 @@ __device__ __forceinline__ void store_sums(const KvAttnParams& p, float m, float
 // t's row 4 a + r is key 16 a + 4 t + r, so that over the four tiles of a page the lane holds
 // keys 16 (L / 16) .. + 15: the 16 bytes that it loads of a V row.
 // A page's values are requested before its scores, the next page's keys as the values are used up.
-constexpr int kAttnWaves = 8;
-
-template <typename T, int D>
-__global__ __launch_bounds__(64 * kAttnWaves, 2) void kv_attn_kernel(KvAttnParams p) {
-  constexpr int F = D / 64, DT = D / 16, W = kAttnWaves;
+template <typename T, int D, int W>
+__global__ __launch_bounds__(64 * W, 2) void kv_attn_kernel(KvAttnParams p) {
+  constexpr int F = D / 64, DT = D / 16;
   static_assert(DT == 4 * F, "a key load for each tile of values");
   extern __shared__ __align__(16) v4f obuf[];  // [W][DT][64]
   __shared__ float mbuf[W][16], lbuf[W][16];
@@ -430,6 +428,15 @@ __global__ __launch_bounds__(64 * kAttnWaves, 2) void kv_attn_kernel(KvAttnParam
   l += __shfl_xor(l, 16, 64);
   l += __shfl_xor(l, 32, 64);
 
+  const int64_t orow = (static_cast<int64_t>(b) * p.t + tok) * p.h + qh;
+  if constexpr (W == 1) {
+    if (row >= rows) return;
+    const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+#pragma unroll
+    for (int i = 0; i < DT; ++i) store_quad<T>(p, o[i], inv, split, orow, D, 16 * i + 4 * g);
+    if (g == 0) store_sums(p, m, l, split, orow, D);
+    return;
+  }
   // The waves' parts meet in LDS, scaled to a common maximum; each wave sums and finishes DT / W tiles
   // of dimensions.
   if (g == 0) {
@@ -448,7 +455,6 @@ __global__ __launch_bounds__(64 * kAttnWaves, 2) void kv_attn_kernel(KvAttnParam
   for (int w = 0; w < W; ++w) lall += lbuf[w][col] * __builtin_amdgcn_exp2f(mbuf[w][col] - mall);
   __syncthreads();
   if (row >= rows) return;
-  const int64_t orow = (static_cast<int64_t>(b) * p.t + tok) * p.h + qh;
   const float inv = lall != 0.0f ? 1.0f / lall : 0.0f;  // 0: no visible key (NaN stays NaN)
   for (int i = wave; i < DT; i += W) {
     v4f v = obuf[i * 64 + lane];
@@ -671,7 +677,9 @@ __global__ __launch_bounds__(256, 1) void kv_attn_wide_kernel(KvAttnParams p) {
   if (h == 0) store_sums(p, m, l, split, orow, D);
 }
 
-// Joins the runs of a row: one wave a row.
+// Joins the runs of a row, at most 64 of them: one wave a row, lane s with the maximum and sum of run s.
+constexpr int kMaxRuns = 64;
+
 template <typename T, int D>
 __global__ __launch_bounds__(256) void kv_attn_join_kernel(KvAttnParams p) {
   constexpr int E = D / 64;
@@ -680,20 +688,36 @@ __global__ __launch_bounds__(256) void kv_attn_join_kernel(KvAttnParams p) {
   const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
   if (row >= rows) return;
   const int64_t plane = split_floats(rows, D);
-  float m = kNone, l = 0.0f, o[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) o[e] = 0.0f;
-  for (int s = 0; s < p.nsplit; ++s) m = fmaxf(m, p.ws[s * plane + rows * D + row * 2]);
-  for (int s = 0; s < p.nsplit; ++s) {
-    const float* const ml = p.ws + s * plane + rows * D + row * 2;
-    const float a = __builtin_amdgcn_exp2f(ml[0] - m);
-    l += ml[1] * a;
-#pragma unroll
-    for (int e = 0; e < E; ++e) o[e] += p.ws[s * plane + row * D + e * 64 + lane] * a;
+  float ms = kNone, ls = 0.0f;
+  if (lane < p.nsplit) {
+    const float2 ml = *reinterpret_cast<const float2*>(p.ws + lane * plane + rows * D + row * 2);
+    ms = ml.x;
+    ls = ml.y;
   }
-  const bool empty = l == 0.0f;
+  float m = ms;
 #pragma unroll
-  for (int e = 0; e < E; ++e) static_cast<T*>(p.out)[row * D + e * 64 + lane] = static_cast<T>(empty ? 0.0f : o[e] / l);
+  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+  const float a = __builtin_amdgcn_exp2f(ms - m);
+  float l = ls * a;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o, 64);
+  struct alignas(4 * E) Vec { float v[E]; };
+  struct alignas(2 * E) Out { T v[E]; };
+  Vec sum{};
+  const float* const src = p.ws + row * D + lane * E;
+#pragma unroll 8
+  for (int s = 0; s < p.nsplit; ++s) {
+    const Vec x = *reinterpret_cast<const Vec*>(src + s * plane);
+    const float as = __shfl(a, s, 64);
+#pragma unroll
+    for (int e = 0; e < E; ++e) sum.v[e] += x.v[e] * as;
+  }
+  const bool empty = l == 0.0f;  // no visible key
+  const float inv = 1.0f / l;
+  Out y;
+#pragma unroll
+  for (int e = 0; e < E; ++e) y.v[e] = static_cast<T>(empty ? 0.0f : sum.v[e] * inv);
+  *reinterpret_cast<Out*>(static_cast<T*>(p.out) + row * D + lane * E) = y;
   if (p.lse != nullptr && lane == 0) p.lse[row] = empty ? -__builtin_inff() : m / kLog2e + __builtin_logf(l);
 }
 
@@ -713,10 +737,15 @@ void launch_attn(const KvAttnParams& p, hipStream_t stream) {
   const bool wide = wide_rows(rows);
   const int tile = wide ? WideAttn<D>::kRows : 16;
   const dim3 grid(static_cast<unsigned>((rows + tile - 1) / tile * p.nsplit), static_cast<unsigned>(p.c.kvh), static_cast<unsigned>(p.b));
-  if (wide)
+  if (wide) {
     kv_attn_wide_kernel<T, D><<<grid, 256, WideAttn<D>::kLds, stream>>>(p);
-  else
-    kv_attn_kernel<T, D><<<grid, 64 * kAttnWaves, kAttnWaves * D * 64, stream>>>(p);
+  } else {
+    // A wave for every page of a run, or for every fourth of a long one.
+    const int run = (p.c.table_pages + p.nsplit - 1) / p.nsplit;
+    if (run >= 6) kv_attn_kernel<T, D, 8><<<grid, 64 * 8, 8 * D * 64, stream>>>(p);
+    else if (run >= 2) kv_attn_kernel<T, D, 2><<<grid, 64 * 2, 2 * D * 64, stream>>>(p);
+    else kv_attn_kernel<T, D, 1><<<grid, 64, 0, stream>>>(p);
+  }
   if (p.nsplit > 1) {
     const int64_t all = static_cast<int64_t>(p.b) * p.t * p.h;
     kv_attn_join_kernel<T, D><<<dim3(static_cast<unsigned>((all + 3) / 4)), 256, 0, stream>>>(p);
@@ -742,18 +771,19 @@ hipError_t launch_kv_append(const KvAppendParams& p, int elem, hipStream_t strea
   return hipGetLastError();
 }
 
-// Runs of pages for each (sequence, KV head, row tile): as many as give every CU a workgroup, a run
-// being at least eight pages long (one for each wave) or, of the wide kernel, four.
+// Runs of pages for each (sequence, KV head, row tile): as many as give every CU a workgroup, since
+// a CU by itself reads no more than 65 to 100 GB/s (13 pages on two CUs: 4.3 us of loads); a run of
+// the wide kernel is at least two pages.
 int kv_attn_splits(int64_t b, int64_t t, int32_t h, int32_t kvh, int32_t d, int64_t table_pages, int cus) {
   (void)d;
   const int64_t rows = t * (h / kvh);
   const bool wide = wide_rows(rows);
   const int64_t groups = (wide ? (rows + 127) / 128 : (rows + 15) / 16) * b * kvh;
-  if (groups <= 0) return 1;
-  const int64_t run = wide ? 4 : 8;
-  int64_t n = (cus + groups - 1) / groups;
-  n = n < (table_pages + run - 1) / run ? n : (table_pages + run - 1) / run;
-  return static_cast<int>(n < 1 ? 1 : n > 64 ? 64 : n);
+  if (groups <= 0 || table_pages <= 0) return 1;
+  const int64_t runs = wide ? (table_pages + 1) / 2 : table_pages;
+  int64_t n = wide ? cus / groups : (cus + groups - 1) / groups;
+  n = n < runs ? n : runs;
+  return static_cast<int>(n < 1 ? 1 : n > kMaxRuns ? kMaxRuns : n);
 }
 
 size_t kv_attn_workspace(int64_t b, int64_t t, int32_t h, int32_t d, int nsplit) {
