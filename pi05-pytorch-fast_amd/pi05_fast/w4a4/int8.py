@@ -63,9 +63,9 @@ def _quantize_impl(x, residual, weight, eps, unit_offset, what):
         residual, ldr = _rows(residual, k, "residual")
     xr, ldx = _rows(x, k, "x")
     m = x.numel() // k
-    q = torch.empty(shape, dtype=torch.int8, device=dev)
+    q = torch.empty_like(x, dtype=torch.int8, memory_format=torch.contiguous_format)
     scale = torch.empty(shape[:-1], dtype=torch.float32, device=dev)
-    h = torch.empty(shape, dtype=x.dtype, device=dev) if residual is not None else None
+    h = torch.empty_like(x, memory_format=torch.contiguous_format) if residual is not None else None
     lib = _ext._lib if _ext._lib is not None else load_int4_gemm()
     with _on_device(dev):
         _check(lib.pi05w4a4_int8_rows(xr.data_ptr(), ldx, _ptr(residual), ldr, _ptr(weight), eps,
@@ -104,12 +104,12 @@ def _gemm_impl(q, q_scale, w, w_scale, bias, residual, out_dtype):
     lead = q.shape[:-1]
     shape = (*lead, n)
     m = q.numel() // k
-    for name, t, want in (("q_scale", q_scale, m), ("w_scale", w_scale, n)):
-        if t.device != dev or t.dtype != torch.float32 or t.numel() != want:
-            raise RuntimeError(f"int8_gemm: {name} must be float32 of {want} values on {dev}")
-    if q_scale.shape != lead or w_scale.dim() != 1:
-        raise RuntimeError(f"int8_gemm: q_scale must be {tuple(lead)} and w_scale [{n}], got "
-                           f"{tuple(q_scale.shape)} and {tuple(w_scale.shape)}")
+    if q_scale.dtype != torch.float32 or q_scale.device != dev or q_scale.shape != lead:
+        raise RuntimeError(f"int8_gemm: q_scale must be float32 {tuple(lead)} on {dev}, got {q_scale.dtype} "
+                           f"{tuple(q_scale.shape)} on {q_scale.device}")
+    if w_scale.dtype != torch.float32 or w_scale.device != dev or w_scale.shape != (n,):
+        raise RuntimeError(f"int8_gemm: w_scale must be float32 [{n}] on {dev}, got {w_scale.dtype} "
+                           f"{tuple(w_scale.shape)} on {w_scale.device}")
     if w.device != dev:
         raise RuntimeError(f"int8_gemm: the weights must be on {dev}, got {w.device}")
     if bias is not None:
@@ -138,7 +138,7 @@ def _gemm_impl(q, q_scale, w, w_scale, bias, residual, out_dtype):
             if len(_GEMM_WS) > 4096:
                 _GEMM_WS.clear()
             need = _GEMM_WS[key] = int(lib.pi05w4a4_int8_gemm_workspace_bytes(m, n, k))
-        ws = _workspace(dev, need)
+        ws = _workspace(dev, need) if need else None
         _check(lib.pi05w4a4_int8_gemm(q.data_ptr(), ldq, q_scale.data_ptr(), m, k, w.data_ptr(), ldw,
                                       w_scale.data_ptr(), n, _ptr(bias), _ptr(residual), ldr, elem, y.data_ptr(),
                                       _ptr(ws), need, _stream(dev)), "pi05w4a4_int8_gemm")

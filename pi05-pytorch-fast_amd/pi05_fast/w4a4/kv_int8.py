@@ -59,20 +59,20 @@ def _strided(t: torch.Tensor) -> tuple[torch.Tensor, ctypes.Array]:
 def _check_cache(what, dev, k_cache, v_cache, k_scale, v_scale, table, lens, b, kvh, d):
     if d not in HEAD_DIMS:
         raise RuntimeError(f"{what}: head_dim must be 64, 128 or 256, got {d}")
-    pages = int(k_cache.size(0)) if k_cache.dim() else 0
-    if k_cache.dtype != torch.int8 or tuple(k_cache.shape) != (pages, kvh, PAGE_TOKENS, d):
+    pages = k_cache.size(0) if k_cache.dim() else 0
+    if k_cache.dtype != torch.int8 or k_cache.shape != (pages, kvh, PAGE_TOKENS, d):
         raise RuntimeError(f"{what}: k_cache must be int8 [pages, {kvh}, {PAGE_TOKENS}, {d}], got {k_cache.dtype} "
                            f"{tuple(k_cache.shape)}")
-    if v_cache.dtype != torch.int8 or tuple(v_cache.shape) != (pages, kvh, d, PAGE_TOKENS):
+    if v_cache.dtype != torch.int8 or v_cache.shape != (pages, kvh, d, PAGE_TOKENS):
         raise RuntimeError(f"{what}: v_cache must be int8 [{pages}, {kvh}, {d}, {PAGE_TOKENS}], got {v_cache.dtype} "
                            f"{tuple(v_cache.shape)}")
     for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
-        if t.dtype != torch.float32 or tuple(t.shape) != (pages, kvh):
+        if t.dtype != torch.float32 or t.shape != (pages, kvh):
             raise RuntimeError(f"{what}: {name} must be float32 [{pages}, {kvh}], got {t.dtype} {tuple(t.shape)}")
-    if table.dtype != torch.int32 or table.dim() != 2 or int(table.size(0)) != b:
+    if table.dtype != torch.int32 or table.dim() != 2 or table.size(0) != b:
         raise RuntimeError(f"{what}: block_table must be int32 [{b}, pages of a sequence], got {table.dtype} "
                            f"{tuple(table.shape)}")
-    if lens.dtype != torch.int32 or tuple(lens.shape) != (b,):
+    if lens.dtype != torch.int32 or lens.shape != (b,):
         raise RuntimeError(f"{what}: lens must be int32 [{b}], got {lens.dtype} {tuple(lens.shape)}")
     for t in (k_cache, v_cache, k_scale, v_scale, table, lens):
         if t.device != dev:
@@ -88,7 +88,7 @@ def _ints(what, name, t, b, dev):
     """An optional int32 [B] on the cache's device, contiguous."""
     if t is None:
         return None
-    if t.dtype != torch.int32 or tuple(t.shape) != (b,) or t.device != dev:
+    if t.dtype != torch.int32 or t.shape != (b,) or t.device != dev:
         raise RuntimeError(f"{what}: {name} must be int32 [{b}] on {dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
     return t.contiguous()
 
@@ -109,7 +109,7 @@ def _append_impl(k, v, k_cache, v_cache, k_scale, v_scale, block_table, lens, co
         raise RuntimeError(f"{what} takes float16 or bfloat16 keys and values of one type, got {k.dtype} and {v.dtype}")
     if k.dim() != 4 or v.shape != k.shape or v.device != dev:
         raise RuntimeError(f"{what} expects k and v [B, T, KVH, D] on one device, got {tuple(k.shape)} and {tuple(v.shape)}")
-    b, t, kvh, d = (int(x) for x in k.shape)
+    b, t, kvh, d = k.shape
     pages = _check_cache(what, dev, k_cache, v_cache, k_scale, v_scale, block_table, lens, b, kvh, d)
     counts = _ints(what, "counts", counts, b, dev)
     if b == 0 or t == 0:
@@ -137,20 +137,20 @@ def _attention_impl(q, k_cache, v_cache, k_scale, v_scale, block_table, lens, sc
     if q.dim() != 4 or k_cache.dim() != 4:
         raise RuntimeError(f"{what} expects q [B, T, H, D] and k_cache [pages, KVH, 64, D], got {tuple(q.shape)} and "
                            f"{tuple(k_cache.shape)}")
-    b, t, h, d = (int(x) for x in q.shape)
-    kvh = int(k_cache.size(1))
+    b, t, h, d = q.shape
+    kvh = k_cache.size(1)
     if kvh == 0 or h == 0 or h % kvh:
         raise RuntimeError(f"{what}: the query heads must be a multiple of the KV heads, got {h} and {kvh}")
     pages = _check_cache(what, dev, k_cache, v_cache, k_scale, v_scale, block_table, lens, b, kvh, d)
     q_lens = _ints(what, "q_lens", q_lens, b, dev)
-    out = torch.empty((b, t, h, d), dtype=q.dtype, device=dev)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = torch.empty((b, t, h), dtype=torch.float32, device=dev) if return_lse else None
     if b == 0 or t == 0:
         return out, lse
     table, stride = _table(block_table)
     lens = lens.contiguous()
     q, qs = _strided(q)
-    tp = int(table.size(1))
+    tp = table.size(1)
     lib = _ext._lib if _ext._lib is not None else load_int4_gemm()
     with _on_device(dev):
         key = (dev.index, b, t, h, kvh, d, tp)
@@ -159,7 +159,7 @@ def _attention_impl(q, k_cache, v_cache, k_scale, v_scale, block_table, lens, sc
             if len(_ATTN_WS) > 4096:
                 _ATTN_WS.clear()
             need = _ATTN_WS[key] = int(lib.pi05w4a4_int8_kv_attention_workspace_bytes(b, t, h, kvh, d, tp))
-        ws = _workspace(dev, need)
+        ws = _workspace(dev, need) if need else None
         _check(lib.pi05w4a4_int8_kv_attention(q.data_ptr(), qs, elem, b, t, h, kvh, d, k_cache.data_ptr(),
                                               v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), pages,
                                               table.data_ptr(), stride, tp, lens.data_ptr(), _ptr(q_lens), scaling,
