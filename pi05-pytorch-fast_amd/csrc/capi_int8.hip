@@ -148,7 +148,7 @@ extern "C" int pi05w4a4_int8_kv_append(const void* k, const int64_t* k_strides, 
 extern "C" size_t pi05w4a4_int8_kv_attention_workspace_bytes(int32_t b, int32_t t, int32_t h, int32_t kvh, int32_t d,
                                                              int32_t table_pages) {
   if (b <= 0 || t <= 0 || kvh <= 0 || h < kvh || table_pages <= 0) return 0;
-  return kv_attn_workspace(b, t, h, d, kv_attn_splits(b, t, h, kvh, d, table_pages, device_cu_count()));
+  return kv_attn_workspace(b, t, h, d, kv_attn_plan(b, t, h, kvh, d, table_pages, device_cu_count()).nsplit);
 }
 
 extern "C" int pi05w4a4_int8_kv_attention(const void* q, const int64_t* q_strides, int32_t elem, int32_t b, int32_t t,
@@ -173,7 +173,9 @@ extern "C" int pi05w4a4_int8_kv_attention(const void* q, const int64_t* q_stride
   if (int rc = check_strides(q, q_strides, "q")) return rc;
   if (out == nullptr || !aligned(out, 16) || !aligned(lse, 4) || !aligned(q_lens, 4))
     return capi_fail(PI05W4A4_EINVAL, "out must be 16-byte aligned");
-  p.nsplit = kv_attn_splits(b, t, h, kvh, d, table_pages, device_cu_count());
+  const KvAttnPlan plan = kv_attn_plan(b, t, h, kvh, d, table_pages, device_cu_count());
+  p.nsplit = plan.nsplit;
+  p.wide = plan.wide;
   const size_t need = kv_attn_workspace(b, t, h, d, p.nsplit);
   if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned(workspace, 16)))
     return capi_fail(PI05W4A4_EWORKSPACE, "int8_kv_attention needs a 16-byte aligned workspace of %zu bytes, got %zu", need, workspace_bytes);

@@ -82,8 +82,13 @@ struct KvAttnParams {
   int32_t causal;
   int32_t b, t, h;
   int32_t nsplit;
+  bool wide;  // 128 rows a workgroup, else 16
 };
-int kv_attn_splits(int64_t b, int64_t t, int32_t h, int32_t kvh, int32_t d, int64_t table_pages, int cus);
+struct KvAttnPlan {
+  bool wide;
+  int nsplit;
+};
+KvAttnPlan kv_attn_plan(int64_t b, int64_t t, int32_t h, int32_t kvh, int32_t d, int64_t table_pages, int cus);
 size_t kv_attn_workspace(int64_t b, int64_t t, int32_t h, int32_t d, int nsplit);
 hipError_t launch_kv_attention(const KvAttnParams& p, int elem, hipStream_t stream);
 

@@ -6,6 +6,8 @@
 // are 16-byte loads of consecutive codes of either array: no transposes, no LDS for the cache.
 
 #include "direct_load.h"
+#include <algorithm>
+
 #include "int8_internal.h"
 
 namespace w4a4 {
@@ -167,8 +169,8 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvAppendParams p) {
 // Two kernels.  kv_attn_kernel: 16 query rows of one KV head (row = token * (H / KVH) + query
 // head) and a run of the sequence's pages a workgroup, whose W waves take every W-th page, each with a
 // softmax of its own (running maximum and sum), and meet in LDS at the end: decoded tokens, where
-// the cache is read once and its bytes bound.  kv_attn_wide_kernel: 128 rows, 32 a
-// wave, over pages that the waves share in LDS: chunks of tokens.
+// the cache is read once and its bytes bound, and as many more rows as one round of the CUs holds.
+// kv_attn_wide_kernel: 128 rows, 32 a wave, over pages that the waves share in LDS: chunks of tokens.
 //
 // Q K^T in int8: a query row is held as 16-bit integers v = rint(q / sq), |v| <= 32512, split
 // v = 256 hi + lo into two int8 operands, so that S = sq ks (256 K hi + K lo) is exact but for
@@ -727,17 +729,12 @@ void launch_append(const KvAppendParams& p, hipStream_t stream) {
   kv_append_kernel<T, D><<<grid, 256, 0, stream>>>(p);
 }
 
-// 32 rows are the fewer and wider tiles' gain: from 33 rows of a KV head on, one workgroup of 128
-// rows in place of several of 16 that read the same pages.
-bool wide_rows(int64_t rows) { return rows > 32; }
-
 template <typename T, int D>
 void launch_attn(const KvAttnParams& p, hipStream_t stream) {
   const int rows = p.t * (p.h / p.c.kvh);
-  const bool wide = wide_rows(rows);
-  const int tile = wide ? WideAttn<D>::kRows : 16;
+  const int tile = p.wide ? WideAttn<D>::kRows : 16;
   const dim3 grid(static_cast<unsigned>((rows + tile - 1) / tile * p.nsplit), static_cast<unsigned>(p.c.kvh), static_cast<unsigned>(p.b));
-  if (wide) {
+  if (p.wide) {
     kv_attn_wide_kernel<T, D><<<grid, 256, WideAttn<D>::kLds, stream>>>(p);
   } else {
     // A wave for every page of a run, or for every fourth of a long one.
@@ -771,19 +768,36 @@ hipError_t launch_kv_append(const KvAppendParams& p, int elem, hipStream_t strea
   return hipGetLastError();
 }
 
-// Runs of pages for each (sequence, KV head, row tile): as many as give every CU a workgroup, since
-// a CU by itself reads no more than 65 to 100 GB/s (13 pages on two CUs: 4.3 us of loads); a run of
-// the wide kernel is at least two pages.
-int kv_attn_splits(int64_t b, int64_t t, int32_t h, int32_t kvh, int32_t d, int64_t table_pages, int cus) {
-  (void)d;
+// Runs of pages: as many as give every CU one workgroup, since a CU by itself reads no more than 65 to
+// 100 GB/s, and none where half of the CUs have one without (us, D = 256: 96 sequences of 8192 keys,
+// 16 rows, with 1 / 2 / 4 runs 116 / 80 / 92; 150 sequences 128 / 154 / 140); a run of the wide kernel
+// is at least two pages.
+// The kernel: the one with the smaller sum of these times of a round of CUs, fitted to measurements
+// (us; rows of a KV head, then narrow / wide).  D = 256: 8 x 400 rows over 826 keys 20 / 28, 1 x 2400
+// over 4096 52 / 38, 32 x 400 over 826 71 / 44.  D = 128: 16 x 200 over 2000 19 / 25, 64 x 200 over
+// 826 41 / 30.  D = 64: 2 x 6208 over 4096 38 / 60.
+KvAttnPlan kv_attn_plan(int64_t b, int64_t t, int32_t h, int32_t kvh, int32_t d, int64_t table_pages, int cus) {
+  KvAttnPlan plan{false, 1};
   const int64_t rows = t * (h / kvh);
-  const bool wide = wide_rows(rows);
-  const int64_t groups = (wide ? (rows + 127) / 128 : (rows + 15) / 16) * b * kvh;
-  if (groups <= 0 || table_pages <= 0) return 1;
-  const int64_t runs = wide ? (table_pages + 1) / 2 : table_pages;
-  int64_t n = wide ? cus / groups : (cus + groups - 1) / groups;
-  n = n < runs ? n : runs;
-  return static_cast<int>(n < 1 ? 1 : n > kMaxRuns ? kMaxRuns : n);
+  if (rows <= 0 || b <= 0 || table_pages <= 0) return plan;
+  struct Cost {
+    double start, page, join;  // of a workgroup, of a page of its run, of joining runs
+  };
+  const Cost narrow = d == 64 ? Cost{2.5, 0.15, 4} : d == 128 ? Cost{8, 0.3, 4} : Cost{10, 0.62, 4};
+  const Cost wide = d == 64 ? Cost{2, 1.6, 6} : d == 128 ? Cost{6, 2.2, 6} : Cost{10, 2.9, 6};
+  auto runs = [&](int64_t groups, int64_t most) {
+    const int64_t n = std::min(cus / groups, std::min(most, static_cast<int64_t>(kMaxRuns)));
+    return n < 1 ? int64_t{1} : n;
+  };
+  auto time = [&](const Cost& c, int64_t groups, int64_t n) {
+    return static_cast<double>((groups * n + cus - 1) / cus) * (c.start + c.page * static_cast<double>((table_pages + n - 1) / n)) +
+           (n > 1 ? c.join : 0);
+  };
+  const int64_t few = (rows + 15) / 16 * b * kvh, many = (rows + 127) / 128 * b * kvh;
+  const int64_t nfew = runs(few, table_pages), nmany = runs(many, (table_pages + 1) / 2);
+  plan.wide = time(wide, many, nmany) < time(narrow, few, nfew);
+  plan.nsplit = static_cast<int>(plan.wide ? nmany : nfew);
+  return plan;
 }
 
 size_t kv_attn_workspace(int64_t b, int64_t t, int32_t h, int32_t d, int nsplit) {

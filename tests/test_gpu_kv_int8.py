@@ -371,6 +371,83 @@ def test_query_strides(cuda):
     assert torch.equal(one, kv.int8_kv_attention(q[:, :1, :1].expand(3, 6, 8, 256).contiguous(), *cache, table, lens, 0.06))
 
 
+def _reference_many(q, cache, table, lens, scaling, causal, q_lens):
+    """_reference with all tokens of a head at once, and the same bounds."""
+    kc, vc, ks, vs = cache
+    b, t, h, d = q.shape
+    kvh = kc.size(1)
+    out = torch.zeros(q.shape, dtype=torch.float64, device="cuda")
+    tol = torch.zeros_like(out)
+    lse = torch.full((b, t, h), float("-inf"), dtype=torch.float64, device="cuda")
+    for i in range(b):
+        n, ql = min(max(lens[i], 0), table.size(1) * PAGE), min(max(q_lens[i], 0), t)
+        if n == 0 or ql == 0:
+            continue
+        ids = table[i].long()
+        ok = ((ids >= 0) & (ids < kc.size(0))).repeat_interleave(PAGE)[:n]
+        ids = ids.clamp(0, kc.size(0) - 1)
+        at = torch.arange(n, device="cuda")
+        last = n - ql + torch.arange(ql, device="cuda") if causal else torch.full((ql,), n, device="cuda")
+        see = ok & (at <= last[:, None])
+        some = see.any(-1)
+        for g in range(kvh):
+            k = (kc[ids, g].double() * ks[ids, g].double()[:, None, None]).reshape(-1, d)[:n].nan_to_num(0, 0, 0) * ok[:, None]
+            v = (vc[ids, g].double() * vs[ids, g].double()[:, None, None]).transpose(1, 2).reshape(-1, d)[:n].nan_to_num(0, 0, 0) * ok[:, None]
+            for hh in range(g * (h // kvh), (g + 1) * (h // kvh)):
+                qq = q[i, :ql, hh].double()
+                z = (qq @ k.t().contiguous() * scaling).masked_fill(~see, float("-inf"))
+                p = torch.softmax(z, -1).nan_to_num(0)
+                top = z.masked_fill(~see, 0).abs().amax(-1, keepdim=True)
+                e = (abs(scaling) * qq.abs().amax(-1) / 65024 * k.abs().sum(-1).max())[:, None]
+                out[i, :ql, hh] = p @ v
+                lse[i, :ql, hh] = torch.logsumexp(z, -1)
+                tol[i, :ql, hh] = some[:, None] * ((2 * e + 2.0**-19 * top + 2.0**-11 + 2.0**-18) * (p @ v.abs())
+                                                   + n * 2.0**-25 * v.abs().max())
+    return out, lse, tol + (torch.finfo(q.dtype).eps / 2) * out.abs() * 1.001 + 2.0**-25
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("b,t,h,kvh,d,pages", [
+    (4, 300, 8, 1, 256, 3), (4, 300, 8, 1, 256, 20), (1, 300, 8, 1, 256, 64), (4, 1100, 2, 2, 256, 2),
+    (4, 800, 8, 1, 128, 3), (4, 700, 6, 2, 128, 30), (5, 451, 8, 2, 64, 2), (4, 1501, 8, 2, 64, 4), (4, 50, 32, 8, 128, 32),
+])
+def test_attention_of_chunks(cuda, b, t, h, kvh, d, pages, dtype):
+    """More rows than one round of small workgroups: whole and ragged chunks, a sequence shorter than its queries, an
+    empty one, junk behind the last token and queries, a page that is none."""
+    gen = _gen(t + pages)
+    cache, table = _pool(gen, b, pages, kvh, d)
+    q = (torch.randn((b, t, h, d), device="cuda", generator=gen) * 1.5).to(dtype)
+    lens = [pages * PAGE - 3, pages * PAGE + 9, 70, 0, 65][:b]
+    q_lens = [t, t - 40, min(t, 100), t, 7][:b]
+    for i, n in enumerate(lens):
+        if n < (pages - 1) * PAGE:
+            for s in cache[2:]:
+                s[table[i, n // PAGE + 1:].long()] = float("nan")
+        q[i, q_lens[i]:] = float("nan")
+    if b > 1:
+        table[1, 1] = -1
+    for causal in (True, False):
+        got, lse = kv.int8_kv_attention(q, *cache, table, _i32(lens), d**-0.5, causal=causal, q_lens=_i32(q_lens), return_lse=True)
+        want, wlse, tol = _reference_many(q, cache, table, lens, d**-0.5, causal, q_lens)
+        assert ((got.double() - want).abs() / tol).max().item() <= 1
+        inf = torch.isinf(wlse)
+        assert torch.equal(inf, torch.isinf(lse)) and not got[inf].any()
+        assert ((lse.double() - wlse).abs() <= 1e-3 + 1e-3 * wlse.abs())[~inf].all()
+
+
+def test_chunks_of_other_strides(cuda):
+    """Queries that are a part of a product's output, and results that do not depend on where they lie."""
+    gen = _gen(23)
+    cache, table = _pool(gen, 4, 4, 1, 256)
+    wide = torch.randn((4, 301, 2560), device="cuda", generator=gen).half()
+    q = wide[:, 1:, :2048].view(4, 300, 8, 256)
+    lens = _i32([250, 256, 3, 190])
+    want = kv.int8_kv_attention(q.contiguous(), *cache, table, lens, 0.06)
+    assert torch.equal(kv.int8_kv_attention(q, *cache, table, lens, 0.06), want)
+    turned = q.transpose(1, 2).contiguous().transpose(1, 2)
+    assert torch.equal(kv.int8_kv_attention(turned, *cache, table, lens, 0.06), want)
+
+
 def test_joined_with_other_keys(cuda):
     """Two halves of a cache joined by their lse are the whole."""
     gen = _gen(18)
