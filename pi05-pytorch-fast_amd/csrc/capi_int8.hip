@@ -56,6 +56,9 @@ extern "C" int pi05w4a4_int8_rows(const void* x, int64_t ldx, const void* residu
   if (m < 0 || m > 0x7fffffffLL) return capi_fail(PI05W4A4_EINVAL, "M must be in [0, 2^31), got %lld", (long long)m);
   if (k <= 0 || k % 8 != 0 || k > 32768)
     return capi_fail(PI05W4A4_EINVAL, "K must be a multiple of 8 of at most 32768, got %d", k);
+  // A launch holds fewer than 2^32 threads: 64, 256 or 1024 of them a row.
+  if (m * (k <= 2048 ? 64 : k <= 8192 ? 256 : 1024) >= 1LL << 32)
+    return capi_fail(PI05W4A4_EINVAL, "M=%lld rows of K=%d are more than one launch holds", (long long)m, k);
   if (residual != nullptr && (norm_w == nullptr || h_out == nullptr))
     return capi_fail(PI05W4A4_EINVAL, "a residual needs a norm weight and an output for the sum");
   if (m == 0) return capi_ok();

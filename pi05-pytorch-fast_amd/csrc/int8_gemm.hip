@@ -700,6 +700,7 @@ Int8GemmPlan int8_gemm_plan(int64_t m, int32_t n, int32_t k, int cus) {
   const double steps = (k + 127) / 128;
   double best = 1e30;
   auto consider = [&](int tile, int64_t w, double step_us, int ks) {
+    if (w * ks >= 1 << 24) return;  // a launch holds fewer than 2^32 threads
     const double load = static_cast<double>(w) * ks / cus;
     const double us = (steps / ks) * step_us * (load < 1 ? 1 : load) +
                       (ks > 1 ? 3.0 + static_cast<double>(m) * n * (8.0 * ks + 2) / 5e6 : 0.0);

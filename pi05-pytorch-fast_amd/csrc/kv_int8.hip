@@ -252,8 +252,8 @@ __device__ __forceinline__ U scalar_load(const U* p) {
   return *reinterpret_cast<const __attribute__((address_space(4))) U*>(reinterpret_cast<uintptr_t>(p));
 }
 
-// Partial results of a run: O (unnormalised, fp32), the maximum and the sum of each row.
-__host__ __device__ inline int64_t split_floats(int64_t rows, int d) { return rows * (d + 2); }
+// Partial results of a run: O (unnormalised, fp32), the maximum and the sum of each row; whole 16 bytes.
+__host__ __device__ inline int64_t split_floats(int64_t rows, int d) { return (rows * (d + 2) + 3) & ~int64_t{3}; }
 
 // What a workgroup's rows see.  ROWS query rows of a KV head from row0 on; a lane's row is given.
 struct Span {
@@ -361,7 +361,7 @@ __global__ __launch_bounds__(64 * W, 2) void kv_attn_kernel(KvAttnParams p) {
     const int8_t* const vp = p.c.v + ph * (kKvPage * D) + voff;
     const float ks = scalar_load(p.c.ks + ph);
     float vs = scalar_load(p.c.vs + ph);
-    if (vs == 0.0f) vs = 1e-30f;  // zeros, whatever the codes: the page still counts in the sum
+    if (vs == 0.0f) vs = 1e-20f;  // zeros, whatever the codes: the page still counts in the sum
     v4i vc[DT];
 #pragma unroll
     for (int i = 0; i < DT; ++i) vc[i] = *reinterpret_cast<const v4i*>(vp + 16 * i * kKvPage);
@@ -576,7 +576,7 @@ __global__ __launch_bounds__(256, 1) void kv_attn_wide_kernel(KvAttnParams p) {
     const int64_t ph = place(page);
     const float ks = scalar_load(p.c.ks + ph);
     float vs = scalar_load(p.c.vs + ph);
-    if (vs == 0.0f) vs = 1e-30f;  // zeros, whatever the codes: the page still counts in the sum
+    if (vs == 0.0f) vs = 1e-20f;  // zeros, whatever the codes: the page still counts in the sum
     const int page3 = entry(pg + 3);
     // Younger than this page's loads: the next page's.
     if (pg + 1 < end) wait_vm<2 * C::kPieces>();

@@ -207,8 +207,8 @@ def int8_kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_ca
     earlier codes are rounded to it; a page whose first token is new is written whole, with
     zeros behind the last token.  No other page is touched.  A NaN or infinity makes its
     page's scale NaN.  Tokens past the table, or whose table entry names no page, are
-    dropped.  A call may write a page for one sequence only: full pages can be shared
-    between sequences, a page that still fills cannot."""
+    dropped.  A call may write a page from one place only: full pages can be shared between
+    sequences, and stand in a table twice, a page that still fills cannot."""
     if _direct(k, v, k_cache, v_cache, k_scale, v_scale, block_table, lens, counts):
         return _append_impl(k, v, k_cache, v_cache, k_scale, v_scale, block_table, lens, counts)
     return torch.ops.pi05_w4a4.int8_kv_append(k, v, k_cache, v_cache, k_scale, v_scale, block_table, lens, counts)

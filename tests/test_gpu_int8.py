@@ -153,6 +153,31 @@ def test_product(cuda, m, k, n, t):
         _check_product(i8.int8_gemm(*args[:4], bias=args[4], residual=args[5], out_dtype=t), *args)
 
 
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("m,k,n", [(4200, 1040, 4200), (8192, 112, 8201), (2600, 16, 2568), (4100, 2048, 4097)])
+def test_product_of_many_tiles(cuda, m, k, n, t):
+    """More large tiles than CUs, the last of a row, column and K ragged, and K of a single step."""
+    args = _product(_gen(m + k + n), m, k, n, t, True, True)
+    y = i8.int8_gemm(*args[:4], bias=args[4], residual=args[5], out_dtype=t)
+    for r in range(0, m, 1024):  # rows at a time: the 64-bit products
+        part = slice(r, r + 1024)
+        _check_product(y[part], args[0][part], args[1][part], args[2], args[3], args[4], args[5][part])
+
+
+def test_product_of_more_rows_than_a_launch_has_tiles(cuda):
+    m, k, n = (1 << 30) + 100, 16, 8
+    q = torch.empty((m, k), dtype=torch.int8, device="cuda")
+    sq = torch.empty((m,), device="cuda")
+    at = [slice(0, 300), slice(m // 2 - 150, m // 2 + 150), slice(m - 300, m)]
+    gen = _gen(5)
+    parts = [_product(gen, 300, k, n, torch.float16, False, False) for _ in at]
+    for s, p in zip(at, parts):
+        q[s], sq[s] = p[0], p[1]
+    y = i8.int8_gemm(q, sq, *parts[0][2:4])
+    for s, p in zip(at, parts):
+        _check_product(y[s], p[0], p[1], *parts[0][2:4], None, None)
+
+
 @pytest.mark.parametrize("m,n", [(1, 64), (40, 200), (300, 300), (700, 1024)])
 def test_product_extreme_sums(cuda, m, n):
     """The largest sum that K = 65536 can make, 2^30, is exact."""

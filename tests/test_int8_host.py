@@ -71,7 +71,8 @@ def _rows(lib, x=P, ldx=64, res=None, w=None, elem=0, m=2, k=64, q=P, scale=P, h
     (dict(elem=2), "elem"), (dict(m=-1), "M must"), (dict(m=1 << 31), "M must"), (dict(k=12), "multiple of 8"),
     (dict(k=32776), "at most 32768"), (dict(k=0), "multiple of 8"), (dict(res=P), "norm weight"),
     (dict(res=P, w=P), "norm weight"), (dict(x=None), "null"), (dict(x=vp(4098)), "aligned"),
-    (dict(ldx=60), "strides"), (dict(ldx=-8), "strides"),
+    (dict(ldx=60), "strides"), (dict(ldx=-8), "strides"), (dict(m=1 << 26), "one launch"),
+    (dict(m=1 << 24, k=2056), "one launch"), (dict(m=1 << 22, k=8200), "one launch"),
 ])
 def test_rows_refusals(lib, kw, text):
     assert _rows(lib, **kw) == 1 and text in _err(lib)
