@@ -43,28 +43,27 @@ struct Epilogue {
       bias[r] = p.bias != nullptr ? static_cast<float>(static_cast<const T*>(p.bias)[c]) : 0.0f;
     }
   }
-  __device__ __forceinline__ vec4<T> operator()(const v4i acc, float sq, const float (&sw)[4], const float (&bias)[4],
-                                                int64_t row, int64_t col) const {
-    float res[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  __device__ __forceinline__ vec4<T> residual(int64_t row, int64_t col) const {
+    vec4<T> v{};
     if (RES && p.res != nullptr && row < p.m) {
       const T* const rp = static_cast<const T*>(p.res) + row * p.ldr + col;
       if (res_vec) {
-        if (col < p.n) {
-          const vec4<T> v = *reinterpret_cast<const vec4<T>*>(rp);
-#pragma unroll
-          for (int r = 0; r < 4; ++r) res[r] = static_cast<float>(v[r]);
-        }
+        if (col < p.n) v = *reinterpret_cast<const vec4<T>*>(rp);
       } else {
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          if (col + r < p.n) res[r] = static_cast<float>(rp[r]);
+          if (col + r < p.n) v[r] = rp[r];
       }
     }
+    return v;
+  }
+  __device__ __forceinline__ vec4<T> operator()(const v4i acc, float sq, const float (&sw)[4], const float (&bias)[4],
+                                                const vec4<T> res) const {
     vec4<T> o;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const float v = fmaf(static_cast<float>(acc[r]) * sq, sw[r], bias[r]);
-      o[r] = static_cast<T>(RES ? v + res[r] : v);
+      o[r] = static_cast<T>(RES ? v + static_cast<float>(res[r]) : v);
     }
     return o;
   }
@@ -101,7 +100,9 @@ struct Int8Tile {
   static constexpr int kOwn = 4 / KW;                                 // blocks that a wave finishes
   static constexpr int kOutStride = 32 + 8;                           // staged output row, elements
   static constexpr int kBlock = KW > 1 ? (KW - 1) * 4096 : 4096;       // LDS of a block: its sums, then its output rows
-  static constexpr int kLds = ST * kStage > kPos * 4 * kBlock ? ST * kStage : kPos * 4 * kBlock;
+  static constexpr int kScale = ST * kStage > kPos * 4 * kBlock ? ST * kStage : kPos * 4 * kBlock;  // fp32 sq, sw, bias
+  static constexpr int kLds = kScale + (BM + 2 * BN) * 4;
+  static_assert(BM + 2 * BN <= 64 * kWaves, "a scale or bias of a thread");
   static_assert(32 * kOutStride * 2 <= kBlock, "a block's output rows fit where its sums were");
   static_assert(BM % (8 * kWaves) == 0 && BN % (8 * kWaves) == 0, "pieces are dealt evenly");
 };
@@ -234,6 +235,16 @@ __global__ __launch_bounds__(64 * (BM / 64) * (BN / 64) * KW, 2) void int8_tile_
     slot = next;
   };
 
+  // A scale or bias of the tile for each thread, on its way before the operands (loaded in the
+  // epilogue they cost 0.6 us there).
+  float scale = 0.0f;
+  if (p.ksplit == 1) {
+    const int i = threadIdx.x;
+    if (i < BM) scale = p.sq[min(m0 + i, p.m - 1)];
+    else if (i < BM + BN) scale = p.sw[min(n0 + i - BM, p.n - 1)];
+    else if (i < BM + 2 * BN && p.bias != nullptr)
+      scale = static_cast<float>(static_cast<const T*>(p.bias)[min(n0 + i - BM - BN, p.n - 1)]);
+  }
 #pragma unroll
   for (int s = 0; s < ST; ++s)
     if (s < nkb) {
@@ -250,6 +261,8 @@ __global__ __launch_bounds__(64 * (BM / 64) * (BN / 64) * KW, 2) void int8_tile_
     step(kb, a0, b0, a1, b1);
     if (kb + 1 < nkb) step(kb + 1, a1, b1, a0, b0);
   }
+  float* const sc = reinterpret_cast<float*>(lds + C::kScale);
+  if (static_cast<int>(threadIdx.x) < BM + 2 * BN) sc[threadIdx.x] = scale;
   lds_done_barrier();  // the ring becomes the waves' sums and the staging of the output rows
 
   if constexpr (KW > 1) {
@@ -279,7 +292,10 @@ __global__ __launch_bounds__(64 * (BM / 64) * (BN / 64) * KW, 2) void int8_tile_
     T* const stage = reinterpret_cast<T*>(mine);
     const int64_t mb = m0 + wm * 64 + (f >> 1) * 32, row = mb + (lane & 31);
     const int nb = n0 + wn * 64 + (f & 1) * 32;
-    const float sq = p.sq[min(row, p.m - 1)];
+    const float sq = sc[wm * 64 + (f >> 1) * 32 + (lane & 31)];
+    vec4<T> res[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) res[t] = p.ksplit == 1 ? epi.residual(row, nb + 8 * t + 4 * (lane >> 5)) : vec4<T>{};
     v4i sum[4];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {  // columns 8 t + 4 (L / 32) .. + 3 of row L % 32
@@ -299,9 +315,10 @@ __global__ __launch_bounds__(64 * (BM / 64) * (BN / 64) * KW, 2) void int8_tile_
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       const int c = 8 * t + 4 * (lane >> 5);
-      float sw[4], bias[4];
-      epi.scales(nb + c, sw, bias);
-      *reinterpret_cast<vec4<T>*>(stage + (lane & 31) * C::kOutStride + c) = epi(sum[t], sq, sw, bias, row, nb + c);
+      const float* const s = sc + BM + wn * 64 + (f & 1) * 32 + c;
+      const float4 s4 = *reinterpret_cast<const float4*>(s), t4 = *reinterpret_cast<const float4*>(s + BN);
+      const float sw[4] = {s4.x, s4.y, s4.z, s4.w}, bias[4] = {t4.x, t4.y, t4.z, t4.w};
+      *reinterpret_cast<vec4<T>*>(stage + (lane & 31) * C::kOutStride + c) = epi(sum[t], sq, sw, bias, res[t]);
     }
     __builtin_amdgcn_wave_barrier();
     if (wide) {
@@ -490,7 +507,7 @@ __global__ __launch_bounds__(512) void int8_big_kernel(Int8GemmParams p) {
         for (int j = 0; j < 4; ++j) {
           const float w4[4] = {sw[j].x, sw[j].y, sw[j].z, sw[j].w}, b4[4] = {bias[j].x, bias[j].y, bias[j].z, bias[j].w};
           *reinterpret_cast<vec4<T>*>(stage + lrow * C::kOutStride + j * 16 + lcol) =
-              epi(acc[i][half * 4 + j], sq, w4, b4, row, nh + j * 16 + lcol);
+              epi(acc[i][half * 4 + j], sq, w4, b4, epi.residual(row, nh + j * 16 + lcol));
         }
         __builtin_amdgcn_wave_barrier();
         if (wide) {
@@ -542,6 +559,22 @@ __global__ __launch_bounds__(256) void int8_stream_kernel(Int8GemmParams p) {
   const int8_t* bp[NI];
 #pragma unroll
   for (int j = 0; j < NI; ++j) bp[j] = p.w + static_cast<int64_t>(min(n0 + j * 16 + (lane & 15), p.n - 1)) * p.ldw;
+  // The wave that ends the tile has its scales, bias and residual on their way before the operands.
+  const Epilogue<T> epi(p);
+  const int64_t row = m0 + (lane & 15);
+  const bool ends = wave == 0 && p.ksplit == 1;
+  float sq = 0.0f, sw[NI][4] = {}, bias[NI][4] = {};
+  vec4<T> res[NI] = {};
+  if (ends) {
+    sq = p.sq[min(row, p.m - 1)];
+#pragma unroll
+    for (int j = 0; j < NI; ++j) {
+      const int64_t col = n0 + j * 16 + (lane >> 4) * 4;
+      epi.scales(col, sw[j], bias[j]);
+      res[j] = epi.residual(row, col);
+    }
+  }
+  __builtin_amdgcn_sched_barrier(0);
   v4i acc[NI];
 #pragma unroll
   for (int j = 0; j < NI; ++j) acc[j] = v4i{0, 0, 0, 0};
@@ -570,10 +603,7 @@ __global__ __launch_bounds__(256) void int8_stream_kernel(Int8GemmParams p) {
     for (int j = 0; j < NI; ++j) sums[wave - 1][j * 64 + lane] = acc[j];
   }
   __syncthreads();
-  if (wave != 0) return;
-  const Epilogue<T> epi(p);
-  const int64_t row = m0 + (lane & 15);
-  if (row >= p.m) return;
+  if (wave != 0 || row >= p.m) return;
 #pragma unroll
   for (int j = 0; j < NI; ++j) {
     v4i s = acc[j];
@@ -583,13 +613,15 @@ __global__ __launch_bounds__(256) void int8_stream_kernel(Int8GemmParams p) {
     if (p.ksplit > 1) {
       store_partial(p, s, split, row, col);
     } else {
-      float sw[4], bias[4];
-      epi.scales(col, sw, bias);
-      const vec4<T> o = epi(s, p.sq[row], sw, bias, row, col);
+      const vec4<T> o = epi(s, sq, sw[j], bias[j], res[j]);
       T* const y = static_cast<T*>(p.y) + row * p.n + col;
+      if ((p.n & 3) == 0) {
+        if (col < p.n) *reinterpret_cast<vec4<T>*>(y) = o;
+      } else {
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (col + r < p.n) y[r] = o[r];
+        for (int r = 0; r < 4; ++r)
+          if (col + r < p.n) y[r] = o[r];
+      }
     }
   }
 }
@@ -601,6 +633,11 @@ __global__ __launch_bounds__(256) void int8_reduce_kernel(Int8GemmParams p) {
   const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   if (i >= p.m * quads) return;
   const int64_t row = i / quads, col = (i - row * quads) * 4;
+  const Epilogue<T> epi(p);
+  float sw[4], bias[4];
+  epi.scales(col, sw, bias);
+  const float sq = p.sq[row];
+  const vec4<T> res = epi.residual(row, col);
   const int64_t plane = p.m * p.n;
   const int32_t* const s = p.partial + row * p.n + col;
   v4i acc{0, 0, 0, 0};
@@ -614,10 +651,7 @@ __global__ __launch_bounds__(256) void int8_reduce_kernel(Int8GemmParams p) {
         if (col + r < p.n) acc[r] += s[k * plane + r];
     }
   }
-  const Epilogue<T> epi(p);
-  float sw[4], bias[4];
-  epi.scales(col, sw, bias);
-  const vec4<T> o = epi(acc, p.sq[row], sw, bias, row, col);
+  const vec4<T> o = epi(acc, sq, sw, bias, res);
   T* const y = static_cast<T*>(p.y) + row * p.n + col;
   if ((p.n & 3) == 0) {
     *reinterpret_cast<vec4<T>*>(y) = o;
