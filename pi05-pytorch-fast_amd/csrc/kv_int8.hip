@@ -495,7 +495,7 @@ struct WideAttn {
 };
 
 template <typename T, int D>
-__global__ __launch_bounds__(256, 1) void kv_attn_wide_kernel(KvAttnParams p) {
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_attn_wide_kernel(KvAttnParams p) {
   using C = WideAttn<D>;
   constexpr int F = D / 32;  // 32-deep steps of Q K^T, and 32-row tiles of O^T
   extern __shared__ __align__(1024) char lds[];
@@ -768,35 +768,41 @@ hipError_t launch_kv_append(const KvAppendParams& p, int elem, hipStream_t strea
   return hipGetLastError();
 }
 
-// Runs of pages: as many as give every CU one workgroup, since a CU by itself reads no more than 65 to
-// 100 GB/s, and none where half of the CUs have one without (us, D = 256: 96 sequences of 8192 keys,
-// 16 rows, with 1 / 2 / 4 runs 116 / 80 / 92; 150 sequences 128 / 154 / 140); a run of the wide kernel
-// is at least two pages.
-// The kernel: the one with the smaller sum of these times of a round of CUs, fitted to measurements
-// (us; rows of a KV head, then narrow / wide).  D = 256: 8 x 400 rows over 826 keys 20 / 28, 1 x 2400
-// over 4096 52 / 38, 32 x 400 over 826 71 / 44.  D = 128: 16 x 200 over 2000 19 / 25, 64 x 200 over
-// 826 41 / 30.  D = 64: 2 x 6208 over 4096 38 / 60.
+// The kernel and its runs of pages: the least of the times (us, beside a launch) that these measurements
+// give: for each round of the CUs the pages of a run, and the start of a workgroup where it does not run
+// beside another (D <= 128: two on a CU); for more than one run the join, partial results at 10 TB/s.
+// Narrow: as many runs as give every CU one workgroup, since a CU by itself reads no more than 65 to
+// 100 GB/s, and none where half of the CUs have one without (D = 256, 16 rows over 8192 keys: 96
+// sequences in 1 / 2 / 4 runs 116 / 80 / 92; 150 sequences 128 / 154 / 140).  Wide: any number, of at
+// least two pages (D = 128, 2 x 6208 rows over 4096 keys in 1 / 2 / 3 / 5 / 8 runs 109 / 69 / 69 / 54 / 63).
+// Narrow / wide: D = 256, 8 x 400 rows over 826 keys 20 / 28, 1 x 2400 over 4096 52 / 38, 32 x 400 over
+// 826 71 / 44; D = 128, 16 x 200 over 2000 19 / 23, 64 x 200 over 826 41 / 28; D = 64, 2 x 6208 over 4096
+// 37 / 42, 32 x 1600 over 826 42 / 30.
 KvAttnPlan kv_attn_plan(int64_t b, int64_t t, int32_t h, int32_t kvh, int32_t d, int64_t table_pages, int cus) {
-  KvAttnPlan plan{false, 1};
   const int64_t rows = t * (h / kvh);
-  if (rows <= 0 || b <= 0 || table_pages <= 0) return plan;
+  if (rows <= 0 || b <= 0 || table_pages <= 0) return {false, 1};
   struct Cost {
-    double start, page, join;  // of a workgroup, of a page of its run, of joining runs
+    double start, page;
   };
-  const Cost narrow = d == 64 ? Cost{2.5, 0.15, 4} : d == 128 ? Cost{8, 0.3, 4} : Cost{10, 0.62, 4};
-  const Cost wide = d == 64 ? Cost{2, 1.6, 6} : d == 128 ? Cost{6, 2.2, 6} : Cost{10, 2.9, 6};
-  auto runs = [&](int64_t groups, int64_t most) {
-    const int64_t n = std::min(cus / groups, std::min(most, static_cast<int64_t>(kMaxRuns)));
-    return n < 1 ? int64_t{1} : n;
-  };
-  auto time = [&](const Cost& c, int64_t groups, int64_t n) {
-    return static_cast<double>((groups * n + cus - 1) / cus) * (c.start + c.page * static_cast<double>((table_pages + n - 1) / n)) +
-           (n > 1 ? c.join : 0);
+  const Cost narrow = d == 64 ? Cost{2.5, 0.12} : d == 128 ? Cost{8, 0.3} : Cost{10, 0.62};
+  const Cost wide = d == 64 ? Cost{4, 1.3} : d == 128 ? Cost{6, 1.65} : Cost{10, 2.9};
+  const double partial = static_cast<double>(rows) * b * kvh * d * 8 / 1e7;  // of a run, written and read
+  auto time = [&](const Cost& c, int64_t groups, int64_t n, int64_t beside) {
+    const int64_t rounds = (groups * n + cus - 1) / cus;
+    return static_cast<double>((rounds + beside - 1) / beside) * c.start +
+           static_cast<double>(rounds * ((table_pages + n - 1) / n)) * c.page + (n > 1 ? 4 + partial * static_cast<double>(n) : 0);
   };
   const int64_t few = (rows + 15) / 16 * b * kvh, many = (rows + 127) / 128 * b * kvh;
-  const int64_t nfew = runs(few, table_pages), nmany = runs(many, (table_pages + 1) / 2);
-  plan.wide = time(wide, many, nmany) < time(narrow, few, nfew);
-  plan.nsplit = static_cast<int>(plan.wide ? nmany : nfew);
+  const int64_t n = std::max<int64_t>(std::min({cus / few, table_pages, int64_t{kMaxRuns}}), 1);
+  KvAttnPlan plan{false, static_cast<int>(n)};
+  double best = time(narrow, few, n, 1);
+  for (int r = 1; r <= kMaxRuns && (r == 1 || 2 * (r - 1) < table_pages); ++r) {
+    const double us = time(wide, many, r, d == 256 ? 1 : 2);
+    if (us < best) {
+      best = us;
+      plan = {true, r};
+    }
+  }
   return plan;
 }
 
