@@ -642,7 +642,7 @@ __global__ __launch_bounds__(256) void int8_reduce_kernel(Int8GemmParams p) {
   const int32_t* const s = p.partial + row * p.n + col;
   v4i acc{0, 0, 0, 0};
   if ((p.n & 3) == 0) {
-#pragma unroll 4
+#pragma unroll 8
     for (int k = 0; k < p.ksplit; ++k) acc += *reinterpret_cast<const v4i*>(s + k * plane);
   } else {
     for (int k = 0; k < p.ksplit; ++k) {
