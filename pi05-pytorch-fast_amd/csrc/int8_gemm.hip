@@ -109,9 +109,10 @@ struct Int8Tile {
 
 // Two waves a SIMD in the bounds: the accumulators then stay in ordinary registers (given twice as
 // many, the compiler moves them to the accumulation registers and back in every step).
-// Measured (us, 2048 deep, 2560 columns): 100 rows 8.5, 776 rows 14; a 64 x 64 step of a CU costs
-// 0.25 us, a 128 x 64 step 0.36, where its MFMAs alone take 0.07 and 0.13: the steps are bound by the
-// issue of their loads and reads.
+// Measured (us, 2048 deep, 2560 columns): 128 rows 8.4, 776 rows 14.1 (6 of them for one step and the
+// ends); a 64 x 64 step of a CU costs 0.25 us, a 128 x 64 step 0.36, where its MFMAs alone take 0.07
+// and 0.13: the steps are bound by the operands' way to the CU, 16 or 24 KB at 64 to 67 GB/s, and no
+// deeper ring (four stages) helps.
 template <typename T, int BM, int BN, int KW, int ST>
 __global__ __launch_bounds__(64 * (BM / 64) * (BN / 64) * KW, 2) void int8_tile_kernel(Int8GemmParams p) {
   using C = Int8Tile<BM, BN, KW, ST>;

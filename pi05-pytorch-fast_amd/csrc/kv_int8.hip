@@ -32,8 +32,8 @@ __device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) {
 //   s = max(s0, max|new| / 127 + 1e-12),  s0 the scale of the tokens that are there (0: none),
 // brings the old codes to it where it grew, c' = rint(c (s0 / s)), and writes the new ones,
 // c = rint(x (1 / s)).  A page whose first token is new is written whole, zeros behind the last
-// token, so that nothing of the page's earlier owner is left.  Bound by latency for single
-// tokens (lens -> table -> scale, one after the other) and by HBM for prefixes.
+// token, so that nothing of the page's earlier owner is left.  Bound by latency (lens -> table -> scale ->
+// codes, one after the other): 16 x 1 tokens 6.8 us, 8 x 776 tokens 6.8 (9.5 MB, 1.4 TB/s).
 template <typename T, int D>
 __global__ __launch_bounds__(256) void kv_append_kernel(KvAppendParams p) {
   // A thread holds kRows consecutive page rows of eight consecutive dimensions, so that a V row (one
@@ -303,6 +303,9 @@ __device__ __forceinline__ void store_sums(const KvAttnParams& p, float m, float
 // t's row 4 a + r is key 16 a + 4 t + r, so that over the four tiles of a page the lane holds
 // keys 16 (L / 16) .. + 15: the 16 bytes that it loads of a V row.
 // A page's values are requested before its scores, the next page's keys as the values are used up.
+// Bound by the cache's bytes: 64 sequences of up to 8192 keys, 8 heads on one of D = 256, 45 us for 202
+// MB, 4.5 TB/s where plain reads reach 6.3; a single sequence by the chain length, table entry, scales
+// and keys, queries (776 keys: 6.8 us, and 3.2 of the join).
 template <typename T, int D, int W>
 __global__ __launch_bounds__(64 * W, 2) void kv_attn_kernel(KvAttnParams p) {
   constexpr int F = D / 64, DT = D / 16;
@@ -470,13 +473,20 @@ __global__ __launch_bounds__(64 * W, 2) void kv_attn_kernel(KvAttnParams p) {
 // ------------------------------------------------------------------ attention of many rows
 // Four waves of 32 query rows; the pages of the run come through an LDS ring of three by direct
 // loads, each read once for 128 rows.  32 x 32 matrix instructions, which one wave a SIMD feeds at
-// their rate (accumulators 128 registers and queries 64 leave no room for a second one).
+// their rate; at D = 256 accumulators (128 registers) and queries (64) leave no room for a second one,
+// below that two workgroups share a CU (D = 128: 8 x 50 tokens of 32 heads on 8 over 826 keys 30 -> 28 us,
+// 1 x 776 tokens 32.6 -> 29.5).
 //
 // Lane L holds query row L % 32 and, of a 32-key S^T tile, the tile rows 8 a + 4 (L / 32) + r.  Tile
 // t's row 8 a + 4 h + r is key 32 h + 16 t + 4 a + r, so that the lane holds keys 32 (L / 32) .. + 31,
 // and eight consecutive of them are what it gives to one 16-deep step of P V: 32 bytes of a V row.
 // LDS: 16-byte chunk c of key row k is kept at c ^ swizzle(k), and of a V row likewise, so that
 // eight lanes that read one chunk of their rows meet eight different bank groups.
+// 2 x 776 tokens of 8 heads on one over 4096 keys, D = 256: 97 us, 400 TFLOP/s where a large fp16 product
+// reaches 1154.  Bound by a wave's own instructions: of the 5700 clocks of a page half are vector
+// instructions (softmax, value codes to fp16), a third MFMAs, the rest waits, one after the other.  The
+// next page's scores issued beside the softmax (107 us) and values converted once for the four waves
+// (109) gain nothing: the waves walk in step.
 typedef int v16i __attribute__((ext_vector_type(16)));
 typedef float v16f __attribute__((ext_vector_type(16)));
 
@@ -746,9 +756,11 @@ void launch_attn(const KvAttnParams& p, hipStream_t stream) {
   if (p.wide) {
     kv_attn_wide_kernel<T, D><<<grid, 256, WideAttn<D>::kLds, stream>>>(p);
   } else {
-    // A wave for every page of a run, or for every fourth of a long one.
+    // Four waves from six pages of a run on, two from two pages on (D = 256, us with 8 / 4 / 2 / 1 waves: 13
+    // pages 20.5 / 18.3 / 18.9 / 27.2, 4 pages 15.7 / 15.3 / 15.2 / 16.6, 1 page - / - / 10.5 / 9.9; D = 128, 32
+    // pages 18.7 / 17.8 / 24.6 / 42).
     const int run = (p.c.table_pages + p.nsplit - 1) / p.nsplit;
-    if (run >= 6) kv_attn_kernel<T, D, 8><<<grid, 64 * 8, 8 * D * 64, stream>>>(p);
+    if (run >= 6) kv_attn_kernel<T, D, 4><<<grid, 64 * 4, 4 * D * 64, stream>>>(p);
     else if (run >= 2) kv_attn_kernel<T, D, 2><<<grid, 64 * 2, 2 * D * 64, stream>>>(p);
     else kv_attn_kernel<T, D, 1><<<grid, 64, 0, stream>>>(p);
   }
@@ -781,38 +793,38 @@ hipError_t launch_kv_append(const KvAppendParams& p, int elem, hipStream_t strea
 
 // The kernel and its runs of pages: the least of the times (us, beside a launch) that these measurements
 // give: for each round of the CUs the pages of a run, and the start of a workgroup where it does not run
-// beside another (D <= 128: two on a CU); for more than one run the join, partial results at 10 TB/s.
-// Narrow: as many runs as give every CU one workgroup, since a CU by itself reads no more than 65 to
-// 100 GB/s, and none where half of the CUs have one without (D = 256, 16 rows over 8192 keys: 96
-// sequences in 1 / 2 / 4 runs 116 / 80 / 92; 150 sequences 128 / 154 / 140).  Wide: any number, of at
-// least two pages (D = 128, 2 x 6208 rows over 4096 keys in 1 / 2 / 3 / 5 / 8 runs 109 / 69 / 69 / 54 / 63).
-// Narrow / wide: D = 256, 8 x 400 rows over 826 keys 20 / 28, 1 x 2400 over 4096 52 / 38, 32 x 400 over
-// 826 71 / 44; D = 128, 16 x 200 over 2000 19 / 23, 64 x 200 over 826 41 / 28; D = 64, 2 x 6208 over 4096
+// beside another (the wide kernel at D <= 128: two on a CU); for more than one run the join, partial
+// results at 10 TB/s.
+// Narrow, D = 256, 16 rows over 8192 keys in 1 / 2 / 3 / 4 / 8 runs: 64 sequences 104 / 65 / 54 / 54 / 57,
+// 96 121 / 77 / 104 / 87 / 83, 150 130 / 150 / 120 / 130 / 129, 300 290 / 245 / 238 / 234 / 249.  Wide, D = 128, 2 x 6208
+// rows over 4096 keys in 1 / 2 / 3 / 5 / 8 runs: 109 / 69 / 69 / 54 / 63.
+// Narrow / wide: D = 256, 8 x 400 rows over 826 keys 18 / 28, 1 x 2400 over 4096 52 / 38, 32 x 400 over
+// 826 71 / 44; D = 128, 16 x 200 over 2000 18 / 23, 64 x 200 over 826 41 / 28; D = 64, 2 x 6208 over 4096
 // 37 / 42, 32 x 1600 over 826 42 / 30.
 KvAttnPlan kv_attn_plan(int64_t b, int64_t t, int32_t h, int32_t kvh, int32_t d, int64_t table_pages, int cus) {
+  KvAttnPlan plan{false, 1};
   const int64_t rows = t * (h / kvh);
-  if (rows <= 0 || b <= 0 || table_pages <= 0) return {false, 1};
+  if (rows <= 0 || b <= 0 || table_pages <= 0) return plan;
   struct Cost {
     double start, page;
   };
   const Cost narrow = d == 64 ? Cost{2.5, 0.12} : d == 128 ? Cost{8, 0.3} : Cost{10, 0.62};
   const Cost wide = d == 64 ? Cost{4, 1.3} : d == 128 ? Cost{6, 1.65} : Cost{10, 2.9};
   const double partial = static_cast<double>(rows) * b * kvh * d * 8 / 1e7;  // of a run, written and read
-  auto time = [&](const Cost& c, int64_t groups, int64_t n, int64_t beside) {
-    const int64_t rounds = (groups * n + cus - 1) / cus;
-    return static_cast<double>((rounds + beside - 1) / beside) * c.start +
-           static_cast<double>(rounds * ((table_pages + n - 1) / n)) * c.page + (n > 1 ? 4 + partial * static_cast<double>(n) : 0);
-  };
   const int64_t few = (rows + 15) / 16 * b * kvh, many = (rows + 127) / 128 * b * kvh;
-  const int64_t n = std::max<int64_t>(std::min({cus / few, table_pages, int64_t{kMaxRuns}}), 1);
-  KvAttnPlan plan{false, static_cast<int>(n)};
-  double best = time(narrow, few, n, 1);
-  for (int r = 1; r <= kMaxRuns && (r == 1 || 2 * (r - 1) < table_pages); ++r) {
-    const double us = time(wide, many, r, d == 256 ? 1 : 2);
+  double best = 1e300;
+  auto consider = [&](bool is_wide, const Cost& c, int64_t groups, int n, int beside) {
+    const int64_t rounds = (groups * n + cus - 1) / cus;
+    const double us = static_cast<double>((rounds + beside - 1) / beside) * c.start +
+                      static_cast<double>(rounds * ((table_pages + n - 1) / n)) * c.page + (n > 1 ? 4 + partial * n : 0);
     if (us < best) {
       best = us;
-      plan = {true, r};
+      plan = {is_wide, n};
     }
+  };
+  for (int n = 1; n <= kMaxRuns && n <= table_pages; ++n) {
+    consider(false, narrow, few, n, 1);
+    if (n == 1 || 2 * (n - 1) < table_pages) consider(true, wide, many, n, d == 256 ? 1 : 2);  // two pages at least
   }
   return plan;
 }
