@@ -25,16 +25,19 @@ typedef int v4i __attribute__((ext_vector_type(4)));
 typedef int v16i __attribute__((ext_vector_type(16)));
 template <typename T>
 using vec4 = T __attribute__((ext_vector_type(4)));
+// The same at the alignment of their elements: rows of an N that is no multiple of a vector (one
+// access all the same: 1071 x 2048 x 15980 57 us, in elements 76).
+typedef int v4i_w __attribute__((ext_vector_type(4), aligned(4)));
+typedef int v4i_h __attribute__((ext_vector_type(4), aligned(2)));
+template <typename T>
+using vec4_h = T __attribute__((ext_vector_type(4), aligned(2)));
 
 // y[row, col .. col + 3] of one accumulator quad, with the bias and (RES) the residual: fp32, one
 // rounding.
 template <typename T, bool RES = true>
 struct Epilogue {
   const Int8GemmParams& p;
-  bool res_vec;  // residual quads can be read as one aligned load
-  __device__ explicit Epilogue(const Int8GemmParams& q) : p(q) {
-    res_vec = (q.n & 3) == 0 && (q.ldr & 3) == 0 && (reinterpret_cast<uintptr_t>(q.res) & 7) == 0;
-  }
+  __device__ explicit Epilogue(const Int8GemmParams& q) : p(q) {}
   __device__ __forceinline__ void scales(int64_t col, float (&sw)[4], float (&bias)[4]) const {
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -47,8 +50,8 @@ struct Epilogue {
     vec4<T> v{};
     if (RES && p.res != nullptr && row < p.m) {
       const T* const rp = static_cast<const T*>(p.res) + row * p.ldr + col;
-      if (res_vec) {
-        if (col < p.n) v = *reinterpret_cast<const vec4<T>*>(rp);
+      if (col + 4 <= p.n) {
+        v = *reinterpret_cast<const vec4_h<T>*>(rp);
       } else {
 #pragma unroll
         for (int r = 0; r < 4; ++r)
@@ -73,12 +76,22 @@ struct Epilogue {
 __device__ __forceinline__ void store_partial(const Int8GemmParams& p, const v4i s, int split, int64_t row, int64_t col) {
   if (row >= p.m) return;
   int32_t* const o = p.partial + (split * p.m + row) * p.n + col;
-  if ((p.n & 3) == 0) {
-    if (col < p.n) *reinterpret_cast<v4i*>(o) = s;
+  if (col + 4 <= p.n) {
+    *reinterpret_cast<v4i_w*>(o) = s;
   } else {
 #pragma unroll
     for (int r = 0; r < 4; ++r)
       if (col + r < p.n) o[r] = s[r];
+  }
+}
+
+// Eight staged columns of an output row, of which `left` (or fewer than none) are there.
+template <typename T>
+__device__ __forceinline__ void store_chunk(T* y, const T* staged, int left) {
+  if (left >= 8) {
+    *reinterpret_cast<v4i_h*>(y) = *reinterpret_cast<const v4i*>(staged);
+  } else {
+    for (int e = 0; e < left; ++e) y[e] = staged[e];
   }
 }
 
@@ -285,7 +298,6 @@ __global__ __launch_bounds__(64 * (BM / 64) * (BN / 64) * KW, 2) void int8_tile_
   }
   const Epilogue<T> epi(p);
   T* const y = static_cast<T*>(p.y);
-  const bool wide = (p.n & 7) == 0;
 #pragma unroll
   for (int f = 0; f < 4; ++f) {
     if (f / C::kOwn != kg) continue;
@@ -322,18 +334,10 @@ __global__ __launch_bounds__(64 * (BM / 64) * (BN / 64) * KW, 2) void int8_tile_
       *reinterpret_cast<vec4<T>*>(stage + (lane & 31) * C::kOutStride + c) = epi(sum[t], sq, sw, bias, res[t]);
     }
     __builtin_amdgcn_wave_barrier();
-    if (wide) {
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const int r = s * 16 + (lane >> 2), c = (lane & 3) * 8;
-        if (mb + r < p.m && nb + c < p.n)
-          *reinterpret_cast<v4i*>(y + (mb + r) * p.n + nb + c) = *reinterpret_cast<const v4i*>(stage + r * C::kOutStride + c);
-      }
-    } else {
-      for (int e = lane; e < 32 * 32; e += 64) {
-        const int r = e >> 5, c = e & 31;
-        if (mb + r < p.m && nb + c < p.n) y[(mb + r) * p.n + nb + c] = stage[r * C::kOutStride + c];
-      }
+    for (int s = 0; s < 2; ++s) {
+      const int r = s * 16 + (lane >> 2), c = (lane & 3) * 8;
+      if (mb + r < p.m) store_chunk(y + (mb + r) * p.n + nb + c, stage + r * C::kOutStride + c, p.n - nb - c);
     }
     __builtin_amdgcn_wave_barrier();
   }
@@ -511,21 +515,22 @@ __global__ __launch_bounds__(512) void int8_big_kernel(Int8GemmParams p) {
               epi(acc[i][half * 4 + j], sq, w4, b4, epi.residual(row, nh + j * 16 + lcol));
         }
         __builtin_amdgcn_wave_barrier();
+        // Past the L2, which the operands need: 248 -> 238 us at 6208 x 2048 x 16384.  Whole chunks at
+        // once where N allows (206 us against 214 through the other form).
         if (wide) {
 #pragma unroll
           for (int s = 0; s < 2; ++s) {
             const int r = s * 8 + (l >> 3), c = (l & 7) * 8;
             const int64_t orow = mw + i * 16 + r;
-            // Past the L2, which the operands need: 248 -> 238 us at 6208 x 2048 x 16384.
             if (orow < p.m && nh + c < p.n)
               __builtin_nontemporal_store(*reinterpret_cast<const v4i*>(stage + r * C::kOutStride + c),
                                           reinterpret_cast<v4i*>(y + orow * p.n + nh + c));
           }
         } else {
-          for (int e = l; e < 16 * 64; e += 64) {
-            const int r = e >> 6, c = e & 63;
+          for (int s = 0; s < 2; ++s) {
+            const int r = s * 8 + (l >> 3), c = (l & 7) * 8;
             const int64_t orow = mw + i * 16 + r;
-            if (orow < p.m && nh + c < p.n) y[orow * p.n + nh + c] = stage[r * C::kOutStride + c];
+            if (orow < p.m) store_chunk(y + orow * p.n + nh + c, stage + r * C::kOutStride + c, p.n - nh - c);
           }
         }
         __builtin_amdgcn_wave_barrier();
@@ -616,8 +621,8 @@ __global__ __launch_bounds__(256) void int8_stream_kernel(Int8GemmParams p) {
     } else {
       const vec4<T> o = epi(s, sq, sw[j], bias[j], res[j]);
       T* const y = static_cast<T*>(p.y) + row * p.n + col;
-      if ((p.n & 3) == 0) {
-        if (col < p.n) *reinterpret_cast<vec4<T>*>(y) = o;
+      if (col + 4 <= p.n) {
+        *reinterpret_cast<vec4_h<T>*>(y) = o;
       } else {
 #pragma unroll
         for (int r = 0; r < 4; ++r)
@@ -642,9 +647,9 @@ __global__ __launch_bounds__(256) void int8_reduce_kernel(Int8GemmParams p) {
   const int64_t plane = p.m * p.n;
   const int32_t* const s = p.partial + row * p.n + col;
   v4i acc{0, 0, 0, 0};
-  if ((p.n & 3) == 0) {
+  if (col + 4 <= p.n) {
 #pragma unroll 8
-    for (int k = 0; k < p.ksplit; ++k) acc += *reinterpret_cast<const v4i*>(s + k * plane);
+    for (int k = 0; k < p.ksplit; ++k) acc += *reinterpret_cast<const v4i_w*>(s + k * plane);
   } else {
     for (int k = 0; k < p.ksplit; ++k) {
 #pragma unroll
@@ -654,8 +659,8 @@ __global__ __launch_bounds__(256) void int8_reduce_kernel(Int8GemmParams p) {
   }
   const vec4<T> o = epi(acc, sq, sw, bias, res);
   T* const y = static_cast<T*>(p.y) + row * p.n + col;
-  if ((p.n & 3) == 0) {
-    *reinterpret_cast<vec4<T>*>(y) = o;
+  if (col + 4 <= p.n) {
+    *reinterpret_cast<vec4_h<T>*>(y) = o;
   } else {
 #pragma unroll
     for (int r = 0; r < 4; ++r)
@@ -728,16 +733,17 @@ Int8GemmPlan int8_gemm_plan(int64_t m, int32_t n, int32_t k, int cus) {
     return plan;
   }
   // The least of the times (us, beside a launch) that these measurements give, 128 bytes of K a step
-  // and w workgroups on the CUs: 64 x 64 tiles 0.25 a step and workgroup of a CU (2048 deep, 2560
-  // columns: 200 rows 8.7 us, 1500 rows 20.2), 128 x 64 tiles 0.36 (10.9, 15.7), 256 x 256 tiles 1.4 a
-  // step and round of CUs, and 2 for their longer ends (27.2, 28.0; 776 rows x 16384 columns 31.4 us,
-  // against 54.4 and 49.6).  A K slice shortens the steps and costs the sums' way through memory.
+  // and w workgroups on the CUs: 64 x 64 tiles 0.25 a step and workgroup of a CU and 1 for its end (2048
+  // deep, 2560 columns: 128 rows 8.4 us, 1500 rows 21), 128 x 64 tiles 0.36 and 2 (11, 17), 256 x 256 tiles 1.4
+  // a step and 6 for the end of a round of CUs (26, 28; 776 rows x 16384 columns 31.7 us, against 55 and
+  // 49; 3355 rows, 256 deep, 2608 columns 12.5, against 16.6 and 16.4).  A K slice shortens the steps and costs
+  // the sums' way through memory.
   const double steps = (k + 127) / 128;
   double best = 1e30;
-  auto consider = [&](int tile, int64_t w, double step_us, int ks) {
+  auto consider = [&](int tile, int64_t w, double step_us, double end_us, int ks) {
     if (w * ks >= 1 << 24) return;  // a launch holds fewer than 2^32 threads
     const double load = static_cast<double>(w) * ks / cus;
-    const double us = (steps / ks) * step_us * (load < 1 ? 1 : load) +
+    const double us = ((steps / ks) * step_us + end_us) * (load < 1 ? 1 : load) +
                       (ks > 1 ? 3.0 + static_cast<double>(m) * n * (8.0 * ks + 2) / 5e6 : 0.0);
     if (us < best) {
       best = us;
@@ -747,11 +753,11 @@ Int8GemmPlan int8_gemm_plan(int64_t m, int32_t n, int32_t k, int cus) {
   };
   for (int ks = 1; ks <= 8; ks *= 2) {
     if (ks > 1 && steps / ks < 8) break;
-    consider(kTile64, ((m + 63) / 64) * ((n + 63) / 64), 0.25, ks);
-    consider(kTile128x64, ((m + 127) / 128) * ((n + 63) / 64), 0.36, ks);
+    consider(kTile64, ((m + 63) / 64) * ((n + 63) / 64), 0.25, 1, ks);
+    consider(kTile128x64, ((m + 127) / 128) * ((n + 63) / 64), 0.36, 2, ks);
   }
   const int64_t big = ((m + 255) / 256) * ((n + 255) / 256);
-  if (2.0 + steps * 1.4 * static_cast<double>((big + cus - 1) / cus) < best) plan = {kBig, 1};
+  if ((steps * 1.4 + 6) * static_cast<double>((big + cus - 1) / cus) < best) plan = {kBig, 1};
   return plan;
 }
 
