@@ -791,6 +791,9 @@ hipError_t launch_kv_append(const KvAppendParams& p, int elem, hipStream_t strea
   return hipGetLastError();
 }
 
+// No call asks for more partial results than the Infinity Cache holds.
+constexpr size_t kMaxPartial = size_t{1} << 28;
+
 // The kernel and its runs of pages: the least of the times (us, beside a launch) that these measurements
 // give: for each round of the CUs the pages of a run, and the start of a workgroup where it does not run
 // beside another (the wide kernel at D <= 128: two on a CU); for more than one run the join, partial
@@ -823,6 +826,7 @@ KvAttnPlan kv_attn_plan(int64_t b, int64_t t, int32_t h, int32_t kvh, int32_t d,
     }
   };
   for (int n = 1; n <= kMaxRuns && n <= table_pages; ++n) {
+    if (n > 1 && kv_attn_workspace(b, t, h, d, n) > kMaxPartial) break;
     consider(false, narrow, few, n, 1);
     if (n == 1 || 2 * (n - 1) < table_pages) consider(true, wide, many, n, d == 256 ? 1 : 2);  // two pages at least
   }

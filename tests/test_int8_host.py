@@ -144,3 +144,9 @@ def test_attention_workspace_is_checked(lib):
     assert need > 0
     assert _attend(lib, h=8, d=256, tp=128, pages=128, ws=P, wsb=need - 4) == 3 and "workspace" in _err(lib)
     assert lib.pi05w4a4_int8_kv_attention_workspace_bytes(1, 1, 8, 1, 256, 0) == 0
+
+
+@pytest.mark.parametrize("b,t,h,kvh,d,pages", [(1, 8320, 8, 1, 256, 2048), (1, 1, 8, 1, 256, 1 << 24), (3, 2000, 32, 8, 128, 4000),
+                                               (65535, 1, 32767, 32767, 64, 1), (1, 1 << 24, 4, 1, 64, 1 << 24)])
+def test_attention_workspace_is_bounded(lib, b, t, h, kvh, d, pages):
+    assert lib.pi05w4a4_int8_kv_attention_workspace_bytes(b, t, h, kvh, d, pages) <= 1 << 28
