@@ -164,6 +164,20 @@ def test_product_of_many_tiles(cuda, m, k, n, t):
         _check_product(y[part], args[0][part], args[1][part], args[2], args[3], args[4], args[5][part])
 
 
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("m,k,n", [(4, 16384, 67), (70, 16384, 67), (200, 8192, 129), (900, 512, 771), (300, 256, 2), (5000, 256, 4099)])
+def test_product_of_odd_rows(cuda, m, k, n, t):
+    """Output rows, K slices and residual rows that begin at any element."""
+    q, sq, w, sw, bias, res = _product(_gen(m + n), m, k, n, t, True, True)
+    want = i8.int8_gemm(q, sq, w, sw, bias, res, out_dtype=t)
+    _check_product(want, q, sq, w, sw, bias, res)
+    wide = torch.zeros((m, n + 6), dtype=t, device="cuda")
+    wide[:, 3:n + 3] = res
+    odd_bias = torch.zeros(n + 1, dtype=t, device="cuda")
+    odd_bias[1:] = bias
+    assert torch.equal(i8.int8_gemm(q, sq, w, sw, odd_bias[1:], wide[:, 3:n + 3], out_dtype=t), want)
+
+
 def test_product_of_more_rows_than_a_launch_has_tiles(cuda):
     m, k, n = (1 << 30) + 100, 16, 8
     q = torch.empty((m, k), dtype=torch.int8, device="cuda")
