@@ -463,7 +463,7 @@ int pi05w4a4_gemm_e3m2_rows(const void* q6, const float* sa, int64_t m, int32_t 
  *     (unit_offset) or w, with h = x, or, with a residual (row stride ldr), h = x + residual
  *     rounded to the element type and written to h_out [M, K].
  *     scale = max|y| / 127 + 1e-12, q = rint(y / scale).  A row with a NaN or an infinity:
- *     scale NaN, codes 0.
+ *     scale NaN, codes 0.  M < 2^26 up to K = 2048, 2^24 up to 8192, else 2^22 (one launch).
  * pi05w4a4_int8_gemm: y[m, n] = (sum_k q[m, k] w[n, k]) * sq[m] * sw[n] + bias[n] +
  *   residual[m, n], in fp32 with one rounding; bias and residual may be null.  q and w have
  *   row strides ldq, ldw (bytes, % 16 == 0; rows 16-byte aligned), K % 16 == 0, K <= 65536;
@@ -480,14 +480,14 @@ int pi05w4a4_gemm_e3m2_rows(const void* q6, const float* sa, int64_t m, int32_t 
  *   (% 8 == 0), 16-byte aligned.  The scale of a page is the largest that its tokens needed,
  *   max|.| / 127 + 1e-12; where it grows, the page's earlier codes are rounded to it.  A page
  *   whose first token is new is written whole, zeros behind the last token.  Tokens past
- *   table_pages * 64 are dropped.  lens is read only.  A page may be written for one sequence
- *   at a time.
+ *   table_pages * 64 are dropped.  lens is read only.  A page may be written from one place
+ *   of the table only.
  * pi05w4a4_int8_kv_attention: out [B, T, H, D] = softmax(scaling q K^T) V over the tokens that
  *   query i of sequence b sees: with ql = q_lens[b] (null: T), the first lens[b] - ql + i + 1
  *   when causal, else lens[b]; none for i >= ql.  lens counts the new tokens too.  A query
  *   that sees none gets zeros.  lse, when not null, fp32 [B, T, H]: the natural log of the sum
  *   of exp(scaling q k) (-inf where none is seen).  Query head h reads KV head h / (H / KVH).
- *   Needs pi05w4a4_int8_kv_attention_workspace_bytes(...) bytes (0 without a split).
+ *   Needs pi05w4a4_int8_kv_attention_workspace_bytes(...) bytes (0 without a split, at most 2^28).
  */
 #define PI05W4A4_FP16 0
 #define PI05W4A4_BF16 1

@@ -2,12 +2,12 @@
 //
 //   y[m, n] = T( float(sum_k q[m, k] w[n, k]) * sq[m] * sw[n] + bias[n] + residual[m, n] )
 //
-// on v_mfma_i32_16x16x64_i8: the int32 sums are exact (K <= 65536), so neither tile, nor K split, nor
+// on the int8 MFMAs: the int32 sums are exact (K <= 65536), so neither tile, nor K split, nor
 // order changes a result; the epilogue runs in fp32 and rounds once.  Both operands are row-major
 // with K contiguous, as the quantizer writes them: no layout of the weights' own.
 //
 // The weights are MFMA operand A, so that a lane ends with four consecutive columns of one row.
-// In a 64-deep step lane L holds k = 16 (L / 16) .. + 15 of row L % 16 of either operand.
+// In a step of v_mfma_i32_16x16x64_i8 lane L holds k = 16 (L / 16) .. + 15 of row L % 16 of either operand.
 //
 // Three kernels:
 //   int8_stream_kernel  up to 16 rows: the weights stream from memory straight into registers,

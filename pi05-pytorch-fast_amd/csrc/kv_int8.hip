@@ -2,8 +2,8 @@
 // have their own), the append that writes it and the attention that reads it.
 //
 // Layout: K codes [pages, KVH, 64, D]; V codes transposed within the page, [pages, KVH, D, 64].  The
-// attention computes S^T = K Q^T and O^T = V^T P^T on 16-row matrix instructions whose operands
-// are 16-byte loads of consecutive codes of either array: no transposes, no LDS for the cache.
+// attention computes S^T = K Q^T and O^T = V^T P^T on matrix instructions whose operands are 16-byte
+// loads of consecutive codes of either array: no transposes.
 
 #include "direct_load.h"
 #include <algorithm>
