@@ -429,7 +429,7 @@ __global__ __launch_bounds__(512) void int8_big_kernel(Int8GemmParams p) {
   const int aoff = wm * 64 * 128 + roff, boff = 32768 + wn * 128 * 128 + roff;
   const Epilogue<T, RES> epi(p);
   float* const sc = reinterpret_cast<float*>(lds + C::kScale);
-  const bool wide = (p.n & 7) == 0;
+  const bool lines = (p.n & 63) == 0;  // output rows are whole 128-byte lines
 
   Tile cur = tile_at(t);
   load_tile(cur);
@@ -515,9 +515,9 @@ __global__ __launch_bounds__(512) void int8_big_kernel(Int8GemmParams p) {
               epi(acc[i][half * 4 + j], sq, w4, b4, epi.residual(row, nh + j * 16 + lcol));
         }
         __builtin_amdgcn_wave_barrier();
-        // Past the L2, which the operands need: 248 -> 238 us at 6208 x 2048 x 16384.  Whole chunks at
-        // once where N allows (206 us against 214 through the other form).
-        if (wide) {
+        // Whole lines go past the L2, which the operands need (us, past / through: 6208 x 2048 x 16384 212 / 218,
+        // x 2560 32.5 / 35), parts of lines through it (1071 x 2048 x 15984 63 / 56).
+        if (lines) {
 #pragma unroll
           for (int s = 0; s < 2; ++s) {
             const int r = s * 8 + (l >> 3), c = (l & 7) * 8;

@@ -154,14 +154,17 @@ def test_product(cuda, m, k, n, t):
 
 
 @pytest.mark.parametrize("t", TYPES)
-@pytest.mark.parametrize("m,k,n", [(4200, 1040, 4200), (8192, 112, 8201), (2600, 16, 2568), (4100, 2048, 4097)])
+@pytest.mark.parametrize("m,k,n", [(4200, 1040, 4200), (8192, 112, 8201), (2600, 16, 2568), (4100, 2048, 4097),
+                                   (4100, 272, 4160), (3355, 256, 2624)])
 def test_product_of_many_tiles(cuda, m, k, n, t):
     """More large tiles than CUs, the last of a row, column and K ragged, and K of a single step."""
-    args = _product(_gen(m + k + n), m, k, n, t, True, True)
-    y = i8.int8_gemm(*args[:4], bias=args[4], residual=args[5], out_dtype=t)
+    q, sq, w, sw, bias, res = _product(_gen(m + k + n), m, k, n, t, True, True)
+    y = i8.int8_gemm(q, sq, w, sw, bias, res, out_dtype=t)
+    plain = i8.int8_gemm(q, sq, w, sw, out_dtype=t)
     for r in range(0, m, 1024):  # rows at a time: the 64-bit products
         part = slice(r, r + 1024)
-        _check_product(y[part], args[0][part], args[1][part], args[2], args[3], args[4], args[5][part])
+        _check_product(y[part], q[part], sq[part], w, sw, bias, res[part])
+        _check_product(plain[part], q[part], sq[part], w, sw, None, None)
 
 
 @pytest.mark.parametrize("t", TYPES)
