@@ -462,8 +462,8 @@ int pi05w4a4_gemm_e3m2_rows(const void* q6, const float* sa, int64_t m, int32_t 
  *     norm_w == NULL: y = x.  Otherwise y = h * g / sqrt(mean(h^2) + eps), g = 1 + w
  *     (unit_offset) or w, with h = x, or, with a residual (row stride ldr), h = x + residual
  *     rounded to the element type and written to h_out [M, K].
- *     scale = max|y| / 127 + 1e-12, q = rint(y / scale).  A row with a NaN or an infinity:
- *     scale NaN, codes 0.  M < 2^26 up to K = 2048, 2^24 up to 8192, else 2^22 (one launch).
+ *     scale = max|y| / 127 + 1e-12, q = rint(y / scale).  A row with a NaN or an infinity, in y
+ *     too: scale NaN, codes 0; finite rows whose squares leave fp32's range have their y.  M < 2^26 up to K = 2048, 2^24 up to 8192, else 2^22 (one launch).
  * pi05w4a4_int8_gemm: y[m, n] = (sum_k q[m, k] w[n, k]) * sq[m] * sw[n] + bias[n] +
  *   residual[m, n], in fp32 with one rounding; bias and residual may be null.  q and w have
  *   row strides ldq, ldw (bytes, % 16 == 0; rows 16-byte aligned), K % 16 == 0, K <= 65536;

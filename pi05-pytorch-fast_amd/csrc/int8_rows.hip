@@ -11,6 +11,9 @@
 // fp32 throughout; nothing is rounded between the norm and the code.
 // The maximum is taken of the bits of |h g| as integers, in which a NaN is larger than every
 // number: a row that holds a NaN or an infinity gets the scale NaN and codes 0.
+// bf16 rows can leave fp32's range in h^2 or h g where y does not.  Such a row is read again, its squares are
+// taken of h 2^96 or h 2^-96, and it goes on as the rows y themselves with r = 1; only a y past fp32 makes the
+// scale NaN.
 //
 // Bound by HBM: 7 bytes an element in the add form, 3 in the others; 6208 x 2048 with the add take 17.0
 // us, 5.2 TB/s, where a copy reaches 4.96.  A row belongs to one wave (K <= 2048 and enough rows) or to
@@ -38,6 +41,7 @@ __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
 }
 
 constexpr float kRintMagic = 12582912.0f;  // 1.5 * 2^23
+constexpr float kMax = 3.4028235e38f;
 
 // WPR waves share a row; a thread holds CPT chunks of 8 elements, chunk j * 64 WPR + its index.
 template <typename T, bool NORM, bool ADD, int WPR, int CPT>
@@ -88,28 +92,69 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void int8_rows_kernel(In
       if (c < chunks) top = max(top, __float_as_uint(f[j][e]) & 0x7fffffffu);
     }
   }
-  top = wave_max_u32(top);
-  if constexpr (NORM) ss = wave_sum_f(ss);
-  if constexpr (WPR > 1) {
-    __shared__ float red_ss[WPR];
-    __shared__ uint32_t red_top[WPR];
-    if (lane == 0) {
-      red_ss[wave] = ss;
-      red_top[wave] = top;
-    }
-    __syncthreads();
-    ss = red_ss[0];
-    top = red_top[0];
+  // Over the waves of the row; every thread holds the results.
+  __shared__ float red_ss[WPR];
+  __shared__ uint32_t red_top[WPR];
+  auto reduce = [&]() {
+    top = wave_max_u32(top);
+    if constexpr (NORM) ss = wave_sum_f(ss);
+    if constexpr (WPR > 1) {
+      if (lane == 0) {
+        red_ss[wave] = ss;
+        red_top[wave] = top;
+      }
+      __syncthreads();
+      ss = red_ss[0];
+      top = red_top[0];
 #pragma unroll
-    for (int i = 1; i < WPR; ++i) {
-      ss += red_ss[i];
-      top = max(top, red_top[i]);
+      for (int i = 1; i < WPR; ++i) {
+        ss += red_ss[i];
+        top = max(top, red_top[i]);
+      }
+    }
+  };
+  reduce();
+  float r = 1.0f;
+  if constexpr (NORM) {
+    const float mean = ss / static_cast<float>(p.k) + p.eps;
+    r = 1.0f / __builtin_sqrtf(mean);
+    // fp16 does not come here but for what is not finite: 2^32 * 32768 at most, 2^-48 at least.
+    if (!(ss <= kMax) || mean < 1e-30f || !(__uint_as_float(top) <= kMax)) {  // uniform over the row
+      const float c = !(ss <= kMax) ? 0x1p-96f : mean < 1e-30f ? 0x1p96f : 1.0f;
+      const T* const again = ADD ? static_cast<const T*>(p.h) + row * p.k : x;  // h, as this thread wrote it
+      if constexpr (WPR > 1) __syncthreads();  // the first sums have been read
+      ss = 0.0f;
+#pragma unroll 1
+      for (int i = t; i < chunks; i += 64 * WPR) {
+        const vec8<T> h = *reinterpret_cast<const vec8<T>*>(again + 8 * i);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float hc = static_cast<float>(h[e]) * c;
+          ss = fmaf(hc, hc, ss);
+        }
+      }
+      reduce();
+      const float rc = 1.0f / __builtin_sqrtf(ss / static_cast<float>(p.k) + p.eps * c * c);
+      top = 0;
+#pragma unroll
+      for (int j = 0; j < CPT; ++j) {
+        const int i = j * 64 * WPR + t;
+        if (i >= chunks) continue;
+        const vec8<T> h = *reinterpret_cast<const vec8<T>*>(again + 8 * i);
+        const vec8<T> g = *reinterpret_cast<const vec8<T>*>(wt + 8 * i);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          f[j][e] = static_cast<float>(h[e]) * c * rc * (p.unit_offset ? 1.0f + static_cast<float>(g[e]) : static_cast<float>(g[e]));
+          top = max(top, __float_as_uint(f[j][e]) & 0x7fffffffu);
+        }
+      }
+      if constexpr (WPR > 1) __syncthreads();  // the second sums have been read
+      reduce();
+      r = 1.0f;
     }
   }
-  float r = 1.0f;
-  if constexpr (NORM) r = 1.0f / __builtin_sqrtf(ss / static_cast<float>(p.k) + p.eps);
   const float amax = __uint_as_float(top) * r;
-  const bool finite = amax <= 3.4028235e38f;  // false for NaN too
+  const bool finite = amax <= kMax;  // false for NaN too
   const float s = amax / 127.0f + 1e-12f;
   const float cf = finite ? r * (1.0f / s) : 0.0f;
   if (t == 0) p.scale[row] = finite ? s : __builtin_nanf("");

@@ -207,7 +207,9 @@ def quantize_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float,
                   unit_offset: bool = True) -> tuple[torch.Tensor, torch.Tensor]:
     """``quantize_int8`` of the RMSNorm of x, x / sqrt(mean(x^2) + eps) * (unit_offset + weight),
-    held in fp32 between the two (``rms_norm`` would round it to 16 bits)."""
+    held in fp32 between the two (``rms_norm`` would round it to 16 bits).  Squares past fp32's
+    range do no harm; a row that holds a NaN or an infinity, or is past fp32 behind the norm,
+    gets the scale NaN and codes 0."""
     if _direct(x, weight):
         return _quantize_impl(x, None, weight, float(eps), bool(unit_offset), "rms_norm_int8")[:2]
     return torch.ops.pi05_w4a4.rms_norm_int8(x, weight, float(eps), bool(unit_offset))
