@@ -33,6 +33,7 @@ import weakref
 from pathlib import Path
 
 import torch
+from torch.autograd import forward_ad as _forward_ad
 
 MFMA_MARKER_WORDS = 16
 WMMA_MARKER_WORDS = 9
@@ -1447,17 +1448,30 @@ _register_custom_op()
 # Eager calls skip the torch.ops dispatcher (tens of microseconds of host time per call,
 # several per decoder layer) when nothing needs it: plain tensors, no autograd graph to
 # record, no Dynamo trace, no torch.jit.trace (whose graph only sees dispatched ops), no
-# dispatch or function mode.  The direct and the dispatched route run the same
-# implementation.
+# dispatch or function mode, no function transform (vmap calls the dispatched op once a
+# sample).  The direct and the dispatched route run the same implementation.
 _is_compiling = torch.compiler.is_compiling
 _jit_tracing = torch._C._get_tracing_state
 _dispatch_modes = torch._C._len_torch_dispatch_stack
 _function_modes = torch._C._is_torch_function_mode_enabled
+_transforms = torch._C._functorch.peek_interpreter_stack
 _PLAIN = (torch.Tensor, torch.nn.Parameter)
+
+
+def _refuse_tangents(*ts) -> None:
+    """Neither route carries forward-mode tangents: refused rather than dropped."""
+    if _forward_ad._current_level < 0:
+        return
+    for t in ts:
+        if t is not None and _forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError("the pi05_w4a4 operators have no forward-mode derivatives, and an argument carries a tangent")
 
 
 def _direct(*ts) -> bool:
     if _is_compiling() or _jit_tracing() is not None or _dispatch_modes() or _function_modes():
+        return False
+    _refuse_tangents(*ts)
+    if _transforms() is not None:
         return False
     grad = torch.is_grad_enabled()
     for t in ts:

@@ -16,7 +16,8 @@ from __future__ import annotations
 import torch
 
 from pi05_fast.w4a4 import extension as _ext
-from pi05_fast.w4a4.extension import _check, _direct, _on_device, _ptr, _stream, _workspace, load_int4_gemm
+from pi05_fast.w4a4.extension import (_check, _direct, _on_device, _ptr, _refuse_tangents, _stream, _workspace,
+                                      load_int4_gemm)
 
 ELEM = {torch.float16: 0, torch.bfloat16: 1}
 MAX_ROW = 32768  # longest row of the quantizers
@@ -148,6 +149,7 @@ def _gemm_impl(q, q_scale, w, w_scale, bias, residual, out_dtype):
 # ----------------------------------------------------------------------------- custom ops
 @torch.library.custom_op("pi05_w4a4::quantize_int8", mutates_args=())
 def _quantize_op(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    _refuse_tangents(x)
     return _quantize_impl(x, None, None, 0.0, False, "quantize_int8")[:2]
 
 
@@ -163,6 +165,7 @@ def _quantize_fake(x):
 @torch.library.custom_op("pi05_w4a4::rms_norm_int8", mutates_args=())
 def _rms_norm_op(x: torch.Tensor, weight: torch.Tensor, eps: float,
                  unit_offset: bool) -> tuple[torch.Tensor, torch.Tensor]:
+    _refuse_tangents(x, weight)
     return _quantize_impl(x, None, weight, eps, unit_offset, "rms_norm_int8")[:2]
 
 
@@ -174,6 +177,7 @@ def _rms_norm_fake(x, weight, eps, unit_offset):
 @torch.library.custom_op("pi05_w4a4::add_rms_norm_int8", mutates_args=())
 def _add_rms_norm_op(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, eps: float,
                      unit_offset: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    _refuse_tangents(x, residual, weight)
     return _quantize_impl(x, residual, weight, eps, unit_offset, "add_rms_norm_int8")
 
 
@@ -185,6 +189,7 @@ def _add_rms_norm_fake(x, residual, weight, eps, unit_offset):
 @torch.library.custom_op("pi05_w4a4::int8_gemm", mutates_args=())
 def _gemm_op(q: torch.Tensor, q_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
              bias: torch.Tensor | None, residual: torch.Tensor | None, out_dtype: torch.dtype) -> torch.Tensor:
+    _refuse_tangents(q_scale, w_scale, bias, residual)
     return _gemm_impl(q, q_scale, w, w_scale, bias, residual, out_dtype)
 
 

@@ -20,7 +20,8 @@ import ctypes
 import torch
 
 from pi05_fast.w4a4 import extension as _ext
-from pi05_fast.w4a4.extension import _check, _direct, _on_device, _ptr, _stream, _workspace, load_int4_gemm
+from pi05_fast.w4a4.extension import (_check, _direct, _on_device, _ptr, _refuse_tangents, _stream, _workspace,
+                                      load_int4_gemm)
 from pi05_fast.w4a4.int8 import ELEM
 
 PAGE_TOKENS = 64
@@ -173,6 +174,7 @@ def _attention_impl(q, k_cache, v_cache, k_scale, v_scale, block_table, lens, sc
 def _append_op(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
                v_scale: torch.Tensor, block_table: torch.Tensor, lens: torch.Tensor,
                counts: torch.Tensor | None) -> None:
+    _refuse_tangents(k, v, k_scale, v_scale)
     _append_impl(k, v, k_cache, v_cache, k_scale, v_scale, block_table, lens, counts)
 
 
@@ -185,6 +187,7 @@ def _append_fake(k, v, k_cache, v_cache, k_scale, v_scale, block_table, lens, co
 def _attention_op(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
                   v_scale: torch.Tensor, block_table: torch.Tensor, lens: torch.Tensor, scaling: float, causal: bool,
                   q_lens: torch.Tensor | None, return_lse: bool) -> tuple[torch.Tensor, torch.Tensor]:
+    _refuse_tangents(q, k_scale, v_scale)
     out, lse = _attention_impl(q, k_cache, v_cache, k_scale, v_scale, block_table, lens, scaling, causal, q_lens,
                                return_lse)
     return out, lse if lse is not None else out.new_empty((0,), dtype=torch.float32)
