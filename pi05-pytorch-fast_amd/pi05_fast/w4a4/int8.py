@@ -22,6 +22,7 @@ from pi05_fast.w4a4.extension import (_check, _direct, _on_device, _ptr, _refuse
 ELEM = {torch.float16: 0, torch.bfloat16: 1}
 MAX_ROW = 32768  # longest row of the quantizers
 MAX_K = 65536  # longest K of the product: its int32 sums are exact
+MAX_N = 1 << 28  # most weight rows of the product
 
 _GEMM_WS: dict[tuple, int] = {}
 
@@ -102,6 +103,8 @@ def _gemm_impl(q, q_scale, w, w_scale, bias, residual, out_dtype):
         raise RuntimeError(f"int8_gemm: the codes have K={k}, the weights {tuple(w.shape)}")
     if k <= 0 or k % 16 or k > MAX_K:
         raise RuntimeError(f"int8_gemm: K must be a multiple of 16 of at most {MAX_K}, got {k}")
+    if n > MAX_N:  # here: the library takes N as 32 bits
+        raise RuntimeError(f"int8_gemm: N must be at most {MAX_N}, got {n}")
     lead = q.shape[:-1]
     shape = (*lead, n)
     m = q.numel() // k

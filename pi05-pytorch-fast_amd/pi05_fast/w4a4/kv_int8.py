@@ -26,6 +26,8 @@ from pi05_fast.w4a4.int8 import ELEM
 
 PAGE_TOKENS = 64
 HEAD_DIMS = (64, 128, 256)
+MAX_BATCH = 65535
+MAX_TOKENS = 1 << 24  # tokens of a sequence in a call, and pages of a table row
 
 _STRIDES: dict[tuple, ctypes.Array] = {}
 _ATTN_WS: dict[tuple, int] = {}
@@ -57,7 +59,7 @@ def _strided(t: torch.Tensor) -> tuple[torch.Tensor, ctypes.Array]:
     return t, arr
 
 
-def _check_cache(what, dev, k_cache, v_cache, k_scale, v_scale, table, lens, b, kvh, d):
+def _check_cache(what, dev, k_cache, v_cache, k_scale, v_scale, table, lens, b, t, kvh, d):
     if d not in HEAD_DIMS:
         raise RuntimeError(f"{what}: head_dim must be 64, 128 or 256, got {d}")
     pages = k_cache.size(0) if k_cache.dim() else 0
@@ -67,17 +69,20 @@ def _check_cache(what, dev, k_cache, v_cache, k_scale, v_scale, table, lens, b, 
     if v_cache.dtype != torch.int8 or v_cache.shape != (pages, kvh, d, PAGE_TOKENS):
         raise RuntimeError(f"{what}: v_cache must be int8 [{pages}, {kvh}, {d}, {PAGE_TOKENS}], got {v_cache.dtype} "
                            f"{tuple(v_cache.shape)}")
-    for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
-        if t.dtype != torch.float32 or t.shape != (pages, kvh):
-            raise RuntimeError(f"{what}: {name} must be float32 [{pages}, {kvh}], got {t.dtype} {tuple(t.shape)}")
+    for name, s in (("k_scale", k_scale), ("v_scale", v_scale)):
+        if s.dtype != torch.float32 or s.shape != (pages, kvh):
+            raise RuntimeError(f"{what}: {name} must be float32 [{pages}, {kvh}], got {s.dtype} {tuple(s.shape)}")
     if table.dtype != torch.int32 or table.dim() != 2 or table.size(0) != b:
         raise RuntimeError(f"{what}: block_table must be int32 [{b}, pages of a sequence], got {table.dtype} "
                            f"{tuple(table.shape)}")
+    if b > MAX_BATCH or t > MAX_TOKENS or table.size(1) > MAX_TOKENS:  # here: the library takes them as 32 bits
+        raise RuntimeError(f"{what}: at most {MAX_BATCH} sequences, {MAX_TOKENS} tokens and {MAX_TOKENS} pages of a sequence, "
+                           f"got {b}, {t} and {table.size(1)}")
     if lens.dtype != torch.int32 or lens.shape != (b,):
         raise RuntimeError(f"{what}: lens must be int32 [{b}], got {lens.dtype} {tuple(lens.shape)}")
-    for t in (k_cache, v_cache, k_scale, v_scale, table, lens):
-        if t.device != dev:
-            raise RuntimeError(f"{what}: the cache, block_table and lens must be on {dev}, got {t.device}")
+    for c in (k_cache, v_cache, k_scale, v_scale, table, lens):
+        if c.device != dev:
+            raise RuntimeError(f"{what}: the cache, block_table and lens must be on {dev}, got {c.device}")
     if not (k_cache.is_contiguous() and v_cache.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous()):
         raise RuntimeError(f"{what}: the cache must be contiguous")
     if k_cache.data_ptr() % 16 or v_cache.data_ptr() % 16:
@@ -111,7 +116,7 @@ def _append_impl(k, v, k_cache, v_cache, k_scale, v_scale, block_table, lens, co
     if k.dim() != 4 or v.shape != k.shape or v.device != dev:
         raise RuntimeError(f"{what} expects k and v [B, T, KVH, D] on one device, got {tuple(k.shape)} and {tuple(v.shape)}")
     b, t, kvh, d = k.shape
-    pages = _check_cache(what, dev, k_cache, v_cache, k_scale, v_scale, block_table, lens, b, kvh, d)
+    pages = _check_cache(what, dev, k_cache, v_cache, k_scale, v_scale, block_table, lens, b, t, kvh, d)
     counts = _ints(what, "counts", counts, b, dev)
     if b == 0 or t == 0:
         return
@@ -142,7 +147,7 @@ def _attention_impl(q, k_cache, v_cache, k_scale, v_scale, block_table, lens, sc
     kvh = k_cache.size(1)
     if kvh == 0 or h == 0 or h % kvh:
         raise RuntimeError(f"{what}: the query heads must be a multiple of the KV heads, got {h} and {kvh}")
-    pages = _check_cache(what, dev, k_cache, v_cache, k_scale, v_scale, block_table, lens, b, kvh, d)
+    pages = _check_cache(what, dev, k_cache, v_cache, k_scale, v_scale, block_table, lens, b, t, kvh, d)
     q_lens = _ints(what, "q_lens", q_lens, b, dev)
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = torch.empty((b, t, h), dtype=torch.float32, device=dev) if return_lse else None
