@@ -484,7 +484,9 @@ int pi05w4a4_gemm_e3m2_rows(const void* q6, const float* sa, int64_t m, int32_t 
  *   of the table only.
  * pi05w4a4_int8_kv_attention: out [B, T, H, D] = softmax(scaling q K^T) V over the tokens that
  *   query i of sequence b sees: with ql = q_lens[b] (null: T), the first lens[b] - ql + i + 1
- *   when causal, else lens[b]; none for i >= ql.  lens counts the new tokens too.  A query
+ *   when causal, else lens[b]; none for i >= ql.  lens counts the new tokens too; one past
+ *   table_pages * 64 counts as that, for the place of the queries as well (where the append dropped
+ *   tokens, leave their queries out of q_lens: the others then see their tokens).  A query
  *   that sees none gets zeros.  lse, when not null, fp32 [B, T, H]: the natural log of the sum
  *   of exp(scaling q k) (-inf where none is seen).  Query head h reads KV head h / (H / KVH).
  *   Needs pi05w4a4_int8_kv_attention_workspace_bytes(...) bytes (0 without a split, at most 2^28).

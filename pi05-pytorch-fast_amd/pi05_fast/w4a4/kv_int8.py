@@ -231,8 +231,10 @@ def int8_kv_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
 
     The queries are the last T tokens (``q_lens`` [B]: the last q_lens[b], the rows behind
     them padding) of ``lens`` [B] cached ones, whose keys the cache holds already.  When
-    ``causal``, query i sees the first lens - q_len + i + 1 tokens, else all of them.  A query that
-    sees no token, a padding row among them, gets zeros.  With ``return_lse``, also the
+    ``causal``, query i sees the first lens - q_len + i + 1 tokens, else all of them.  A length
+    past the table (64 tokens an entry) counts as the table's, for the place of the queries
+    too: where an append dropped tokens, ``q_lens`` without their queries gives the others what
+    they see.  A query that sees no token, a padding row among them, gets zeros.  With ``return_lse``, also the
     natural log of the sum of exp(scaling q k), fp32 [B, T, H] (-inf where none is seen), with
     which attention over further keys can be joined."""
     if _direct(q, k_cache, v_cache, k_scale, v_scale, block_table, lens, q_lens):
