@@ -124,8 +124,9 @@ struct Int8Tile {
 // many, the compiler moves them to the accumulation registers and back in every step).
 // Measured (us, 2048 deep, 2560 columns): 128 rows 8.4, 776 rows 14.1 (6 of them for one step and the
 // ends); a 64 x 64 step of a CU costs 0.25 us, a 128 x 64 step 0.36, where its MFMAs alone take 0.07
-// and 0.13: the steps are bound by the operands' way to the CU, 16 or 24 KB at 64 to 67 GB/s, and no
-// deeper ring (four stages) helps.
+// and 0.13: a step lasts as long as its operands take to the CU, 16 or 24 KB at 64 to 67 GB/s, which is
+// what this ring gets and no limit of the chip.  Of a wave's clocks at 776 rows 45% are waits for loads and
+// barriers and 17% MFMAs; a deeper ring (four stages) does not help.
 template <typename T, int BM, int BN, int KW, int ST>
 __global__ __launch_bounds__(64 * (BM / 64) * (BN / 64) * KW, 2) void int8_tile_kernel(Int8GemmParams p) {
   using C = Int8Tile<BM, BN, KW, ST>;
@@ -350,12 +351,14 @@ __global__ __launch_bounds__(64 * (BM / 64) * (BN / 64) * KW, 2) void int8_tile_
 // us: 431 / 469 / 462).
 // The workgroups walk the tiles, one a CU; the loads run on into the next tile, so that its first
 // stage lands during the epilogue, whose scales wait in LDS since the tile's first step.
-// What bounds it: power.  8192^3 takes 395 us with operands of ones and 431-445 with random ones, the
-// clock falling from 2.3 to 1.87 GHz; four waves of 128 x 128 on 32 x 32 x 32 MFMAs need a fifth
-// fewer clocks and run them at 1.62 GHz, in the same time.  MFMAs on random registers alone hold
-// 3450 TOP/s of the 5000 that the matrix units issue.
+// What bounds it: at 8192^3 the MFMAs are busy for 61% of the clocks, and the clock follows the power: 2.3 to
+// 2.4 GHz with operands of ones (379, after hundreds of calls 358 us), 1.9 to 2.2 with random ones (448, 399);
+// four waves of 128 x 128 on 32 x 32 x 32 MFMAs need a fifth fewer clocks and run them slower, in the same
+// time.  MFMAs on random registers alone hold 3450 TOP/s of the 5000 that the matrix units issue.  With 16
+// steps a tile (6208 x 2048 x 16384, 194 us) they are busy for 46%: the rest are a tile's ends.  A
+// residual costs more than its bytes (270 us, 41 of them its bytes): it is read group by group in the epilogue.
 // Tiles of 128 x 256 with two workgroups a CU, so that one's epilogue overlaps the other's product,
-// lose more to their operand traffic (6208 x 2048 x 16384: 238 us against 227).
+// lose more to their operand traffic (5% slower there).
 struct Int8Big {
   static constexpr int kTile = 256, kWaves = 8, MI = 4, NI = 8;
   static constexpr int kStage = 2 * kTile * 128;
@@ -515,8 +518,8 @@ __global__ __launch_bounds__(512) void int8_big_kernel(Int8GemmParams p) {
               epi(acc[i][half * 4 + j], sq, w4, b4, epi.residual(row, nh + j * 16 + lcol));
         }
         __builtin_amdgcn_wave_barrier();
-        // Whole lines go past the L2, which the operands need (us, past / through: 6208 x 2048 x 16384 212 / 218,
-        // x 2560 32.5 / 35), parts of lines through it (1071 x 2048 x 15984 63 / 56).
+        // Whole lines go past the L2, which the operands need (us, past / through: 6208 x 2048 x 16384 194 / 203,
+        // x 2560 34.3 / 34.9), parts of lines through it (1071 x 2048 x 15984 61 / 54).
         if (lines) {
 #pragma unroll
           for (int s = 0; s < 2; ++s) {

@@ -32,8 +32,9 @@ __device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) {
 //   s = max(s0, max|new| / 127 + 1e-12),  s0 the scale of the tokens that are there (0: none),
 // brings the old codes to it where it grew, c' = rint(c (s0 / s)), and writes the new ones,
 // c = rint(x (1 / s)).  A page whose first token is new is written whole, zeros behind the last
-// token, so that nothing of the page's earlier owner is left.  Bound by latency (lens -> table -> scale ->
-// codes, one after the other): 16 x 1 tokens 6.8 us, 8 x 776 tokens 6.8 (9.5 MB, 1.4 TB/s).
+// token, so that nothing of the page's earlier owner is left.  Its time is a chain of loads, lens -> table ->
+// values and scale -> old codes, of which only the first link has to be one: 16 x 1 tokens 6.5 us, 8 x 776
+// tokens 6.3 (9.5 MB, 1.5 TB/s; 69% of a wave's clocks are waits).
 template <typename T, int D>
 __global__ __launch_bounds__(256) void kv_append_kernel(KvAppendParams p) {
   // A thread holds kRows consecutive page rows of eight consecutive dimensions, so that a V row (one
@@ -488,7 +489,7 @@ __global__ __launch_bounds__(64 * W, 2) void kv_attn_kernel(KvAttnParams p) {
 // eight lanes that read one chunk of their rows meet eight different bank groups.
 // 2 x 776 tokens of 8 heads on one over 4096 keys, D = 256: 97 us, 400 TFLOP/s where a large fp16 product
 // reaches 1154.  Bound by a wave's own instructions: of the 5700 clocks of a page half are vector
-// instructions (softmax, value codes to fp16), a third MFMAs, the rest waits, one after the other.  The
+// instructions (softmax, value codes to fp16), a quarter MFMAs, a fifth waits, one after the other.  The
 // next page's scores issued beside the softmax (107 us) and values converted once for the four waves
 // (109) gain nothing: the waves walk in step.
 typedef int v16i __attribute__((ext_vector_type(16)));

@@ -10,7 +10,9 @@ queries over it: decoded tokens, the action tokens behind a prefix, or a prompt'
 Half the bytes of an fp16 cache.  A page's scale is that of its largest value; where a later
 token raises it, the page's earlier codes are rounded again (half a step of the new scale at
 most), so that a page filled token by token is up to about 1.4 times as far from its values as
-one written at once.  Lengths live on the device and are the caller's to advance.
+one written at once.  The scale does not fall again while the page keeps tokens: tokens that are
+written over and over at one length leave it at the largest they ever needed.  Lengths live on the
+device and are the caller's to advance.
 """
 
 from __future__ import annotations
@@ -227,7 +229,9 @@ def int8_kv_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
                       causal: bool = True, q_lens: torch.Tensor | None = None, return_lse: bool = False):
     """softmax(scaling q K^T) V of q [B, T, H, D] (fp16 or bf16, RoPE applied, any strides)
     over the cache: [B, T, H, D] in q's type.  H is a multiple of KVH; query head h reads KV
-    head h // (H / KVH).
+    head h // (H / KVH).  The work is planned for the table's width: pass a table held at
+    capacity as ``block_table[:, :n]``, n the pages of the longest sequence.  Entries that name
+    no page hide their 64 tokens.
 
     The queries are the last T tokens (``q_lens`` [B]: the last q_lens[b], the rows behind
     them padding) of ``lens`` [B] cached ones, whose keys the cache holds already.  When
