@@ -513,6 +513,74 @@ int pi05w4a4_int8_kv_attention(const void* q, const int64_t* q_strides, int32_t 
                                int32_t causal, void* out, float* lse, void* workspace, size_t workspace_bytes,
                                void* stream);
 
+/*
+ * 16-bit serving operators, on fp16 or bf16 data (elem as above).  No counterpart in the reference,
+ * whose attention rotates by tables and leaves the cache and adapters to its caller's framework.
+ *
+ * pi05w4a4_qk_norm_rope: q [B, T, H, D] and k [B, T, KVH, D] (strides {batch, token, head} in elements,
+ *   % 8 == 0, 16-byte aligned; D % 16 == 0, D <= 512; B * T <= 2^24) to q_out and k_out, contiguous.
+ *     f = x * g / sqrt(mean_d(x^2) + eps), g = 1 + w (unit_offset) or w, or f = x where the weight is null;
+ *     pair j < rot / 2 is dimensions (j, j + rot / 2), or (2j, 2j + 1) when interleaved, and turns by
+ *     pos * inv_freq[j]: (f1 c - f2 s, f2 c + f1 s); dimensions from rot on stay f.
+ *   rot % 16 == 0 (0: no rotation).  Positions are [axes, B, T] of int32 or int64 (pos_bytes 4 or 8), with strides
+ *   {axis, batch, token} in elements; axis_of_pair (host, rot / 2 bytes; null: all 0) names the axis of each
+ *   pair, at most 4 axes.  fp32 with one rounding; angles are reduced in 64 bits.
+ *
+ * KV cache: pages of 64 tokens, k_cache and v_cache [pages, KVH, 64, D]; D is 64, 128 or 256.  Token i of sequence
+ *   b is row i % 64 of page table[b * table_stride + i / 64].  Table entries outside [0, pages) name no
+ *   page: tokens there are neither written nor read.
+ * pi05w4a4_kv_append: writes tokens lens[b] .. lens[b] + counts[b] - 1 (counts null: all t) of every
+ *   sequence; k, v [B, T, KVH, D] with strides as above.  Nothing else of the cache changes.  Tokens past
+ *   table_pages * 64 are dropped.  lens is read only.  A row of a page may be written from one place of the
+ *   table only.
+ * pi05w4a4_qk_norm_rope_append: both in one launch: q_out, and the rotated keys and the values as they
+ *   are into the cache (D as the cache takes it).  All T tokens of q are done.
+ * pi05w4a4_kv_attention: out [B, T, H, D] = softmax(scaling q K^T) V over the tokens that query i of sequence b
+ *   sees: with ql = q_lens[b] (null: T), the first lens[b] - ql + i + 1 when causal, else lens[b]; none for
+ *   i >= ql.  lens counts the new tokens too; one past table_pages * 64 counts as that, for the place of the
+ *   queries as well.  A query that sees none gets zeros.  What a query does not see has no effect on it, NaN
+ *   and infinities too; a NaN or infinity among the values that it sees makes its outputs in that
+ *   dimension NaN.  lse, when not null, fp32 [B, T, H]: the natural log of the sum of exp(scaling q k) (-inf
+ *   where none is seen).  Query head h reads KV head h / (H / KVH).  Needs
+ *   pi05w4a4_kv_attention_workspace_bytes(...) bytes (0 without a split, at most 2^28).
+ *
+ * pi05w4a4_lora_add: out[m, n] = y[m, n] + scale[id] * sum_r (sum_k x[m, k] a[id, g r0 + r, k]) b[id, n, r] with
+ *   id = ids[m / per_id] and r0 = r, g the slice of column n: slice g has widths[g] columns (widths null: one
+ *   slice of N), at most 4, and rows g r .. g r + r - 1 of a.  a [adapters, slices * r, K], b [adapters, N, r],
+ *   contiguous; scale [adapters], null for 1.  ids outside [0, adapters) name no adapter: out = y.  x has row
+ *   stride ldx (% 8 == 0, 16-byte aligned), K % 8 == 0, K <= 2^20; y and out have row strides of any size and may
+ *   be the same matrix, but must not overlap otherwise (x may be either: it is read before out is written).
+ *   r % 8 == 0, r <= 128; smaller ranks are padded with zeros.  fp32 with one rounding.  M <= 2^26, N <= 2^22.
+ *   Needs pi05w4a4_lora_workspace_bytes(...) bytes.
+ */
+int pi05w4a4_qk_norm_rope(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, int32_t elem,
+                          int32_t b, int32_t t, int32_t h, int32_t kvh, int32_t d, const void* q_weight,
+                          const void* k_weight, float eps, int32_t unit_offset, const void* positions,
+                          const int64_t* pos_strides, int32_t pos_bytes, int32_t axes, const uint8_t* axis_of_pair,
+                          const float* inv_freq, int32_t rot, int32_t interleaved, void* q_out, void* k_out, void* stream);
+int pi05w4a4_qk_norm_rope_append(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                                 const void* v, const int64_t* v_strides, int32_t elem, int32_t b, int32_t t, int32_t h,
+                                 int32_t kvh, int32_t d, const void* q_weight, const void* k_weight, float eps,
+                                 int32_t unit_offset, const void* positions, const int64_t* pos_strides, int32_t pos_bytes,
+                                 int32_t axes, const uint8_t* axis_of_pair, const float* inv_freq, int32_t rot,
+                                 int32_t interleaved, void* q_out, void* k_cache, void* v_cache, int32_t pages,
+                                 const int32_t* table, int64_t table_stride, int32_t table_pages, const int32_t* lens,
+                                 const int32_t* counts, void* stream);
+int pi05w4a4_kv_append(const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides, int32_t elem, int32_t b,
+                       int32_t t, int32_t kvh, int32_t d, void* k_cache, void* v_cache, int32_t pages, const int32_t* table,
+                       int64_t table_stride, int32_t table_pages, const int32_t* lens, const int32_t* counts, void* stream);
+size_t pi05w4a4_kv_attention_workspace_bytes(int32_t b, int32_t t, int32_t h, int32_t kvh, int32_t d, int32_t table_pages);
+int pi05w4a4_kv_attention(const void* q, const int64_t* q_strides, int32_t elem, int32_t b, int32_t t, int32_t h, int32_t kvh,
+                          int32_t d, const void* k_cache, const void* v_cache, int32_t pages, const int32_t* table,
+                          int64_t table_stride, int32_t table_pages, const int32_t* lens, const int32_t* q_lens, float scaling,
+                          int32_t causal, void* out, float* lse, void* workspace, size_t workspace_bytes, void* stream);
+size_t pi05w4a4_lora_workspace_bytes(int64_t m, int64_t per_id, int32_t k, int32_t n, int32_t r, int32_t slices,
+                                     int32_t adapters);
+int pi05w4a4_lora_add(const void* y, int64_t ldy, const void* x, int64_t ldx, int64_t m, int32_t k, const void* a, const void* b,
+                      const float* scale, int32_t adapters, int32_t r, const int32_t* ids, int64_t per_id, int32_t n,
+                      int32_t slices, const int32_t* widths, int32_t elem, void* out, int64_t ldo, void* workspace,
+                      size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

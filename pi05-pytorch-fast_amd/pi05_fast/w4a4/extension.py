@@ -158,6 +158,21 @@ def load_int4_gemm():
         "pi05w4a4_int8_kv_attention": (
             ctypes.c_int, [vp, vp, i32, i32, i32, i32, i32, i32, vp, vp, vp, vp, i32, vp, i64, i32, vp, vp,
                            ctypes.c_float, i32, vp, vp, vp, sz, vp]),
+        "pi05w4a4_qk_norm_rope": (
+            ctypes.c_int, [vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, vp, vp, ctypes.c_float, i32, vp, vp, i32, i32, vp,
+                           vp, i32, i32, vp, vp, vp]),
+        "pi05w4a4_qk_norm_rope_append": (
+            ctypes.c_int, [vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, vp, vp, ctypes.c_float, i32, vp, vp, i32, i32,
+                           vp, vp, i32, i32, vp, vp, vp, i32, vp, i64, i32, vp, vp, vp]),
+        "pi05w4a4_kv_append": (
+            ctypes.c_int, [vp, vp, vp, vp, i32, i32, i32, i32, i32, vp, vp, i32, vp, i64, i32, vp, vp, vp]),
+        "pi05w4a4_kv_attention_workspace_bytes": (sz, [i32, i32, i32, i32, i32, i32]),
+        "pi05w4a4_kv_attention": (
+            ctypes.c_int, [vp, vp, i32, i32, i32, i32, i32, i32, vp, vp, i32, vp, i64, i32, vp, vp, ctypes.c_float, i32, vp,
+                           vp, vp, sz, vp]),
+        "pi05w4a4_lora_workspace_bytes": (sz, [i64, i64, i32, i32, i32, i32, i32]),
+        "pi05w4a4_lora_add": (
+            ctypes.c_int, [vp, i64, vp, i64, i64, i32, vp, vp, vp, i32, i32, vp, i64, i32, i32, vp, i32, vp, i64, vp, sz, vp]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)
