@@ -58,8 +58,8 @@ struct Span {
   int causal;
   __device__ __forceinline__ Span(const KvAttn16Params& p, int b) {
     const int64_t cap = static_cast<int64_t>(p.c.table_pages) * kKvPage;
-    len = p.c.pages > 0 ? min(static_cast<int64_t>(max(p.c.lens[b], 0)), cap) : 0;
-    q_len = min(max(p.q_lens != nullptr ? p.q_lens[b] : p.t, 0), p.t);
+    len = p.c.pages > 0 ? min(static_cast<int64_t>(max(scalar_load(p.c.lens + b), 0)), cap) : 0;
+    q_len = min(max(p.q_lens != nullptr ? scalar_load(p.q_lens + b) : p.t, 0), p.t);
     causal = p.causal;
   }
   // Tokens that query `token` sees: none past q_len.
@@ -101,14 +101,23 @@ __device__ __forceinline__ float weight_of(float m, float to) {
   return m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m - to);
 }
 
+// Two elements of a word: whether one is NaN or infinite, and the word with zeros in such places.
+template <typename T>
+constexpr uint32_t kExponent = static_cast<float>(static_cast<T>(65536.0f)) > 1e30f ? 0x7c00u : 0x7f80u;  // fp16, bf16
 template <typename T>
 __device__ __forceinline__ bool any_nonfinite(uint32_t w) {
-  constexpr uint32_t kExp = sizeof(T) == 2 && static_cast<float>(static_cast<T>(65536.0f)) > 1e30f ? 0x7c00u : 0x7f80u;
-  return (w & kExp) == kExp || ((w >> 16) & kExp) == kExp;
+  constexpr uint32_t kLow = kExponent<T>, kHigh = kLow << 16;
+  return (w & kLow) == kLow || (w & kHigh) == kHigh;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t finite_halves(uint32_t w) {
+  constexpr uint32_t kLow = kExponent<T>, kHigh = kLow << 16;
+  return ((w & kLow) == kLow ? 0u : w & 0xffffu) | ((w & kHigh) == kHigh ? 0u : w & 0xffff0000u);
 }
 
-template <typename T, int D, int W>
-__global__ __launch_bounds__(64 * W, W >= 8 ? 1 : 2) void kv_attn16_kernel(KvAttn16Params p) {
+// MIXED: rows of a tile may be of several tokens, which see different keys.
+template <typename T, int D, int W, bool MIXED>
+__global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void kv_attn16_kernel(KvAttn16Params p) {
   constexpr int F = D / 32, DT = D / 16;
   constexpr int VE = D >= 128 ? 8 : 4, CH = D / (16 * VE), VW = VE / 2;  // a value chunk: elements, chunks, words
   extern __shared__ __align__(16) v4f obuf[];  // [W][DT][64]
@@ -131,10 +140,11 @@ __global__ __launch_bounds__(64 * W, W >= 8 ? 1 : 2) void kv_attn16_kernel(KvAtt
   const int64_t most = span.most(tok_first, tok_last);
   const int64_t least = tile * 16 + 15 < rows ? span.least(tok_first, tok_last) : 0;
   const int pages = static_cast<int>((most + kKvPage - 1) / kKvPage);
-  const int per = (pages + p.nsplit - 1) / p.nsplit;
-  // Steps of 32 keys.
-  const int begin = 2 * split * per;
-  const int end = static_cast<int>(min(static_cast<int64_t>(2 * min((split + 1) * per, pages)), (most + kHalf - 1) / kHalf));
+  // The run's pages are split, split + nsplit, ..: the first is known without the length.  Its steps are
+  // the halves of 32 keys; a last half that no row sees is left out.
+  const int mine = pages > split ? (pages - split - 1) / p.nsplit + 1 : 0;
+  const bool half = mine > 0 && split + (mine - 1) * p.nsplit == pages - 1 && most <= static_cast<int64_t>(pages) * kKvPage - kHalf;
+  const int end = 2 * mine - (half ? 1 : 0);
 
   vec8<T> q[F];
   const T* const qrow = static_cast<const T*>(p.q) + b * p.q_stride[0] + tok * p.q_stride[1] + qh * p.q_stride[2];
@@ -149,12 +159,16 @@ __global__ __launch_bounds__(64 * W, W >= 8 ? 1 : 2) void kv_attn16_kernel(KvAtt
 
   // Entries that name no page are read as page 0, whose keys then count as not there.
   const int32_t* const table = p.c.table + b * p.c.table_stride;
-  auto page_at = [&](int step) { return step < end ? scalar_load(table + __builtin_amdgcn_readfirstlane(step >> 1)) : -1; };
+  auto page_of = [&](int step) { return __builtin_amdgcn_readfirstlane(split + (step >> 1) * p.nsplit); };
+  auto page_at = [&](int step) { return page_of(step) < p.c.table_pages ? scalar_load(table + page_of(step)) : -1; };
   auto place = [&](int page, int step) {  // first element of the step's keys
     const int64_t id = __builtin_amdgcn_readfirstlane(page >= 0 && page < p.c.pages ? page : 0);
     return ((id * p.c.kvh + head) * kKvPage + (step & 1) * kHalf) * D;
   };
-  const int koff = (8 * (col >> 2) + (col & 3)) * D + 8 * g, voff = 8 * g * D + col * VE;
+  // Four neighbouring lanes load 64 consecutive bytes of a key (16 lanes 16 keys, as the operand has them, are 16
+  // bytes of as many lines: a quarter of the rate); the fragment's chunk is lane 4 row + chunk's.
+  const int kr = lane >> 2, from = (4 * col + g) * 4;
+  const int koff = (8 * (kr >> 2) + (kr & 3)) * D + 8 * (lane & 3), voff = 8 * g * D + col * VE;
   vec8<T> kc[2][F];
   auto load_keys = [&](int64_t at) {
     const T* const kp = static_cast<const T*>(p.c.k) + at + koff;
@@ -163,9 +177,9 @@ __global__ __launch_bounds__(64 * W, W >= 8 ? 1 : 2) void kv_attn16_kernel(KvAtt
 #pragma unroll
       for (int f = 0; f < F; ++f) kc[t][f] = *reinterpret_cast<const vec8<T>*>(kp + 4 * t * D + 32 * f);
   };
-  int step = begin + wave;
+  int step = wave;
   int page = page_at(step);
-  if (step < end) load_keys(place(page, step));
+  if (p.c.pages > 0) load_keys(place(page, step));  // before the length is known
   for (; step < end; step += W) {
     const int64_t at = place(page, step);
     const bool there = page >= 0 && page < p.c.pages;
@@ -183,14 +197,19 @@ __global__ __launch_bounds__(64 * W, W >= 8 ? 1 : 2) void kv_attn16_kernel(KvAtt
     for (int t = 0; t < 2; ++t) {
       v4f a{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int f = 0; f < F; ++f) a = mfma(kc[t][f], q[f], a);
+      for (int f = 0; f < F; ++f) {
+        v4u x = __builtin_bit_cast(v4u, kc[t][f]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = __builtin_amdgcn_ds_bpermute(from, x[i]);
+        a = mfma(__builtin_bit_cast(vec8<T>, x), q[f], a);
+      }
 #pragma unroll
       for (int r = 0; r < 4; ++r) s[t][r] = a[r] * qfac;
     }
     // The next step's keys (past the last one: this one's again, not used).
     load_keys(step + W < end ? place(next, step + W) : at);
     page = next;
-    const int64_t key0 = static_cast<int64_t>(step) * kHalf;
+    const int64_t key0 = static_cast<int64_t>(page_of(step)) * kKvPage + (step & 1) * kHalf;
     if (!there) continue;  // uniform
     const bool edge = key0 + kHalf > least;  // some row does not see all of the step
     uint32_t poison = 0;  // bit j: key 8 g + j's value holds a NaN or infinity somewhere in this lane's part
@@ -209,7 +228,7 @@ __global__ __launch_bounds__(64 * W, W >= 8 ? 1 : 2) void kv_attn16_kernel(KvAtt
 #pragma unroll
           for (int w = 0; w < VW; ++w) {
             if (hidden) v[c][j][w] = 0u;
-            if (any_nonfinite<T>(v[c][j][w])) poison |= 1u << j;
+            if (MIXED && any_nonfinite<T>(v[c][j][w])) poison |= 1u << j;
           }
       }
     }
@@ -220,9 +239,10 @@ __global__ __launch_bounds__(64 * W, W >= 8 ? 1 : 2) void kv_attn16_kernel(KvAtt
       for (int r = 0; r < 4; ++r) top = fmaxf(top, s[t][r]);
     top = fmaxf(top, __shfl_xor(top, 16, 64));
     top = fmaxf(top, __shfl_xor(top, 32, 64));
-    if (__any(top > m + kTop)) {
-      const float m1 = fmaxf(m, top - kLift);
-      const float alpha = weight_of(m, m1);
+    const bool up = top > m + kTop;
+    if (__any(up)) {  // each row by itself: what it gets does not depend on the rows beside it
+      const float m1 = up ? top - kLift : m;
+      const float alpha = up ? weight_of(m, m1) : 1.0f;
       m = m1;
       l *= alpha;
 #pragma unroll
@@ -249,9 +269,9 @@ __global__ __launch_bounds__(64 * W, W >= 8 ? 1 : 2) void kv_attn16_kernel(KvAtt
         x[i] = __builtin_amdgcn_perm(v[c][2 * i + 1][e >> 1], v[c][2 * i][e >> 1], (e & 1) ? 0x07060302u : 0x05040100u);
       return __builtin_bit_cast(vec8<T>, x);
     };
-    if (edge && __any(poison != 0)) {
+    if (MIXED && edge && __any(poison != 0)) {
       // A value that some rows see and others do not is NaN or infinite: it makes NaN of the rows that
-      // see it, and leaves the others alone.  Rare.
+      // see it, and is zero for the product.  Rare.
       vec8<T> sees;
 #pragma unroll
       for (int j = 0; j < 8; ++j) sees[j] = static_cast<T>(key0 + 8 * g + j < seen ? 1.0f : 0.0f);
@@ -259,22 +279,23 @@ __global__ __launch_bounds__(64 * W, W >= 8 ? 1 : 2) void kv_attn16_kernel(KvAtt
       for (int c = 0; c < CH; ++c)
 #pragma unroll
         for (int e = 0; e < VE; ++e) {
-          vec8<T> x = turned(c, e), bad{};
+          const vec8<T> x = turned(c, e);
+          vec8<T> bad{};
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            if (!(__builtin_fabsf(static_cast<float>(x[j])) <= 3.4028235e38f)) {
-              bad[j] = static_cast<T>(1.0f);
-              x[j] = static_cast<T>(0.0f);
-            }
-          }
+          for (int j = 0; j < 8; ++j)
+            if (!(__builtin_fabsf(static_cast<float>(x[j])) <= 3.4028235e38f)) bad[j] = static_cast<T>(1.0f);
           const v4f count = mfma(bad, sees, v4f{0.0f, 0.0f, 0.0f, 0.0f});
-          v4f y = mfma(x, lo, mfma(x, hi, o[c * VE + e]));
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            if (count[r] > 0.0f) y[r] = __builtin_nanf("");
-          o[c * VE + e] = y;
+            if (count[r] > 0.0f) o[c * VE + e][r] = __builtin_nanf("");
+          __builtin_amdgcn_sched_barrier(0);
         }
-      continue;
+#pragma unroll
+      for (int c = 0; c < CH; ++c)
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+          for (int w = 0; w < VW; ++w) v[c][j][w] = finite_halves<T>(v[c][j][w]);
     }
 #pragma unroll
     for (int c = 0; c < CH; ++c)
@@ -315,9 +336,9 @@ __global__ __launch_bounds__(64 * W, W >= 8 ? 1 : 2) void kv_attn16_kernel(KvAtt
   float mall = mbuf[0][col];
 #pragma unroll
   for (int w = 1; w < W; ++w) mall = fmaxf(mall, mbuf[w][col]);
-  const float mine = weight_of(m, mall);
+  const float share = weight_of(m, mall);
 #pragma unroll
-  for (int i = 0; i < DT; ++i) obuf[(wave * DT + i) * 64 + lane] = quad(i) * mine;
+  for (int i = 0; i < DT; ++i) obuf[(wave * DT + i) * 64 + lane] = quad(i) * share;
   float lall = 0.0f;
 #pragma unroll
   for (int w = 0; w < W; ++w) lall += lbuf[w][col] * weight_of(mbuf[w][col], mall);
@@ -388,9 +409,16 @@ template <typename T, int D>
 void launch_attn(const KvAttn16Params& p, hipStream_t stream) {
   const int rows = p.t * (p.h / p.c.kvh);
   const dim3 grid(static_cast<unsigned>((rows + 15) / 16 * p.nsplit), static_cast<unsigned>(p.c.kvh), static_cast<unsigned>(p.b));
-  if (p.waves == 4) kv_attn16_kernel<T, D, 4><<<grid, 64 * 4, 4 * D * 64, stream>>>(p);
-  else if (p.waves == 2) kv_attn16_kernel<T, D, 2><<<grid, 64 * 2, 2 * D * 64, stream>>>(p);
-  else kv_attn16_kernel<T, D, 1><<<grid, 64, 0, stream>>>(p);
+  auto launch = [&](auto kernel, int waves) { kernel<<<grid, 64 * waves, waves > 1 ? waves * D * 64 : 0, stream>>>(p); };
+  if (p.t > 1) {
+    if (p.waves == 4) launch(kv_attn16_kernel<T, D, 4, true>, 4);
+    else if (p.waves == 2) launch(kv_attn16_kernel<T, D, 2, true>, 2);
+    else launch(kv_attn16_kernel<T, D, 1, true>, 1);
+  } else {
+    if (p.waves == 4) launch(kv_attn16_kernel<T, D, 4, false>, 4);
+    else if (p.waves == 2) launch(kv_attn16_kernel<T, D, 2, false>, 2);
+    else launch(kv_attn16_kernel<T, D, 1, false>, 1);
+  }
   if (p.nsplit > 1) {
     const int64_t all = static_cast<int64_t>(p.b) * p.t * p.h;
     const dim3 joins(static_cast<unsigned>((all + 3) / 4));
@@ -404,17 +432,36 @@ void launch_attn(const KvAttn16Params& p, hipStream_t stream) {
 // No call asks for more partial results than the Infinity Cache holds.
 constexpr size_t kMaxPartial = size_t{1} << 28;
 
-// Runs of pages: two rounds of workgroups of the CUs, two pages a run at least.
+// The runs of pages: the least of the times (us) that these measurements give.  A workgroup's start, and a step of
+// its four waves, for each round of the CUs (two workgroups beside each other at D <= 128); not less than the cache's
+// bytes at 5.5 TB/s, which fewer workgroups than CUs do not reach; for more than one run the join, whose loads past
+// the sixteenth run follow one another, and partial results at 10 TB/s.
+// us in 1 / 2 / 4 / 8 / 16 / 32 runs: D = 256, one sequence of 8192 keys 109 / - / - / - / 16.3 / 17.0, 16 of 2048
+// 32.5 / 23.1 / 17.3 / 14.6 / 15.0 (12) / -, 64 of 8192 - / 108 / 83 / 85 / 94 / -, 8 x 50 tokens over 826 18.2 / 26; D = 128, 8
+// KV heads, 8 of 1024 13.3 / 12.3 / 11.5 / 12.8 / - / -; D = 64, 8 KV heads, 4 of 4096 25.4 / 18.3 / 13.3 / 11.8 / 13.1 / 17.4.
+// Runs of one page take two waves (one sequence of 776 keys, 13 runs, 1 / 2 / 4 waves: 9.6 / 9.8 / 11.2).
 KvAttn16Plan kv_attn16_plan(int64_t b, int64_t t, int32_t h, int32_t kvh, int32_t d, int64_t table_pages, int cus) {
   KvAttn16Plan plan{1, 4};
   const int64_t rows = t * (h / kvh);
   if (rows <= 0 || b <= 0 || table_pages <= 0) return plan;
-  const int64_t groups = (rows + 15) / 16 * b * kvh;
-  int64_t n = std::min<int64_t>({(2 * cus + groups - 1) / groups, (table_pages + 1) / 2, kMaxRuns});
-  while (n > 1 && kv_attn16_workspace(b, t, h, d, static_cast<int>(n)) > kMaxPartial) --n;
-  plan.nsplit = static_cast<int>(std::max<int64_t>(n, 1));
-  const int64_t run = (table_pages + plan.nsplit - 1) / plan.nsplit;
-  plan.waves = run >= 2 ? 4 : 2;
+  const double start = d == 256 ? 5.5 : 4.0, step = d == 256 ? 1.6 : d == 128 ? 1.1 : 0.67;
+  const int64_t groups = (rows + 15) / 16 * b * kvh, slots = static_cast<int64_t>(cus) * (d == 256 ? 1 : 2);
+  const double bytes = static_cast<double>(b) * kvh * table_pages * kKvPage * d * 4;
+  const double partial = static_cast<double>(rows) * b * kvh * d * 8 / 1e7;
+  double best = 1e300;
+  for (int n = 1; n <= kMaxRuns && n <= table_pages; ++n) {
+    if (n > 1 && kv_attn16_workspace(b, t, h, d, n) > kMaxPartial) break;
+    const int64_t steps = (2 * ((table_pages + n - 1) / n) + 3) / 4, rounds = (groups * n + slots - 1) / slots;
+    const double filled = std::min(1.0, 0.7 + 0.3 * static_cast<double>(groups * n) / static_cast<double>(cus));
+    const double each = table_pages > n ? step : step / 2;  // two waves
+    const double us = std::max(static_cast<double>(rounds) * (start + static_cast<double>(steps) * each), start + bytes / (5.5e6 * filled)) +
+                      (n > 1 ? 3.5 + 0.05 * n + 0.2 * std::max(0, n - 16) + partial * n : 0.0);
+    if (us < best) {
+      best = us;
+      plan.nsplit = n;
+    }
+  }
+  plan.waves = table_pages > plan.nsplit ? 4 : 2;
   return plan;
 }
 
