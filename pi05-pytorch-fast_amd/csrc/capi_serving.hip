@@ -234,7 +234,8 @@ extern "C" int pi05w4a4_kv_attention(const void* q, const int64_t* q_strides, in
 
 static int check_lora(int64_t m, int64_t per_id, int32_t k, int32_t n, int32_t r, int32_t slices, int32_t adapters) {
   if (m < 0 || m > (1 << 26)) return capi_fail(PI05W4A4_EINVAL, "M must be in [0, 2^26], got %lld", (long long)m);
-  if (per_id < 1) return capi_fail(PI05W4A4_EINVAL, "rows of an id must be positive, got %lld", (long long)per_id);
+  if (per_id < 1 || per_id > (1 << 26))
+    return capi_fail(PI05W4A4_EINVAL, "rows of an id must be in [1, 2^26], got %lld", (long long)per_id);
   if (k <= 0 || k % 8 != 0 || k > (1 << 20))
     return capi_fail(PI05W4A4_EINVAL, "K must be a multiple of 8 of at most 2^20, got %d", k);
   if (n < 0 || n > (1 << 22)) return capi_fail(PI05W4A4_EINVAL, "N must be in [0, 2^22], got %d", n);
@@ -246,7 +247,7 @@ static int check_lora(int64_t m, int64_t per_id, int32_t k, int32_t n, int32_t r
 }
 
 static size_t lora_workspace(int64_t m, int32_t r, int32_t slices, int ksplit) {
-  return sizeof(float) * static_cast<size_t>(ksplit) * static_cast<size_t>(m) * static_cast<size_t>(slices * r);
+  return sizeof(float) * static_cast<size_t>(ksplit) * static_cast<size_t>(lora_h_floats(m, r, slices));
 }
 
 extern "C" size_t pi05w4a4_lora_workspace_bytes(int64_t m, int64_t per_id, int32_t k, int32_t n, int32_t r, int32_t slices,

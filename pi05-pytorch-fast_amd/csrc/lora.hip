@@ -5,16 +5,20 @@
 // g(n) is the slice of column n (the parts of a joined projection have first factors of their own, one
 // below the other in A).  Two launches on 16 x 16 x 32 matrix instructions:
 //
-// lora_down_kernel: 16 rows x up to 64 rows of A, the K slice of a workgroup over its four waves, joined
+// lora_down_kernel: 16 rows x up to 64 rows of A, the K slice of a workgroup over its eight waves, joined
 // in LDS; fp32 sums of each K slice to the workspace.
-// lora_up_kernel: 16 rows x 64 columns a wave at a time.  h is the sum of the K slices in fp32, split into two
-// 16-bit parts whose products with B are summed (fp16: after a shift that brings a row's largest into the
-// upper range, so that no h overflows), so that nothing of h is lost beside the rounding of out.
+// lora_up_kernel: 16 rows x 128 columns a wave.  h is the sum of the K slices in fp32, split into two 16-bit
+// parts whose products with B are summed (fp16: after a shift that brings a row's largest into the upper
+// range, so that no h overflows), so that nothing of h is lost beside the rounding of out.
 //
 // Rows need no order.  The adapters that occur in a tile of 16 rows are taken one by one: each is applied to the
-// whole tile and kept for its own rows, and the workgroups of a tile share them out (the first row
-// of each adapter in the tile stands for it).  A tile of one request has one; 16 decoded tokens of 16
-// adapters have 16, whose weights have to be read anyway.  Rows without an adapter keep y.
+// whole tile and kept for its own rows, and the workgroups of a tile share them out.  A tile of one request
+// has one; 16 decoded tokens of 16 adapters have 16, whose weights have to be read anyway.  Rows without an
+// adapter keep y.
+//
+// Operands are loaded with four neighbouring lanes on 64 consecutive bytes of a row and then handed to the
+// lanes that the matrix instruction wants them in: as it has them, 16 neighbouring lanes are 16 bytes of as many rows,
+// which arrive at a quarter of the rate (first launch, 6208 x 2048 with 64 rows of A: 26 -> 17 us).
 
 #include <algorithm>
 
@@ -24,6 +28,7 @@ namespace w4a4 {
 namespace {
 
 typedef float v4f __attribute__((ext_vector_type(4)));
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 template <typename T>
 using vec8 = T __attribute__((ext_vector_type(8)));
 
@@ -34,70 +39,103 @@ __device__ __forceinline__ v4f mfma(const vec8<__bf16> a, const vec8<__bf16> b, 
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
-// The adapter of a lane's row (row = first + lane % 16; -1: none), and the rows that stand for one.
-struct TileIds {
-  int id;
-  uint32_t leaders;  // bit i: row i is the first of its adapter in the tile (none counts as one when `none`)
-  __device__ __forceinline__ TileIds(const LoraParams& p, int64_t first, bool none) {
-    const int i = threadIdx.x & 15;
-    const int64_t row = first + i;
-    id = -2;  // behind the last row
-    if (row < p.m) {
-      id = p.ids[row / p.per_id];
-      if (id < 0 || id >= p.adapters) id = -1;
-    }
-    bool lead = id >= (none ? -1 : 0);
+// From lanes 4 row + chunk to lanes 16 chunk + row.
+template <typename T>
+__device__ __forceinline__ vec8<T> to_operand(const vec8<T> v) {
+  const int from = ((threadIdx.x & 15) * 4 + ((threadIdx.x & 63) >> 4)) * 4;
+  v4u x = __builtin_bit_cast(v4u, v);
 #pragma unroll
-    for (int j = 0; j < 15; ++j) {
-      const int other = __builtin_amdgcn_readlane(id, j);
-      if (j < i && other == id) lead = false;
-    }
-    leaders = static_cast<uint32_t>(__ballot(lead) & 0xffffu);
-  }
-};
+  for (int i = 0; i < 4; ++i) x[i] = __builtin_amdgcn_ds_bpermute(from, x[i]);
+  return __builtin_bit_cast(vec8<T>, x);
+}
 
-// Rows 64 y .. of A (NR tiles of 16), K slice z.
+// h between the launches: blocks of 16 rows x 32 ranks of a slice, [K slice, row tile, slice, ranks / 32], as the lanes
+// of the second launch take them: lane 16 g + row has ranks 8 g .. + 7.
+__device__ __forceinline__ int64_t lora_h_index(const LoraParams& p, int64_t tile, int slice, int s) {
+  return ((tile * p.slices + slice) * ((p.r + 31) / 32) + s) * 512;
+}
+
+__device__ __forceinline__ int lora_raw_id(const LoraParams& p, int64_t row) {
+  return p.ids[static_cast<uint32_t>(row) / static_cast<uint32_t>(p.per_id)];  // M and per_id <= 2^26
+}
+// -1: no adapter, -2: behind the last row.
+__device__ __forceinline__ int lora_id(const LoraParams& p, int raw, int64_t row) {
+  return row >= p.m ? -2 : raw < 0 || raw >= p.adapters ? -1 : raw;
+}
+
+// Calls f(id) for every which-th of a tile's adapters, in the order of their first rows (-1 among them when `none`).
+// `id` is that of the tile's row lane % 16.  Uniform over the workgroup.
+template <typename F>
+__device__ __forceinline__ void each_adapter(int id, bool none, int which, int groups, F f) {
+  uint32_t left = static_cast<uint32_t>(__ballot(id >= (none ? -1 : 0))) & 0xffffu;
+  for (int n = 0; left != 0; ++n) {
+    const int now = __builtin_amdgcn_readlane(id, __builtin_ctz(left));
+    left &= ~static_cast<uint32_t>(__ballot(id == now));
+    if (n % groups == which) f(now);
+  }
+}
+
+// Rows 16 NR y .. of A, K slice z; the slice's chunks of 32 elements are dealt to the waves in runs.
+// Bound by the arrival of x and A (A from the L2 for all row tiles but the first): kAhead chunks of both are
+// under way at once.  6208 x 2048 with 64 rows of A: 17 us.
 template <typename T, int NR>
-__global__ __launch_bounds__(256) void lora_down_kernel(LoraParams p) {
-  constexpr int W = 4;
+__global__ __launch_bounds__(512) void lora_down_kernel(LoraParams p) {
+  constexpr int W = 8, kAhead = 4;
   __shared__ __align__(16) v4f part[W][NR][64];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, col = lane & 15;
-  const int64_t first = static_cast<int64_t>(blockIdx.x / p.groups) * 16;
-  const int which = blockIdx.x % p.groups;
-  const TileIds ids(p, first, false);
+  const int lr = lane >> 2, lc = lane & 3;  // row and chunk that the lane loads
+  const int tile = blockIdx.x / p.groups;
+  const int64_t first = 16LL * tile;
+  const int64_t row = first + col;
+  const int my_id = lora_id(p, lora_raw_id(p, min(row, p.m - 1)), row);
   const int total = p.slices * p.r;  // rows of an adapter's A
   const int rank0 = blockIdx.y * 16 * NR;
-  // Chunks of 32 elements: the slice's, dealt to the waves in runs.
   const int chunks = (p.k + 31) / 32;
   const int per_slice = (chunks + p.ksplit - 1) / p.ksplit;
   const int c0 = blockIdx.z * per_slice, c1 = min(c0 + per_slice, chunks);
   const int per_wave = (per_slice + W - 1) / W;
   const int w0 = min(c0 + wave * per_wave, c1), w1 = min(w0 + per_wave, c1);
+  const int whole = min(w1, p.k / 32);  // chunks that K fills
 
-  const int64_t xrow = min(first + col, p.m - 1);
-  const T* const xp = static_cast<const T*>(p.x) + xrow * p.ldx + 8 * g;
-  int n = 0;
-  for (uint32_t left = ids.leaders; left != 0; left &= left - 1, ++n) {
-    if (n % p.groups != which) continue;  // uniform
-    const int id = __builtin_amdgcn_readlane(ids.id, __builtin_ctz(left));
+  const T* const xp = static_cast<const T*>(p.x) + min(first + lr, p.m - 1) * p.ldx + 8 * lc;
+  each_adapter(my_id, false, blockIdx.x % p.groups, p.groups, [&](int id) {
     const T* ap[NR];
 #pragma unroll
     for (int i = 0; i < NR; ++i)  // rows past the last one: the last one again, not stored
-      ap[i] = static_cast<const T*>(p.a) + (static_cast<int64_t>(id) * total + min(rank0 + 16 * i + col, total - 1)) * p.k + 8 * g;
+      ap[i] = static_cast<const T*>(p.a) + (static_cast<int64_t>(id) * total + min(rank0 + 16 * i + lr, total - 1)) * p.k + 8 * lc;
     v4f acc[NR];
 #pragma unroll
     for (int i = 0; i < NR; ++i) acc[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-    for (int c = w0; c < w1; ++c) {
-      const bool in = 32 * c + 8 * g < p.k;
-      const vec8<T> x = in ? *reinterpret_cast<const vec8<T>*>(xp + 32 * c) : vec8<T>{};
+    auto add = [&](const vec8<T> x, const vec8<T> (&a)[NR]) {
+      const vec8<T> u = to_operand<T>(x);
 #pragma unroll
-      for (int i = 0; i < NR; ++i) {
-        const vec8<T> a = in ? *reinterpret_cast<const vec8<T>*>(ap[i] + 32 * c) : vec8<T>{};
-        acc[i] = mfma(x, a, acc[i]);
+      for (int i = 0; i < NR; ++i) acc[i] = mfma(u, to_operand<T>(a[i]), acc[i]);
+    };
+    auto load = [&](vec8<T>& x, vec8<T> (&a)[NR], int k) {
+      x = *reinterpret_cast<const vec8<T>*>(xp + k);
+#pragma unroll
+      for (int i = 0; i < NR; ++i) a[i] = *reinterpret_cast<const vec8<T>*>(ap[i] + k);
+    };
+    int c = w0;
+    for (; c + kAhead <= whole; c += kAhead) {
+      vec8<T> x[kAhead], a[kAhead][NR];
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) load(x[j], a[j], 32 * (c + j));
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) add(x[j], a[j]);
+    }
+    for (; c < w1; ++c) {  // the last ones, and one that K does not fill
+      vec8<T> x, a[NR];
+      const bool in = 32 * c + 8 * lc < p.k;
+      load(x, a, in ? 32 * c : -8 * lc);  // elsewhere the row's first elements
+      if (!in) {
+        x = vec8<T>{};
+#pragma unroll
+        for (int i = 0; i < NR; ++i) a[i] = vec8<T>{};
       }
+      add(x, a);
     }
 #pragma unroll
     for (int i = 0; i < NR; ++i) part[wave][i][lane] = acc[i];
@@ -107,80 +145,128 @@ __global__ __launch_bounds__(256) void lora_down_kernel(LoraParams p) {
 #pragma unroll
       for (int w = 1; w < W; ++w) s += part[w][i][lane];
       const int rank = rank0 + 16 * i + col;
+      float* const hp = p.h + blockIdx.z * p.h_plane + lora_h_index(p, tile, rank / p.r, rank % p.r / 32) +
+                        (rank % p.r % 32 / 8) * 128 + rank % p.r % 8;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int of = __shfl(ids.id, 4 * g + r, 64);  // rows 4 g + r of the tile
-        if (of == id && rank < total)
-          p.h[(static_cast<int64_t>(blockIdx.z) * p.m + first + 4 * g + r) * total + rank] = s[r];
+        const int of = __shfl(my_id, 4 * g + r, 64);  // row 4 g + r of the tile
+        if (of == id && rank < total) hp[(4 * g + r) * 8] = s[r];
       }
     }
     __syncthreads();
-  }
+  });
 }
 
-// Columns: blocks of 64 of each slice, one a wave.
+// A wave takes 16 rows and kCols columns of a slice, h and y (and the ids, on which only B waits) under way at
+// once; nothing is kept for a second row tile, as more waves hide more (B kept over the row tiles of a wave, with the
+// next tile under way: 191 us for 6208 x 32768 in place of 199, 51 for 2560 columns in place of 47).  Column j of tile
+// i is column NT j + i of the block: a lane ends with NT (eight, or four for large ranks) consecutive columns of four
+// rows, and 16 lanes read and write 256 or 128 consecutive bytes of a row.  Bound by y and out in HBM where rows are
+// many: 6208 x 32768 with rank 32, both launches 167 us, 5.1 TB/s.
+template <int KS>
+constexpr int kCols = KS <= 2 ? 128 : 64;
+
+// KS: ranks / 32.
 template <typename T, int KS>
-__global__ __launch_bounds__(256) void lora_up_kernel(LoraParams p) {
+__global__ __launch_bounds__(256, KS == 1 ? 4 : 2) void lora_up_kernel(LoraParams p) {
+  constexpr int C = kCols<KS>, NT = C / 16;  // a lane's consecutive columns
+  constexpr int ZA = KS == 1 ? 4 : 1;        // K slices of h that are loaded at once
+  typedef T vecn __attribute__((ext_vector_type(NT)));
+  typedef T vecn_h __attribute__((ext_vector_type(NT), aligned(2)));  // at any element
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, col = lane & 15;
-  const int64_t first = static_cast<int64_t>(blockIdx.x / p.groups) * 16;
-  const int which = blockIdx.x % p.groups;
-  int block = blockIdx.y * 4 + wave, slice = 0, n0 = 0;
-  while (slice < p.slices && block >= (p.width[slice] + 63) / 64) {
-    block -= (p.width[slice] + 63) / 64;
+  const int lr = lane >> 2, lc = lane & 3;  // row of B's tiles and chunk that the lane loads
+  // The workgroup's four blocks within a slice, its rows, and its part of their adapters.
+  int run = blockIdx.x % p.runs, slice = 0, n0 = 0;
+  const int rest = blockIdx.x / p.runs;
+  const int which = rest % p.groups, tile = rest / p.groups;
+  for (; slice < p.slices; ++slice) {
+    const int runs = (p.width[slice] + 4 * C - 1) / (4 * C);
+    if (run < runs) break;
+    run -= runs;
     n0 += p.width[slice];
-    ++slice;
   }
-  if (slice == p.slices) return;  // no barrier below
   const int end = n0 + p.width[slice];
-  n0 += 64 * block;
+  n0 += (run * 4 + wave) * C;
+  if (n0 >= end) return;  // no barrier below
+  const int nc = n0 + NT * col;
+  const bool whole = n0 + C <= end;  // uniform
   const bool in_place = p.out == p.y && p.ldo == p.ldy;
-  const TileIds ids(p, first, !in_place);
-  const int total = p.slices * p.r;
-  const int64_t row = min(first + col, p.m - 1);
-  // This lane's 16 columns of its row.
-  const int nc = n0 + 16 * g;
-  const T* const yp = static_cast<const T*>(p.y) + row * p.ldy + nc;
-  T* const op = static_cast<T*>(p.out) + row * p.ldo + nc;
-  const bool whole = nc + 16 <= end && p.ldy % 8 == 0 && p.ldo % 8 == 0 && nc % 8 == 0 &&
-                     (reinterpret_cast<uintptr_t>(p.y) & 15) == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
 
-  // h of the lane's row, ranks 32 s + 8 g .. + 7, as two parts.
-  vec8<T> hi[KS], lo[KS];
-  float back = 1.0f;
-  {
-    float f[KS][8];
-    float top = 0.0f;
+  // The ids, h (ranks 32 s + 8 g .. + 7 of row `col`) and y (columns nc .. + NT - 1 of rows 4 g + r).  Rows past the last
+  // one are the last one again.
+  const int64_t first = 16LL * tile;
+  const int last = static_cast<int>(min(p.m - 1 - first, static_cast<int64_t>(15)));
+  const int raw = lora_raw_id(p, first + min(col, last));
+  v4f part[ZA][KS][2];
+  if (p.adapters > 0) {
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
-      const int r = 32 * s + 8 * g;
+      const float* const hp = p.h + lora_h_index(p, tile, slice, s) + lane * 8;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) f[s][e] = 0.0f;
-      if (r < p.r && ids.id >= 0) {
-        const float* hp = p.h + row * total + slice * p.r + r;
-        for (int z = 0; z < p.ksplit; ++z, hp += p.m * total) {
-          const v4f u = *reinterpret_cast<const v4f*>(hp), v = *reinterpret_cast<const v4f*>(hp + 4);
+      for (int z = 0; z < ZA; ++z)
+        if (z < p.ksplit) {
+          part[z][s][0] = *reinterpret_cast<const v4f*>(hp + z * p.h_plane);
+          part[z][s][1] = *reinterpret_cast<const v4f*>(hp + z * p.h_plane + 4);
+        }
+    }
+  }
+  vecn y[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            f[s][e] += u[e];
-            f[s][4 + e] += v[e];
-          }
+  for (int r = 0; r < 4; ++r) {
+    const T* const yp = static_cast<const T*>(p.y) + first * p.ldy + min(4 * g + r, last) * p.ldy + nc;
+    if (whole) {
+      y[r] = *reinterpret_cast<const vecn_h*>(yp);
+    } else {
+#pragma unroll
+      for (int e = 0; e < NT; ++e) y[r][e] = nc + e < end ? yp[e] : static_cast<T>(0.0f);
+    }
+  }
+
+  const int my_id = lora_id(p, raw, first + col);
+  vec8<T> hi[KS], lo[KS];
+  float shift = 1.0f, unshift = 1.0f;
+  {
+    float f[KS][8];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[s][e] = p.adapters > 0 ? part[0][s][e >> 2][e & 3] : 0.0f;
+#pragma unroll
+      for (int z = 1; z < ZA; ++z)
+        if (z < p.ksplit) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) f[s][e] += part[z][s][e >> 2][e & 3];
+        }
+      for (int z = ZA; z < p.ksplit; ++z) {
+        const float* const hp = p.h + lora_h_index(p, tile, slice, s) + lane * 8 + z * p.h_plane;
+        const v4f a = *reinterpret_cast<const v4f*>(hp), b = *reinterpret_cast<const v4f*>(hp + 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          f[s][e] += a[e];
+          f[s][4 + e] += b[e];
         }
       }
+      if (32 * s + 8 * g >= p.r) {  // past the last rank: anything
 #pragma unroll
-      for (int e = 0; e < 8; ++e) top = fmaxf(top, __builtin_fabsf(f[s][e]));
+        for (int e = 0; e < 8; ++e) f[s][e] = 0.0f;
+      }
     }
-    float shift = 1.0f;
     if constexpr (static_cast<float>(static_cast<T>(65536.0f)) > 1e30f) {  // fp16
+      float top = 0.0f;
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, __builtin_fabsf(f[s][e]));
       top = fmaxf(top, __shfl_xor(top, 16, 64));
       top = fmaxf(top, __shfl_xor(top, 32, 64));
-      // The largest to 2^13 .. 2^14; nothing to do for rows of zeros, infinities or NaN.
+      // The row's largest to 2^13 .. 2^14; nothing to do for rows of zeros, infinities or NaN.
       const int e = static_cast<int>(__float_as_uint(top) >> 23) - 127;
       if (top > 0.0f && e < 128) {
         const int by = max(min(13 - e, 126), -126);
         shift = __uint_as_float(static_cast<uint32_t>(127 + by) << 23);
-        back = __uint_as_float(static_cast<uint32_t>(127 - by) << 23);
+        unshift = __uint_as_float(static_cast<uint32_t>(127 - by) << 23);
       }
     }
 #pragma unroll
@@ -192,86 +278,98 @@ __global__ __launch_bounds__(256) void lora_up_kernel(LoraParams p) {
         lo[s][e] = static_cast<T>(v - static_cast<float>(hi[s][e]));
       }
   }
-
-  int n = 0;
-  for (uint32_t left = ids.leaders; left != 0; left &= left - 1, ++n) {
-    if (n % p.groups != which) continue;
-    const int id = __builtin_amdgcn_readlane(ids.id, __builtin_ctz(left));
-    v4f acc[4];
+  // What the lane ends with are rows 4 g + r, whose adapters and factors are in other lanes.
+  float back[4];
+  int of[4];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) acc[t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int r = 0; r < 4; ++r) {
+    back[r] = __shfl(unshift, 4 * g + r, 64);
+    of[r] = __shfl(my_id, 4 * g + r, 64);
+  }
+  each_adapter(my_id, !in_place, which, p.groups, [&](int id) {
+    float scale = 0.0f;
+    v4f acc[NT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) acc[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
     if (id >= 0) {
-      const T* const bp = static_cast<const T*>(p.b) + static_cast<int64_t>(id) * p.n * p.r + 8 * g;
+      scale = p.scale != nullptr ? p.scale[id] : 1.0f;
+      const T* const bp = static_cast<const T*>(p.b) + static_cast<int64_t>(id) * p.n * p.r;
+      vec8<T> w[NT][KS];
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        // Row i of tile t is column 16 (i / 4) + 4 t + i % 4 of the block: a lane ends with 16 consecutive ones.
-        const int nb = min(n0 + 16 * (col >> 2) + 4 * t + (col & 3), end - 1);
+      for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+          w[i][s] = *reinterpret_cast<const vec8<T>*>(bp + static_cast<int64_t>(min(n0 + NT * lr + i, end - 1)) * p.r + min(32 * s + 8 * lc, p.r - 8));
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
-          vec8<T> w{};
-          if (32 * s + 8 * g < p.r) w = *reinterpret_cast<const vec8<T>*>(bp + static_cast<int64_t>(nb) * p.r + 32 * s);
-          acc[t] = mfma(w, hi[s], acc[t]);
-          acc[t] = mfma(w, lo[s], acc[t]);
+          vec8<T> u = to_operand<T>(w[i][s]);
+          if (32 * s + 8 * g >= p.r) u = vec8<T>{};
+          acc[i] = mfma(hi[s], u, acc[i]);
+          acc[i] = mfma(lo[s], u, acc[i]);
         }
-      }
     }
-    if (ids.id != id) continue;  // the rows of other adapters
-    const float scale = id < 0 ? 0.0f : (p.scale != nullptr ? p.scale[id] : 1.0f);
-    if (whole) {
-      const vec8<T> y0 = *reinterpret_cast<const vec8<T>*>(yp), y1 = *reinterpret_cast<const vec8<T>*>(yp + 8);
-      vec8<T> z0 = y0, z1 = y1;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      if (of[r] != id) continue;  // the rows of other adapters
+      vecn z = y[r];
       if (id >= 0) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          z0[e] = static_cast<T>(fmaf(acc[e >> 2][e & 3] * back, scale, static_cast<float>(y0[e])));
-          z1[e] = static_cast<T>(fmaf(acc[2 + (e >> 2)][e & 3] * back, scale, static_cast<float>(y1[e])));
-        }
+        for (int e = 0; e < NT; ++e) z[e] = static_cast<T>(fmaf(acc[e][r] * back[r], scale, static_cast<float>(z[e])));
       }
-      *reinterpret_cast<vec8<T>*>(op) = z0;
-      *reinterpret_cast<vec8<T>*>(op + 8) = z1;
-    } else {
+      T* const op = static_cast<T*>(p.out) + first * p.ldo + (4 * g + r) * p.ldo + nc;
+      if (whole) {
+        __builtin_nontemporal_store(z, reinterpret_cast<vecn_h*>(op));  // past the L2, which B and h need
+      } else {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        if (nc + e >= end) continue;
-        const T y = yp[e];
-        op[e] = id >= 0 ? static_cast<T>(fmaf(acc[e >> 2][e & 3] * back, scale, static_cast<float>(y))) : y;
+        for (int e = 0; e < NT; ++e)
+          if (nc + e < end) op[e] = z[e];
       }
     }
-  }
+  });
 }
 
 template <typename T>
-void launch(const LoraParams& p, hipStream_t stream) {
+void launch_down(const LoraParams& p, hipStream_t stream) {
   const unsigned tiles = static_cast<unsigned>((p.m + 15) / 16 * p.groups);
   const int total = p.slices * p.r;
-  if (p.adapters > 0) {
-    if (total <= 16)
-      lora_down_kernel<T, 1><<<dim3(tiles, 1, p.ksplit), 256, 0, stream>>>(p);
-    else if (total <= 32)
-      lora_down_kernel<T, 2><<<dim3(tiles, 1, p.ksplit), 256, 0, stream>>>(p);
-    else
-      lora_down_kernel<T, 4><<<dim3(tiles, (total + 63) / 64, p.ksplit), 256, 0, stream>>>(p);
-  }
-  int blocks = 0;
-  for (int s = 0; s < p.slices; ++s) blocks += (p.width[s] + 63) / 64;
-  const dim3 grid(tiles, (blocks + 3) / 4);
-  if (p.r <= 32)
-    lora_up_kernel<T, 1><<<grid, 256, 0, stream>>>(p);
-  else if (p.r <= 64)
-    lora_up_kernel<T, 2><<<grid, 256, 0, stream>>>(p);
+  if (total <= 16)
+    lora_down_kernel<T, 1><<<dim3(tiles, 1, p.ksplit), 512, 0, stream>>>(p);
+  else if (total <= 32)
+    lora_down_kernel<T, 2><<<dim3(tiles, 1, p.ksplit), 512, 0, stream>>>(p);
   else
-    lora_up_kernel<T, 4><<<grid, 256, 0, stream>>>(p);
+    lora_down_kernel<T, 4><<<dim3(tiles, (total + 63) / 64, p.ksplit), 512, 0, stream>>>(p);
+}
+
+template <typename T, int KS>
+void launch_up(LoraParams p, hipStream_t stream) {
+  p.runs = 0;
+  for (int s = 0; s < p.slices; ++s) p.runs += (p.width[s] + 4 * kCols<KS> - 1) / (4 * kCols<KS>);
+  const dim3 grid(static_cast<unsigned>((p.m + 15) / 16 * p.groups * p.runs));
+  lora_up_kernel<T, KS><<<grid, 256, 0, stream>>>(p);
+}
+
+template <typename T>
+void launch(LoraParams p, hipStream_t stream) {
+  p.h_plane = lora_h_floats(p.m, p.r, p.slices);
+  if (p.adapters > 0) launch_down<T>(p, stream);
+  if (p.r <= 32) launch_up<T, 1>(p, stream);
+  else if (p.r <= 64) launch_up<T, 2>(p, stream);
+  else launch_up<T, 4>(p, stream);
 }
 
 }  // namespace
 
-// K slices for as many workgroups as CUs where row tiles are few; a tile's adapters go to as many workgroups
-// as it can have adapters, where tiles are few.
+int64_t lora_h_floats(int64_t m, int32_t r, int32_t slices) { return (m + 15) / 16 * slices * ((r + 31) / 32) * 512; }
+
+// K slices for as many workgroups as CUs where row tiles are few; a tile's adapters go to as many workgroups as
+// it can have adapters, where tiles are few.
 LoraPlan lora_plan(int64_t m, int64_t per_id, int32_t k, int32_t n, int32_t r, int32_t slices, int32_t adapters, int cus) {
+  LoraPlan plan;
   const int64_t tiles = (m + 15) / 16;
   const int64_t most = std::min<int64_t>({16, 15 / per_id + 2, adapters + 1});
-  LoraPlan plan;
-  plan.groups = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(most, 4 * cus / tiles)));
+  plan.groups = per_id >= 16 ? 1 : static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(most, 2 * cus / tiles)));
   const int64_t down = tiles * plan.groups * ((slices * r + 63) / 64);
   plan.ksplit = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({cus / down, (k + 511) / 512, 8})));
   return plan;

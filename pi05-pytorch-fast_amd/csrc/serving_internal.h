@@ -78,18 +78,21 @@ struct LoraParams {
   const int32_t* ids;  // [M / per_id]
   const void* y;       // [M, N], row stride ldy
   void* out;           // [M, N], row stride ldo (may be y)
-  float* h;            // [ksplit, M, slices * R]
+  float* h;            // [ksplit, h_plane]
   int64_t m, per_id, ldx, ldy, ldo;
   int32_t k, n, r, adapters, slices;
   int32_t width[kLoraSlices];  // columns of each slice
   int32_t ksplit;
   int32_t groups;      // workgroups that share a row tile's adapters
+  int32_t runs;        // of 512 columns, over the slices
+  int64_t h_plane;     // floats of a K slice in h
 };
 struct LoraPlan {
   int ksplit;
   int groups;
 };
 LoraPlan lora_plan(int64_t m, int64_t per_id, int32_t k, int32_t n, int32_t r, int32_t slices, int32_t adapters, int cus);
+int64_t lora_h_floats(int64_t m, int32_t r, int32_t slices);
 hipError_t launch_lora(const LoraParams& p, int elem, hipStream_t stream);
 
 }  // namespace w4a4
