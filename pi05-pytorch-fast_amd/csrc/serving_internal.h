@@ -82,9 +82,9 @@ struct LoraParams {
   int64_t m, per_id, ldx, ldy, ldo;
   int32_t k, n, r, adapters, slices;
   int32_t width[kLoraSlices];  // columns of each slice
-  int32_t ksplit;
+  int32_t ksplit;      // K slices of the first launch; 0: both products in one
   int32_t groups;      // workgroups that share a row tile's adapters
-  int32_t runs;        // of 512 columns, over the slices
+  int32_t runs;        // of a workgroup's columns, over the slices
   int64_t h_plane;     // floats of a K slice in h
 };
 struct LoraPlan {

@@ -19,12 +19,10 @@ from pi05_fast.w4a4 import extension as _ext
 from pi05_fast.w4a4.extension import (_check, _direct, _on_device, _ptr, _refuse_tangents, _stream, _workspace,
                                       load_int4_gemm)
 from pi05_fast.w4a4.int8 import ELEM
-from pi05_fast.w4a4.kv_int8 import HEAD_DIMS, MAX_BATCH, MAX_TOKENS, PAGE_TOKENS, _ints, _strided, _table
-from pi05_fast.w4a4.rope import _rope_args
+from pi05_fast.w4a4.kv_int8 import HEAD_DIMS, MAX_BATCH, MAX_TOKENS, PAGE_TOKENS, _ints, _table
+from pi05_fast.w4a4.rope import _check_rope, _heads, _meta, _plan, _strides, _weight
 
 MAX_KV_HEADS = 32767
-
-_ATTN_WS: dict[tuple, int] = {}
 
 
 def kv_cache(pages: int, kv_heads: int, head_dim: int, dtype: torch.dtype, device) -> tuple[torch.Tensor, torch.Tensor]:
@@ -59,65 +57,93 @@ def _check_cache(what, x, k_cache, v_cache, table, lens, b, t, kvh, d):
             raise RuntimeError(f"{what}: the cache, block_table and lens must be on {dev}, got {c.device}")
     if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
         raise RuntimeError(f"{what}: the cache must be contiguous")
-    if k_cache.data_ptr() % 16 or v_cache.data_ptr() % 16:
-        raise RuntimeError(f"{what}: the cache must be 16-byte aligned")
     return pages
+
+
+def _check_append(what, k, v, k_cache, v_cache, table, lens, counts):
+    if not k.is_cuda:
+        raise RuntimeError(f"{what} expects CUDA/HIP tensors")
+    elem = ELEM.get(k.dtype)
+    if elem is None or v.dtype != k.dtype:
+        raise RuntimeError(f"{what} takes float16 or bfloat16 keys and values of one type, got {k.dtype} and {v.dtype}")
+    if k.dim() != 4 or v.shape != k.shape or v.device != k.device:
+        raise RuntimeError(f"{what} expects k and v [B, T, KVH, D] on one device, got {tuple(k.shape)} and {tuple(v.shape)}")
+    b, t, kvh, d = k.shape
+    pages = _check_cache(what, k, k_cache, v_cache, table, lens, b, t, kvh, d)
+    _ints(what, "counts", counts, b, k.device)
+    if b * t > MAX_TOKENS:  # here: the library takes them as 32 bits
+        raise RuntimeError(f"{what}: at most {MAX_TOKENS} tokens a call, got {b} x {t}")
+    return (elem, b, t, kvh, d), pages, _strides(k), _strides(v)
+
+
+def _cache_pointers(what, k_cache, v_cache):
+    kp, vp = k_cache.data_ptr(), v_cache.data_ptr()
+    if (kp | vp) & 15:
+        raise RuntimeError(f"{what}: the cache must be 16-byte aligned")
+    return kp, vp
 
 
 def _append_impl(k, v, k_cache, v_cache, block_table, lens, counts):
     what = "kv_append"
-    if not k.is_cuda:
-        raise RuntimeError(f"{what} expects CUDA/HIP tensors")
-    dev = k.device
-    elem = ELEM.get(k.dtype)
-    if elem is None or v.dtype != k.dtype:
-        raise RuntimeError(f"{what} takes float16 or bfloat16 keys and values of one type, got {k.dtype} and {v.dtype}")
-    if k.dim() != 4 or v.shape != k.shape or v.device != dev:
-        raise RuntimeError(f"{what} expects k and v [B, T, KVH, D] on one device, got {tuple(k.shape)} and {tuple(v.shape)}")
-    b, t, kvh, d = k.shape
-    pages = _check_cache(what, k, k_cache, v_cache, block_table, lens, b, t, kvh, d)
-    counts = _ints(what, "counts", counts, b, dev)
-    if b == 0 or t == 0:
+    shape, pages, ks, vs = _plan(
+        (what, _meta(k), _meta(v), _meta(k_cache), _meta(v_cache), _meta(block_table), _meta(lens), _meta(counts)),
+        lambda: _check_append(what, k, v, k_cache, v_cache, block_table, lens, counts))
+    kp, vp = _cache_pointers(what, k_cache, v_cache)
+    if shape[1] == 0 or shape[2] == 0:
         return
+    dev = k.device
     table, stride = _table(block_table)
-    lens = lens.contiguous()
-    k, ks = _strided(k)
-    v, vs = _strided(v)
+    lens, counts = lens.contiguous(), None if counts is None else counts.contiguous()
+    k, ks = _heads(k, ks)
+    v, vs = _heads(v, vs)
     lib = _ext._lib if _ext._lib is not None else load_int4_gemm()
     with _on_device(dev):
-        _check(lib.pi05w4a4_kv_append(k.data_ptr(), ks, v.data_ptr(), vs, elem, b, t, kvh, d, k_cache.data_ptr(),
-                                      v_cache.data_ptr(), pages, table.data_ptr(), stride, table.size(1), lens.data_ptr(),
-                                      _ptr(counts), _stream(dev)), "pi05w4a4_kv_append")
+        _check(lib.pi05w4a4_kv_append(k.data_ptr(), ks, v.data_ptr(), vs, *shape, kp, vp, pages, table.data_ptr(), stride,
+                                      table.size(1), lens.data_ptr(), _ptr(counts), _stream(dev)), "pi05w4a4_kv_append")
+
+
+def _check_rope_append(what, q, k, v, q_weight, k_weight, positions, inv_freq, k_cache, v_cache, table, lens, counts, axes):
+    found = _check_rope(what, q, k, q_weight, k_weight, positions, inv_freq, axes)
+    if v.dtype != k.dtype or v.shape != k.shape or v.device != q.device:
+        raise RuntimeError(f"{what}: v must be {k.dtype} {tuple(k.shape)} on {q.device}, got {v.dtype} {tuple(v.shape)} on {v.device}")
+    _, b, t, _, kvh, d = found[0]
+    pages = _check_cache(what, q, k_cache, v_cache, table, lens, b, t, kvh, d)
+    _ints(what, "counts", counts, b, q.device)
+    return *found, pages, _strides(v)
 
 
 def _rope_append_impl(q, k, v, q_weight, k_weight, eps, positions, inv_freq, k_cache, v_cache, block_table, lens, counts,
                       unit_offset, interleaved, axes):
     what = "qk_norm_rope_append"
-    kept, heads, shape, rest = _rope_args(what, q, k, q_weight, k_weight, eps, positions, inv_freq, unit_offset, interleaved, axes)
+    axes = None if axes is None else tuple(axes)
+    shape, qs, ks, ps, count, amap, pages, vs = _plan(
+        (what, _meta(q), _meta(k), _meta(v), _meta(q_weight), _meta(k_weight), _meta(positions), _meta(inv_freq), _meta(k_cache),
+         _meta(v_cache), _meta(block_table), _meta(lens), _meta(counts), axes),
+        lambda: _check_rope_append(what, q, k, v, q_weight, k_weight, positions, inv_freq, k_cache, v_cache, block_table, lens,
+                                   counts, axes))
+    kp, vp = _cache_pointers(what, k_cache, v_cache)
     dev = q.device
-    if v.dtype != k.dtype or v.shape != k.shape or v.device != dev:
-        raise RuntimeError(f"{what}: v must be {k.dtype} {tuple(k.shape)} on {dev}, got {v.dtype} {tuple(v.shape)} on {v.device}")
-    elem, b, t, h, kvh, d = shape
-    pages = _check_cache(what, q, k_cache, v_cache, block_table, lens, b, t, kvh, d)
-    counts = _ints(what, "counts", counts, b, dev)
     q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
     table, stride = _table(block_table)
-    lens = lens.contiguous()
-    v, vs = _strided(v)
+    lens, counts = lens.contiguous(), None if counts is None else counts.contiguous()
+    q, qs = _heads(q, qs)
+    k, ks = _heads(k, ks)
+    v, vs = _heads(v, vs)
+    q_weight, k_weight, inv_freq = _weight(q_weight), _weight(k_weight), inv_freq.contiguous()
     lib = _ext._lib if _ext._lib is not None else load_int4_gemm()
     with _on_device(dev):
-        _check(lib.pi05w4a4_qk_norm_rope_append(*heads, v.data_ptr(), vs, *shape, *rest, q_out.data_ptr(), k_cache.data_ptr(),
-                                                v_cache.data_ptr(), pages, table.data_ptr(), stride, table.size(1),
-                                                lens.data_ptr(), _ptr(counts), _stream(dev)), "pi05w4a4_qk_norm_rope_append")
-    del kept
+        _check(lib.pi05w4a4_qk_norm_rope_append(q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, *shape, _ptr(q_weight),
+                                                _ptr(k_weight), eps, unit_offset, positions.data_ptr(), ps,
+                                                positions.element_size(), count, amap, inv_freq.data_ptr(), 2 * inv_freq.numel(),
+                                                interleaved, q_out.data_ptr(), kp, vp, pages, table.data_ptr(), stride,
+                                                table.size(1), lens.data_ptr(), _ptr(counts), _stream(dev)),
+               "pi05w4a4_qk_norm_rope_append")
     return q_out
 
 
-def _attention_impl(q, k_cache, v_cache, block_table, lens, scaling, causal, q_lens, return_lse):
-    what = "kv_attention"
+def _check_attention(what, q, k_cache, v_cache, table, lens, q_lens):
     if not q.is_cuda:
         raise RuntimeError(f"{what} expects CUDA/HIP tensors")
-    dev = q.device
     elem = ELEM.get(q.dtype)
     if elem is None:
         raise RuntimeError(f"{what} takes float16 or bfloat16 queries, got {q.dtype}")
@@ -130,29 +156,33 @@ def _attention_impl(q, k_cache, v_cache, block_table, lens, scaling, causal, q_l
         raise RuntimeError(f"{what}: the query heads must be a multiple of the KV heads, got {h} and {kvh}")
     if h > 65535:  # here: the library takes them as 32 bits
         raise RuntimeError(f"{what}: at most 65535 query heads, got {h}")
-    pages = _check_cache(what, q, k_cache, v_cache, block_table, lens, b, t, kvh, d)
-    q_lens = _ints(what, "q_lens", q_lens, b, dev)
+    pages = _check_cache(what, q, k_cache, v_cache, table, lens, b, t, kvh, d)
+    _ints(what, "q_lens", q_lens, b, q.device)
+    with _on_device(q.device):
+        need = int(load_int4_gemm().pi05w4a4_kv_attention_workspace_bytes(b, t, h, kvh, d, table.size(1)))
+    return (elem, b, t, h, kvh, d), pages, _strides(q), need
+
+
+def _attention_impl(q, k_cache, v_cache, block_table, lens, scaling, causal, q_lens, return_lse):
+    what = "kv_attention"
+    shape, pages, qs, need = _plan(
+        (what, _meta(q), _meta(k_cache), _meta(v_cache), _meta(block_table), _meta(lens), _meta(q_lens)),
+        lambda: _check_attention(what, q, k_cache, v_cache, block_table, lens, q_lens))
+    kp, vp = _cache_pointers(what, k_cache, v_cache)
+    dev = q.device
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    lse = torch.empty((b, t, h), dtype=torch.float32, device=dev) if return_lse else None
-    if b == 0 or t == 0:
+    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=dev) if return_lse else None
+    if shape[1] == 0 or shape[2] == 0:
         return out, lse
     table, stride = _table(block_table)
-    lens = lens.contiguous()
-    q, qs = _strided(q)
-    tp = table.size(1)
+    lens, q_lens = lens.contiguous(), None if q_lens is None else q_lens.contiguous()
+    q, qs = _heads(q, qs)
     lib = _ext._lib if _ext._lib is not None else load_int4_gemm()
     with _on_device(dev):
-        key = (dev.index, b, t, h, kvh, d, tp)
-        need = _ATTN_WS.get(key)
-        if need is None:
-            if len(_ATTN_WS) > 4096:
-                _ATTN_WS.clear()
-            need = _ATTN_WS[key] = int(lib.pi05w4a4_kv_attention_workspace_bytes(b, t, h, kvh, d, tp))
         ws = _workspace(dev, need) if need else None
-        _check(lib.pi05w4a4_kv_attention(q.data_ptr(), qs, elem, b, t, h, kvh, d, k_cache.data_ptr(), v_cache.data_ptr(),
-                                         pages, table.data_ptr(), stride, tp, lens.data_ptr(), _ptr(q_lens), scaling,
-                                         1 if causal else 0, out.data_ptr(), _ptr(lse), _ptr(ws), need, _stream(dev)),
-               "pi05w4a4_kv_attention")
+        _check(lib.pi05w4a4_kv_attention(q.data_ptr(), qs, *shape, kp, vp, pages, table.data_ptr(), stride, table.size(1),
+                                         lens.data_ptr(), _ptr(q_lens), scaling, causal, out.data_ptr(), _ptr(lse), _ptr(ws), need,
+                                         _stream(dev)), "pi05w4a4_kv_attention")
     return out, lse
 
 

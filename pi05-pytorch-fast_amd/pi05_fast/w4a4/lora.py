@@ -16,15 +16,13 @@ from pi05_fast.w4a4 import extension as _ext
 from pi05_fast.w4a4.extension import (_check, _direct, _on_device, _ptr, _refuse_tangents, _stream, _workspace,
                                       load_int4_gemm)
 from pi05_fast.w4a4.int8 import ELEM
+from pi05_fast.w4a4.rope import _meta, _plan
 
 MAX_RANK = 128
 MAX_SLICES = 4
 MAX_ROWS = 1 << 26
 MAX_K = 1 << 20
 MAX_N = 1 << 22
-
-_WS: dict[tuple, int] = {}
-_WIDTHS: dict[tuple, ctypes.Array] = {}
 
 
 def _row_stride(t: torch.Tensor) -> int | None:
@@ -46,9 +44,9 @@ def _row_stride(t: torch.Tensor) -> int | None:
     return t.size(-1) if ld is None else ld
 
 
-def _lora_impl(y, x, a, b, ids, scale, slices, out):
-    """out = None: a new tensor; else the tensor (y itself) that is written."""
-    what = "lora_add" if out is None else "lora_add_"
+def _check_lora(what, y, x, a, b, ids, scale, widths, in_place):
+    """The checks, and what they find: (m, k, n, r, adapters, rows an id), the row strides of y and x (None: to be copied), the widths
+    for the library and the workspace."""
     if not y.is_cuda:
         raise RuntimeError(f"{what} expects CUDA/HIP tensors")
     dev, dtype = y.device, y.dtype
@@ -58,7 +56,7 @@ def _lora_impl(y, x, a, b, ids, scale, slices, out):
     if y.dim() < 1 or x.dim() != y.dim() or x.shape[:-1] != y.shape[:-1]:
         raise RuntimeError(f"{what} expects y [..., N] and x [..., K] of the same rows, got {tuple(y.shape)} and {tuple(x.shape)}")
     lead, n, k = y.shape[:-1], y.size(-1), x.size(-1)
-    widths = (n,) if slices is None else tuple(slices)
+    widths = (n,) if widths is None else widths
     if not 1 <= len(widths) <= MAX_SLICES or sum(widths) != n or (n > 0 and min(widths) <= 0):
         raise RuntimeError(f"{what}: slices are 1 to {MAX_SLICES} positive widths whose sum is N = {n}, got {widths}")
     if a.dim() != 3 or b.dim() != 3 or a.size(0) != b.size(0) or a.size(2) != k or b.size(1) != n \
@@ -77,46 +75,47 @@ def _lora_impl(y, x, a, b, ids, scale, slices, out):
         if t is not None and t.device != dev:
             raise RuntimeError(f"{what}: all tensors must be on {dev}, got {t.device}")
     m = 1
-    for s in lead:
-        m *= s
+    for size in lead:
+        m *= size
     if m > MAX_ROWS:
         raise RuntimeError(f"{what}: at most {MAX_ROWS} rows, got {m}")
-    ldy = _row_stride(y)
-    if out is None:
-        if ldy is None:
-            y = y.contiguous()
-            ldy = n
-        out = torch.empty(y.shape, dtype=dtype, device=dev)
-        ldo = n
+    ldy, ldx = _row_stride(y), _row_stride(x)
+    if in_place and (ldy is None or (m > 1 and ldy < n)):
+        raise RuntimeError(f"{what}: the rows of y must lie at one stride and apart, got strides {y.stride()} of {tuple(y.shape)}")
+    per_id = m // ids.numel() if m > 0 else 1
+    need = 0
+    if m > 0 and n > 0:
+        with _on_device(dev):
+            need = int(load_int4_gemm().pi05w4a4_lora_workspace_bytes(m, per_id, k, n, r, len(widths), adapters))
+    return ((m, k, n, r, adapters, per_id), ldy, None if ldx is None or ldx % 8 else ldx,
+            (ctypes.c_int32 * len(widths))(*widths), elem, need)
+
+
+def _lora_impl(y, x, a, b, ids, scale, slices, in_place):
+    what = "lora_add_" if in_place else "lora_add"
+    slices = None if slices is None else tuple(slices)
+    (m, k, n, r, adapters, per_id), ldy, ldx, widths, elem, need = _plan(
+        (what, _meta(y), _meta(x), _meta(a), _meta(b), _meta(ids), _meta(scale), slices),
+        lambda: _check_lora(what, y, x, a, b, ids, scale, slices, in_place))
+    dev = y.device
+    if in_place:
+        out, ldo = y, max(ldy, n)  # of a single row the stride may be anything
     else:
-        ldo = ldy
-        if ldy is None or (m > 1 and ldy < n):
-            raise RuntimeError(f"{what}: the rows of y must lie at one stride and apart, got strides {y.stride()} of {tuple(y.shape)}")
+        out, ldo = torch.empty_like(y, memory_format=torch.contiguous_format), n
+        if ldy is None:
+            y, ldy = y.contiguous(), n
     if m == 0 or n == 0:
         return out
-    ldx = _row_stride(x)
-    if ldx is None or ldx % 8 or x.data_ptr() % 16:
+    if ldx is None or x.data_ptr() % 16:
         x, ldx = x.clone(memory_format=torch.contiguous_format), k
     a, b, ids = _whole(a), _whole(b), ids.contiguous()
     scale = None if scale is None else scale.contiguous()
-    arr = _WIDTHS.get(widths)
-    if arr is None:
-        if len(_WIDTHS) > 4096:
-            _WIDTHS.clear()
-        arr = _WIDTHS[widths] = (ctypes.c_int32 * len(widths))(*widths)
-    per_id = m // ids.numel()
     lib = _ext._lib if _ext._lib is not None else load_int4_gemm()
     with _on_device(dev):
-        key = (dev.index, m, per_id, k, n, r, len(widths), adapters)
-        need = _WS.get(key)
-        if need is None:
-            if len(_WS) > 4096:
-                _WS.clear()
-            need = _WS[key] = int(lib.pi05w4a4_lora_workspace_bytes(m, per_id, k, n, r, len(widths), adapters))
         ws = _workspace(dev, need) if need else None
-        _check(lib.pi05w4a4_lora_add(y.data_ptr(), ldy, x.data_ptr(), ldx, m, k, a.data_ptr(), b.data_ptr(), _ptr(scale), adapters,
-                                     r, ids.data_ptr(), per_id, n, len(widths), arr, elem, out.data_ptr(), ldo, _ptr(ws), need,
-                                     _stream(dev)), "pi05w4a4_lora_add")
+        _check(lib.pi05w4a4_lora_add(y.data_ptr(), ldo if in_place else ldy, x.data_ptr(), ldx, m, k, a.data_ptr(), b.data_ptr(),
+                                     _ptr(scale), adapters, r, ids.data_ptr(), per_id, n, len(widths), widths, elem, out.data_ptr(),
+                                     ldo, _ptr(ws), need, _stream(dev)), "pi05w4a4_lora_add")
     return out
 
 
@@ -131,7 +130,7 @@ def _whole(t: torch.Tensor) -> torch.Tensor:
 def _lora_op(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, ids: torch.Tensor,
              scale: torch.Tensor | None, slices: Sequence[int] | None) -> torch.Tensor:
     _refuse_tangents(y, x, a, b, scale)
-    return _lora_impl(y, x, a, b, ids, scale, slices, None)
+    return _lora_impl(y, x, a, b, ids, scale, slices, False)
 
 
 @_lora_op.register_fake
@@ -143,7 +142,7 @@ def _lora_fake(y, x, a, b, ids, scale, slices):
 def _lora_inplace_op(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, ids: torch.Tensor,
                      scale: torch.Tensor | None, slices: Sequence[int] | None) -> None:
     _refuse_tangents(y, x, a, b, scale)
-    _lora_impl(y, x, a, b, ids, scale, slices, y)
+    _lora_impl(y, x, a, b, ids, scale, slices, True)
 
 
 @_lora_inplace_op.register_fake
@@ -164,7 +163,7 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
     factors of their own: a is then [adapters, len(slices) * R, K], part g's rows g R .. g R + R - 1, and
     columns of part g take the R sums of that part.  There are no derivatives."""
     if _direct(y, x, a, b, ids, scale):
-        return _lora_impl(y, x, a, b, ids, scale, slices, None)
+        return _lora_impl(y, x, a, b, ids, scale, slices, False)
     return torch.ops.pi05_w4a4.lora_add(y, x, a, b, ids, scale, None if slices is None else list(slices))
 
 
@@ -173,6 +172,6 @@ def lora_add_(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor
     """``lora_add`` into y, which may be a part of a wider output (rows at one stride), and y.  Rows without an
     adapter are not touched."""
     if _direct(y, x, a, b, ids, scale):
-        return _lora_impl(y, x, a, b, ids, scale, slices, y)
+        return _lora_impl(y, x, a, b, ids, scale, slices, True)
     torch.ops.pi05_w4a4.lora_add_(y, x, a, b, ids, scale, None if slices is None else list(slices))
     return y

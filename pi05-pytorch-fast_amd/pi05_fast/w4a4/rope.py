@@ -17,15 +17,37 @@ import torch
 from pi05_fast.w4a4 import extension as _ext
 from pi05_fast.w4a4.extension import _check, _direct, _on_device, _ptr, _refuse_tangents, _stream, load_int4_gemm
 from pi05_fast.w4a4.int8 import ELEM
-from pi05_fast.w4a4.kv_int8 import _strided
 
 MAX_HEAD_DIM = 512
 MAX_AXES = 4
 MAX_HEADS = 32767
 MAX_TOKENS = 1 << 24  # tokens of a call
 
-_AXIS_MAPS: dict[tuple, ctypes.Array] = {}
-_POS_STRIDES: dict[tuple, ctypes.Array] = {}
+# What the checks of a call find depends on its tensors' types, devices, shapes and strides only: the arguments of
+# calls that passed them, by these.
+_PLANS: dict[tuple, tuple] = {}
+
+
+def _meta(t: torch.Tensor | None):
+    return None if t is None else (t.dtype, t.device, t.shape, t.stride())
+
+
+def _strides(t: torch.Tensor):
+    """The first three strides of t [B, T, heads, D] for the library, or None where its rows have to be copied
+    (16-byte alignment of the first is not looked at)."""
+    st, sz = t.stride(), t.shape
+    key = tuple(0 if sz[i] == 1 else st[i] for i in range(3))
+    if st[3] != 1 or key[0] % 8 or key[1] % 8 or key[2] % 8:
+        return None
+    return (ctypes.c_int64 * 3)(*key)
+
+
+def _heads(t: torch.Tensor, strides) -> tuple[torch.Tensor, ctypes.Array]:
+    """t with rows that the library takes, copied only where it has none."""
+    if strides is None or t.data_ptr() % 16:
+        t = t.clone(memory_format=torch.contiguous_format)
+        strides = (ctypes.c_int64 * 3)(*t.stride()[:3])
+    return t, strides
 
 
 def _axis_map(what, axes, pairs: int, count: int):
@@ -34,32 +56,27 @@ def _axis_map(what, axes, pairs: int, count: int):
         if count > 1:
             raise RuntimeError(f"{what}: positions of {count} axes need `axes`, the axis of each of the {pairs} rotated pairs")
         return None
-    key = (tuple(axes), count)
-    got = _AXIS_MAPS.get(key)
-    if got is None:
-        if any(not 0 <= int(a) < count for a in key[0]):
-            raise RuntimeError(f"{what}: axes must be in [0, {count}), the positions' axes, got {sorted(set(key[0]))}")
-        if len(_AXIS_MAPS) > 256:
-            _AXIS_MAPS.clear()
-        got = _AXIS_MAPS[key] = (ctypes.c_uint8 * len(key[0]))(*key[0])
-    if len(got) != pairs:
-        raise RuntimeError(f"{what}: axes must name the axis of each of the {pairs} rotated pairs, got {len(got)}")
-    return got
+    if len(axes) != pairs:
+        raise RuntimeError(f"{what}: axes must name the axis of each of the {pairs} rotated pairs, got {len(axes)}")
+    if any(not 0 <= a < count for a in axes):
+        raise RuntimeError(f"{what}: axes must be in [0, {count}), the positions' axes, got {sorted(set(axes))}")
+    return (ctypes.c_uint8 * pairs)(*axes)
 
 
-def _weight(what, name, w, x, d):
-    if w is None:
-        return None
-    if w.device != x.device or w.dtype != x.dtype or w.shape != (d,):
+def _check_weight(what, name, w, x, d):
+    if w is not None and (w.device != x.device or w.dtype != x.dtype or w.shape != (d,)):
         raise RuntimeError(f"{what}: {name} must be a {x.dtype} tensor [{d}] on {x.device}")
-    if not w.is_contiguous() or w.data_ptr() % 16:
+
+
+def _weight(w: torch.Tensor | None) -> torch.Tensor | None:
+    if w is not None and (not w.is_contiguous() or w.data_ptr() % 16):
         w = w.clone(memory_format=torch.contiguous_format)
     return w
 
 
-def _rope_args(what, q, k, q_weight, k_weight, eps, positions, inv_freq, unit_offset, interleaved, axes):
-    """Checks shared by the forms of the call, and the arguments that they hand on: (kept tensors,
-    the library's arguments up to the first output)."""
+def _check_rope(what, q, k, q_weight, k_weight, positions, inv_freq, axes):
+    """The checks shared by the forms of the call, and what they find: (elem, b, t, h, kvh, d), the strides of q, k and the
+    positions, the number of axes and their map."""
     if not q.is_cuda:
         raise RuntimeError(f"{what} expects CUDA/HIP tensors")
     dev = q.device
@@ -75,8 +92,8 @@ def _rope_args(what, q, k, q_weight, k_weight, eps, positions, inv_freq, unit_of
         raise RuntimeError(f"{what}: head_dim must be a multiple of 16 of at most {MAX_HEAD_DIM}, got {d}")
     if not 0 < h <= MAX_HEADS or not 0 < kvh <= MAX_HEADS or b * t > MAX_TOKENS:  # here: the library takes them as 32 bits
         raise RuntimeError(f"{what}: 1 to {MAX_HEADS} heads and at most {MAX_TOKENS} tokens, got {h} and {kvh} heads, {b} x {t}")
-    q_weight = _weight(what, "q_weight", q_weight, q, d)
-    k_weight = _weight(what, "k_weight", k_weight, q, d)
+    _check_weight(what, "q_weight", q_weight, q, d)
+    _check_weight(what, "k_weight", k_weight, q, d)
     if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or inv_freq.device != dev:
         raise RuntimeError(f"{what}: inv_freq must be float32 [rotated dimensions / 2] on {dev}, got {inv_freq.dtype} "
                            f"{tuple(inv_freq.shape)} on {inv_freq.device}")
@@ -90,31 +107,37 @@ def _rope_args(what, q, k, q_weight, k_weight, eps, positions, inv_freq, unit_of
     count = positions.size(0) if positions.dim() == 3 else 1
     amap = _axis_map(what, axes, pairs, count)
     ps = positions.stride() if positions.dim() == 3 else (0, *positions.stride())
-    strides = _POS_STRIDES.get(ps)
-    if strides is None:
-        if len(_POS_STRIDES) > 4096:
-            _POS_STRIDES.clear()
-        strides = _POS_STRIDES[ps] = (ctypes.c_int64 * 3)(*ps)
-    q, qs = _strided(q)
-    k, ks = _strided(k)
-    inv_freq = inv_freq.contiguous()
-    kept = (q, k, q_weight, k_weight, inv_freq)
-    shape = (elem, b, t, h, kvh, d)
-    rest = (_ptr(q_weight), _ptr(k_weight), eps, 1 if unit_offset else 0, positions.data_ptr(), strides,
-            positions.element_size(), count, amap, inv_freq.data_ptr(), 2 * pairs, 1 if interleaved else 0)
-    return kept, (q.data_ptr(), qs, k.data_ptr(), ks), shape, rest
+    return (elem, b, t, h, kvh, d), _strides(q), _strides(k), (ctypes.c_int64 * 3)(*ps), count, amap
+
+
+def _plan(key: tuple, make) -> tuple:
+    got = _PLANS.get(key)
+    if got is None:
+        got = make()
+        if len(_PLANS) > 4096:
+            _PLANS.clear()
+        _PLANS[key] = got
+    return got
 
 
 def _rope_impl(q, k, q_weight, k_weight, eps, positions, inv_freq, unit_offset, interleaved, axes):
     what = "qk_norm_rope"
-    kept, heads, shape, rest = _rope_args(what, q, k, q_weight, k_weight, eps, positions, inv_freq, unit_offset, interleaved, axes)
+    axes = None if axes is None else tuple(axes)
+    shape, qs, ks, ps, count, amap = _plan(
+        (what, _meta(q), _meta(k), _meta(q_weight), _meta(k_weight), _meta(positions), _meta(inv_freq), axes),
+        lambda: _check_rope(what, q, k, q_weight, k_weight, positions, inv_freq, axes))
+    dev = q.device
     q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
     k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
+    q, qs = _heads(q, qs)
+    k, ks = _heads(k, ks)
+    q_weight, k_weight, inv_freq = _weight(q_weight), _weight(k_weight), inv_freq.contiguous()
     lib = _ext._lib if _ext._lib is not None else load_int4_gemm()
-    with _on_device(q.device):
-        _check(lib.pi05w4a4_qk_norm_rope(*heads, *shape, *rest, q_out.data_ptr(), k_out.data_ptr(), _stream(q.device)),
-               "pi05w4a4_qk_norm_rope")
-    del kept
+    with _on_device(dev):
+        _check(lib.pi05w4a4_qk_norm_rope(q.data_ptr(), qs, k.data_ptr(), ks, *shape, _ptr(q_weight), _ptr(k_weight), eps,
+                                         unit_offset, positions.data_ptr(), ps, positions.element_size(), count, amap,
+                                         inv_freq.data_ptr(), 2 * inv_freq.numel(), interleaved, q_out.data_ptr(),
+                                         k_out.data_ptr(), _stream(dev)), "pi05w4a4_qk_norm_rope")
     return q_out, k_out
 
 

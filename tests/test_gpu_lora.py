@@ -63,7 +63,8 @@ def _exact(y, x, a, b, row_ids, scale, widths):
 
 
 SHAPES = [(1, 64, 8, 8, 1, 1), (1, 2048, 2560, 16, 5, 3), (3, 104, 33, 24, 2, 1), (17, 2048, 130, 8, 30, 2), (64, 512, 2048, 16, 64, 1),
-          (40, 1000, 999, 40, 7, 1), (200, 264, 192, 64, 3, 3), (33, 16384, 64, 128, 4, 4), (700, 128, 257, 32, 6, 1), (257, 40, 96, 128, 2, 2)]
+          (40, 1000, 999, 40, 7, 1), (200, 264, 192, 64, 3, 3), (33, 16384, 64, 128, 4, 4), (700, 128, 257, 32, 6, 1), (257, 40, 96, 128, 2, 2),
+          (40, 4104, 320, 64, 5, 1), (20, 16384, 130, 24, 3, 1), (1, 16384, 96, 16, 2, 3), (300, 2048, 1100, 16, 40, 1)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)

@@ -193,8 +193,9 @@ def test_lora_refusals(lib, kw, text):
 
 
 def test_lora_workspace_is_checked(lib):
-    need = lib.pi05w4a4_lora_workspace_bytes(2, 1, 64, 32, 8, 1, 2)
+    need = lib.pi05w4a4_lora_workspace_bytes(2, 1, 16384, 32, 8, 1, 2)
     assert need > 0 and need % (512 * 4) == 0
-    assert _lora(lib, wsb=need - 4) == 3 and "workspace" in _err(lib)
-    for args in ((0, 1, 64, 32, 8, 1, 2), (2, 1, 60, 32, 8, 1, 2), (2, 0, 64, 32, 8, 1, 2), (2, 1, 64, 0, 8, 1, 2), (2, 1, 64, 32, 8, 1, 0)):
+    assert _lora(lib, k=16384, ldx=16384, wsb=need - 4) == 3 and "workspace" in _err(lib)
+    for args in ((0, 1, 64, 32, 8, 1, 2), (2, 1, 60, 32, 8, 1, 2), (2, 0, 64, 32, 8, 1, 2), (2, 1, 64, 0, 8, 1, 2), (2, 1, 64, 32, 8, 1, 0),
+                 (2, 1, 64, 32, 8, 1, 2)):  # the last: one launch
         assert lib.pi05w4a4_lora_workspace_bytes(*args) == 0
