@@ -522,7 +522,8 @@ int pi05w4a4_int8_kv_attention(const void* q, const int64_t* q_strides, int32_t 
  *     f = x * g / sqrt(mean_d(x^2) + eps), g = 1 + w (unit_offset) or w, or f = x where the weight is null;
  *     pair j < rot / 2 is dimensions (j, j + rot / 2), or (2j, 2j + 1) when interleaved, and turns by
  *     pos * inv_freq[j]: (f1 c - f2 s, f2 c + f1 s); dimensions from rot on stay f.
- *   rot % 16 == 0 (0: no rotation).  Positions are [axes, B, T] of int32 or int64 (pos_bytes 4 or 8), with strides
+ *   A call of more than 2^26 waves, each three times 1024 / D heads of a token, is refused.  rot % 16 == 0 (0: no
+ *   rotation).  Positions are [axes, B, T] of int32 or int64 (pos_bytes 4 or 8), with strides
  *   {axis, batch, token} in elements; axis_of_pair (host, rot / 2 bytes; null: all 0) names the axis of each
  *   pair, at most 4 axes.  fp32 with one rounding; angles are reduced in 64 bits.
  *
@@ -540,8 +541,8 @@ int pi05w4a4_int8_kv_attention(const void* q, const int64_t* q_strides, int32_t 
  *   i >= ql.  lens counts the new tokens too; one past table_pages * 64 counts as that, for the place of the
  *   queries as well.  A query that sees none gets zeros.  What a query does not see has no effect on it, NaN
  *   and infinities too; a NaN or infinity among the values that it sees makes its outputs in that
- *   dimension NaN.  lse, when not null, fp32 [B, T, H]: the natural log of the sum of exp(scaling q k) (-inf
- *   where none is seen).  Query head h reads KV head h / (H / KVH).  Needs
+ *   dimension NaN or infinite.  lse, when not null, fp32 [B, T, H]: the natural log of the sum of
+ *   exp(scaling q k) (-inf where none is seen).  Query head h reads KV head h / (H / KVH).  Needs
  *   pi05w4a4_kv_attention_workspace_bytes(...) bytes (0 without a split, at most 2^28).
  *
  * pi05w4a4_lora_add: out[m, n] = y[m, n] + scale[id] * sum_r (sum_k x[m, k] a[id, g r0 + r, k]) b[id, n, r] with
@@ -549,7 +550,7 @@ int pi05w4a4_int8_kv_attention(const void* q, const int64_t* q_strides, int32_t 
  *   slice of N), at most 4, and rows g r .. g r + r - 1 of a.  a [adapters, slices * r, K], b [adapters, N, r],
  *   contiguous; scale [adapters], null for 1.  ids outside [0, adapters) name no adapter: out = y.  x has row
  *   stride ldx (% 8 == 0, 16-byte aligned), K % 8 == 0, K <= 2^20; y and out have row strides of any size and may
- *   be the same matrix, but must not overlap otherwise (x may be either: it is read before out is written).
+ *   be the same matrix, but must not overlap otherwise, nor x and out.
  *   r % 8 == 0, r <= 128; smaller ranks are padded with zeros.  fp32 with one rounding.  M <= 2^26, N <= 2^22.
  *   Needs pi05w4a4_lora_workspace_bytes(...) bytes.
  */

@@ -61,6 +61,15 @@ void set_strides(int64_t* to, const int64_t* from) {
 
 }  // namespace
 
+static int run_head_rope(HeadRopeParams& p, int32_t elem, void* stream, const char* what) {
+  p.parts = head_rope_parts(p, device_cu_count());
+  // A launch holds fewer than 2^32 threads: a wave for each part of a token.
+  if (static_cast<int64_t>(p.b) * p.t * p.parts >= (1 << 26))
+    return capi_fail(PI05W4A4_EINVAL, "%d x %d tokens of %d heads are more than one launch holds", p.b, p.t,
+                     p.heads[0] + p.heads[1] + p.heads[2]);
+  return capi_hip(launch_head_rope(p, elem, static_cast<hipStream_t>(stream)), what);
+}
+
 // Everything of pi05w4a4_qk_norm_rope and its append form but the destination of the keys.
 static int rope_params(HeadRopeParams& p, const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
                        int32_t elem, int32_t b, int32_t t, int32_t h, int32_t kvh, int32_t d, const void* q_weight,
@@ -131,7 +140,7 @@ extern "C" int pi05w4a4_qk_norm_rope(const void* q, const int64_t* q_strides, co
   if (b == 0 || t == 0) return capi_ok();
   if (k_out == nullptr || !aligned(k_out, 16)) return capi_fail(PI05W4A4_EINVAL, "the outputs must be 16-byte aligned");
   p.k_out = k_out;
-  return capi_hip(launch_head_rope(p, elem, static_cast<hipStream_t>(stream)), "qk_norm_rope launch");
+  return run_head_rope(p, elem, stream, "qk_norm_rope launch");
 }
 
 extern "C" int pi05w4a4_qk_norm_rope_append(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
@@ -157,7 +166,7 @@ extern "C" int pi05w4a4_qk_norm_rope_append(const void* q, const int64_t* q_stri
   set_strides(p.stride[2], v_strides);
   p.heads[2] = kvh;
   p.counts = counts;
-  return capi_hip(launch_head_rope(p, elem, static_cast<hipStream_t>(stream)), "qk_norm_rope_append launch");
+  return run_head_rope(p, elem, stream, "qk_norm_rope_append launch");
 }
 
 extern "C" int pi05w4a4_kv_append(const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides, int32_t elem,
@@ -184,7 +193,7 @@ extern "C" int pi05w4a4_kv_append(const void* k, const int64_t* k_strides, const
   set_strides(p.stride[1], k_strides);
   set_strides(p.stride[2], v_strides);
   p.counts = counts;
-  return capi_hip(launch_head_rope(p, elem, static_cast<hipStream_t>(stream)), "kv_append launch");
+  return run_head_rope(p, elem, stream, "kv_append launch");
 }
 
 extern "C" size_t pi05w4a4_kv_attention_workspace_bytes(int32_t b, int32_t t, int32_t h, int32_t kvh, int32_t d,
@@ -246,6 +255,16 @@ static int check_lora(int64_t m, int64_t per_id, int32_t k, int32_t n, int32_t r
   return PI05W4A4_OK;
 }
 
+// Whether rows of k elements at x and of n at out share bytes (2 bytes an element): rows beside each other in wider ones do not.
+static bool rows_overlap(const void* x, int64_t ldx, int32_t k, const void* out, int64_t ldo, int32_t n, int64_t m) {
+  const int64_t a = reinterpret_cast<intptr_t>(x), b = reinterpret_cast<intptr_t>(out);
+  const int64_t a_end = a + 2 * ((m - 1) * ldx + k), b_end = b + 2 * ((m - 1) * ldo + n);
+  if (a_end <= b || b_end <= a) return false;
+  if (ldx != ldo || ldx < k + static_cast<int64_t>(n)) return true;
+  const int64_t ld = 2 * ldo, off = ((a - b) % ld + ld) % ld;  // of x's rows behind out's
+  return off < 2 * static_cast<int64_t>(n) || off + 2 * static_cast<int64_t>(k) > ld;
+}
+
 static size_t lora_workspace(int64_t m, int32_t r, int32_t slices, int ksplit) {
   return sizeof(float) * static_cast<size_t>(ksplit) * static_cast<size_t>(lora_h_floats(m, r, slices));
 }
@@ -277,6 +296,7 @@ extern "C" int pi05w4a4_lora_add(const void* y, int64_t ldy, const void* x, int6
     return capi_fail(PI05W4A4_EINVAL, "x, a and b must be 16-byte aligned");
   if (ldx < 0 || ldx % 8 != 0) return capi_fail(PI05W4A4_EINVAL, "the row stride of x must be a multiple of 8 elements, got %lld", (long long)ldx);
   if (ldy < 0 || ldo < n) return capi_fail(PI05W4A4_EINVAL, "row strides must be >= 0, and those of the output >= N");
+  if (rows_overlap(x, ldx, k, out, ldo, n, m)) return capi_fail(PI05W4A4_EINVAL, "x must not overlap the output");
   const LoraPlan plan = lora_plan(m, per_id, k, n, r, slices, adapters, device_cu_count());
   const size_t need = adapters > 0 ? lora_workspace(m, r, slices, plan.ksplit) : 0;
   if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned(workspace, 16)))

@@ -239,21 +239,27 @@ void launch_lanes(const HeadRopeParams& p, int lanes, hipStream_t stream) {
 
 }  // namespace
 
-hipError_t launch_head_rope(HeadRopeParams p, int elem, hipStream_t stream) {
-  if (p.b <= 0 || p.t <= 0) return hipSuccess;
+static int head_lanes(int32_t d) {
   int lanes = 1;
-  while (lanes < p.d / 16) lanes *= 2;
-  // A wave for each round of heads where tokens are few, else up to three rounds a wave (4 x 1536 tokens of 32 + 8 heads
-  // of 128, five rounds, in 1 / 2 parts: 28.1 / 26.6 us; 8 x 776 of 8 + 1 + 1 heads of 256, three rounds: 17.3 / 20.1).
-  const int rounds = (p.heads[0] + p.heads[1] + p.heads[2] + 64 / lanes - 1) / (64 / lanes);
-  const int64_t tokens = static_cast<int64_t>(p.b) * p.t;
-  const int64_t want = (8LL * device_cu_count() + tokens - 1) / tokens;
-  p.parts = static_cast<int>(want < rounds ? want : rounds);
-  if (p.parts < (rounds + 2) / 3) p.parts = (rounds + 2) / 3;
+  while (lanes < d / 16) lanes *= 2;
+  return lanes;
+}
+
+// A wave for each round of heads where tokens are few, else up to three rounds a wave (4 x 1536 tokens of 32 + 8 heads
+// of 128, five rounds, in 1 / 2 parts: 28.1 / 26.6 us; 8 x 776 of 8 + 1 + 1 heads of 256, three rounds: 17.3 / 20.1).
+int32_t head_rope_parts(const HeadRopeParams& p, int cus) {
+  const int64_t heads_a_round = 64 / head_lanes(p.d), tokens = static_cast<int64_t>(p.b) * p.t;
+  const int64_t rounds = (static_cast<int64_t>(p.heads[0]) + p.heads[1] + p.heads[2] + heads_a_round - 1) / heads_a_round;
+  const int64_t want = (8LL * cus + tokens - 1) / tokens, few = want < rounds ? want : rounds, least = (rounds + 2) / 3;
+  return static_cast<int32_t>(few > least ? few : least);
+}
+
+hipError_t launch_head_rope(const HeadRopeParams& p, int elem, hipStream_t stream) {
+  if (p.b <= 0 || p.t <= 0) return hipSuccess;
   if (elem == kFp16)
-    launch_lanes<_Float16>(p, lanes, stream);
+    launch_lanes<_Float16>(p, head_lanes(p.d), stream);
   else
-    launch_lanes<__bf16>(p, lanes, stream);
+    launch_lanes<__bf16>(p, head_lanes(p.d), stream);
   return hipGetLastError();
 }
 

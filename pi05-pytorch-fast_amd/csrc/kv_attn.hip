@@ -132,13 +132,13 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void kv_attn16_kernel(KvA
   const int head = blockIdx.y, b = blockIdx.z;
   const Span span(p, b);
 
-  // This lane's row; rows past the last one, and tokens past q_len, see nothing.
+  // This lane's row; tokens past q_len see nothing.
   const int row = tile * 16 + col;
   const int tok = min(row / group, p.t - 1), qh = head * group + row % group;
   const int64_t seen = row < rows ? span.seen(row / group) : 0;
   const int64_t tok_first = tile * 16 / group, tok_last = min(tile * 16 + 15, rows - 1) / group;
   const int64_t most = span.most(tok_first, tok_last);
-  const int64_t least = tile * 16 + 15 < rows ? span.least(tok_first, tok_last) : 0;
+  const int64_t least = span.least(tok_first, tok_last);  // rows past the last one are computed as they come, and not stored
   const int pages = static_cast<int>((most + kKvPage - 1) / kKvPage);
   // The run's pages are split, split + nsplit, ..: the first is known without the length.  Its steps are
   // the halves of 32 keys; a last half that no row sees is left out.

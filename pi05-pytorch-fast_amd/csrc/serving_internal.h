@@ -43,7 +43,8 @@ struct HeadRopeParams {
   KvCache16 c;            // c.lens null: no cache
   const int32_t* counts;  // [B] or null: all T
 };
-hipError_t launch_head_rope(HeadRopeParams p, int elem, hipStream_t stream);
+int32_t head_rope_parts(const HeadRopeParams& p, int cus);
+hipError_t launch_head_rope(const HeadRopeParams& p, int elem, hipStream_t stream);
 
 struct KvAttn16Params {
   KvCache16 c;

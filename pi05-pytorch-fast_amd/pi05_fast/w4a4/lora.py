@@ -44,6 +44,16 @@ def _row_stride(t: torch.Tensor) -> int | None:
     return t.size(-1) if ld is None else ld
 
 
+def _may_share(x: torch.Tensor, y: torch.Tensor) -> bool:
+    """Whether x and y can hold the same bytes: x is then copied, as the kernels read it while they write y."""
+    if x.data_ptr() == y.data_ptr():
+        return True
+    ends = []
+    for t in (x, y):
+        ends.append(t.data_ptr() + 2 * (1 + sum((n - 1) * st for n, st in zip(t.shape, t.stride()))))
+    return x.data_ptr() < ends[1] and y.data_ptr() < ends[0]
+
+
 def _check_lora(what, y, x, a, b, ids, scale, widths, in_place):
     """The checks, and what they find: (m, k, n, r, adapters, rows an id), the row strides of y and x (None: to be copied), the widths
     for the library and the workspace."""
@@ -106,7 +116,7 @@ def _lora_impl(y, x, a, b, ids, scale, slices, in_place):
             y, ldy = y.contiguous(), n
     if m == 0 or n == 0:
         return out
-    if ldx is None or x.data_ptr() % 16:
+    if ldx is None or x.data_ptr() % 16 or (in_place and _may_share(x, y)):
         x, ldx = x.clone(memory_format=torch.contiguous_format), k
     a, b, ids = _whole(a), _whole(b), ids.contiguous()
     scale = None if scale is None else scale.contiguous()
@@ -170,7 +180,7 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
 def lora_add_(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, ids: torch.Tensor,
               scale: torch.Tensor | None = None, slices: Sequence[int] | None = None) -> torch.Tensor:
     """``lora_add`` into y, which may be a part of a wider output (rows at one stride), and y.  Rows without an
-    adapter are not touched."""
+    adapter are not touched.  An x in the same memory is copied first."""
     if _direct(y, x, a, b, ids, scale):
         return _lora_impl(y, x, a, b, ids, scale, slices, True)
     torch.ops.pi05_w4a4.lora_add_(y, x, a, b, ids, scale, None if slices is None else list(slices))

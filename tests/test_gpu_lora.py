@@ -136,11 +136,15 @@ def test_strides(cuda):
     assert torch.equal(w4a4.lora_add(y, x, a, b.transpose(1, 2).contiguous().transpose(1, 2), ids, scale), want)
     rows = y[:1].expand(37, 100)
     assert torch.equal(w4a4.lora_add(rows, x, a, b, ids, scale), _exact(rows.contiguous(), x, a, b, ids, scale, [100]))
-    # the projection's input is its output too
-    sq = x.clone()
+    # the projection's input is its output too, or lies in the same rows
     b2 = torch.randint(-2, 3, (4, 128, 8), device="cuda", generator=gen).bfloat16()
-    w4a4.lora_add_(sq, sq, a, b2, ids, scale)
-    assert torch.equal(sq, _exact(x, x, a, b2, ids, scale, [128]))
+    for _ in range(5):
+        sq = x.clone()
+        w4a4.lora_add_(sq, sq, a, b2, ids, scale)
+        assert torch.equal(sq, _exact(x, x, a, b2, ids, scale, [128]))
+    both = torch.cat((y, torch.zeros_like(y)[:, :4], x), dim=1)
+    w4a4.lora_add_(both[:, :100], both[:, 104:], a, b, ids, scale)
+    assert torch.equal(both[:, :100], want) and torch.equal(both[:, 104:], x)
 
 
 def test_what_is_not_finite_stays_in_its_rows(cuda):

@@ -161,6 +161,13 @@ def test_attention_refusals(lib, kw, text):
     assert _attend(lib, q=None, t=0) == 0 and _attend(lib, q=None, b=0) == 0
 
 
+def test_launches_of_too_many_waves(lib):
+    big = dict(b=4096, t=4096, kvh=32767)
+    assert _append(lib, **big) == 1 and "one launch" in _err(lib)
+    assert _rope(lib, h=32767, **big) == 1 and "one launch" in _err(lib)
+    assert _rope_append(lib, h=32767, **big) == 1 and "one launch" in _err(lib)
+
+
 def test_attention_workspace_is_checked(lib):
     need = lib.pi05w4a4_kv_attention_workspace_bytes(1, 1, 8, 1, 256, 128)
     assert need > 0
@@ -174,7 +181,7 @@ def test_attention_workspace_is_bounded(lib, b, t, h, kvh, d, pages):
     assert lib.pi05w4a4_kv_attention_workspace_bytes(b, t, h, kvh, d, pages) <= 1 << 28
 
 
-def _lora(lib, y=P, ldy=32, x=P, ldx=64, m=2, k=64, a=P, adapters=2, r=8, ids=P, per=1, n=32, slices=1, widths=None, elem=0, out=P, ldo=32,
+def _lora(lib, y=P, ldy=32, x=vp(1 << 20), ldx=64, m=2, k=64, a=P, adapters=2, r=8, ids=P, per=1, n=32, slices=1, widths=None, elem=0, out=P, ldo=32,
           ws=P, wsb=1 << 30):
     return lib.pi05w4a4_lora_add(y, ldy, x, ldx, m, k, a, P, None, adapters, r, ids, per, n, slices, widths, elem, out, ldo, ws, wsb, None)
 
@@ -186,6 +193,8 @@ def _lora(lib, y=P, ldy=32, x=P, ldx=64, m=2, k=64, a=P, adapters=2, r=8, ids=P,
     (dict(slices=2, widths=(ctypes.c_int32 * 2)(32, 0)), "has 0 columns"), (dict(slices=2, widths=(ctypes.c_int32 * 2)(16, 8)), "24 columns"),
     (dict(y=None), "null"), (dict(a=None), "null"), (dict(ids=None), "null"), (dict(x=vp(4104)), "aligned"), (dict(y=vp(4097)), "aligned"),
     (dict(ldx=60), "row stride of x"), (dict(ldo=31), "row strides"), (dict(ldy=-1), "row strides"),
+    (dict(x=vp(4096 + 64), out=P), "must not overlap"), (dict(x=vp(8192), ldx=128, out=vp(8192 + 100), ldo=128), "must not overlap"),
+    (dict(x=vp(8192 + 64), ldx=80, out=vp(8192), ldo=80), "must not overlap"),
 ])
 def test_lora_refusals(lib, kw, text):
     assert _lora(lib, **kw) == 1 and text in _err(lib)
