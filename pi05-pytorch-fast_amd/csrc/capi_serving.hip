@@ -215,6 +215,8 @@ extern "C" int pi05w4a4_kv_attention(const void* q, const int64_t* q_strides, in
     return capi_fail(PI05W4A4_EINVAL, "query heads must be a multiple of the KV heads, got %d and %d", h, kvh);
   if (static_cast<int64_t>(t) * (h / kvh) > (1 << 26))
     return capi_fail(PI05W4A4_EINVAL, "T * H / KVH must be at most 2^26, got T=%d H=%d KVH=%d", t, h, kvh);
+  if (static_cast<int64_t>(b) * t * h > (1 << 30))
+    return capi_fail(PI05W4A4_EINVAL, "B * T * H must be at most 2^30, got %d x %d x %d", b, t, h);
   if (!std::isfinite(scaling)) return capi_fail(PI05W4A4_EINVAL, "scaling must be finite");
   if (b == 0 || t == 0) return capi_ok();
   if (int rc = check_cache_pointers(p.c)) return rc;
@@ -224,6 +226,7 @@ extern "C" int pi05w4a4_kv_attention(const void* q, const int64_t* q_strides, in
   const KvAttn16Plan plan = kv_attn16_plan(b, t, h, kvh, d, table_pages, device_cu_count());
   p.nsplit = plan.nsplit;
   p.waves = plan.waves;
+  p.wide = plan.wide;
   const size_t need = kv_attn16_workspace(b, t, h, d, p.nsplit);
   if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned(workspace, 16)))
     return capi_fail(PI05W4A4_EWORKSPACE, "kv_attention needs a 16-byte aligned workspace of %zu bytes, got %zu", need, workspace_bytes);

@@ -59,10 +59,12 @@ struct KvAttn16Params {
   int32_t b, t, h;
   int32_t nsplit;         // runs of pages of a sequence
   int32_t waves;          // of a workgroup
+  int32_t wide;           // 64 rows a workgroup, not 16
 };
 struct KvAttn16Plan {
   int nsplit;
   int waves;
+  bool wide;
 };
 KvAttn16Plan kv_attn16_plan(int64_t b, int64_t t, int32_t h, int32_t kvh, int32_t d, int64_t table_pages, int cus);
 size_t kv_attn16_workspace(int64_t b, int64_t t, int32_t h, int32_t d, int nsplit);

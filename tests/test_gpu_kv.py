@@ -174,6 +174,52 @@ def test_hidden_junk(cuda, junk, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("h,kvh,d,b,t", [(8, 1, 256, 6, 110), (8, 2, 128, 12, 97), (3, 1, 64, 70, 70), (40, 2, 64, 5, 83)])
+def test_many_rows(cuda, h, kvh, d, b, t, dtype):
+    """More than one round of 16 rows a workgroup: tiles of tokens across each other, lengths below the queries', padding
+    queries, pages that no entry names, hidden junk."""
+    gen = _gen(b + t)
+    cache, table = _pool(gen, b, 5, kvh, d, dtype)
+    table[1, 1], table[2, 0] = -1, cache[0].size(0)
+    q = torch.randn((b, t, h, d), device="cuda", generator=gen).to(dtype)
+    lens = torch.randint(1, 5 * PAGE + 1, (b,), device="cuda", generator=gen).tolist()
+    lens[:5] = [300, 130, 190, 64, 33]
+    q_lens = torch.randint(0, t + 1, (b,), device="cuda", generator=gen).tolist()
+    q_lens[:3] = [t, t - 1, 40]
+    dirty = [c.clone() for c in cache]
+    for c in dirty:
+        used = torch.zeros(c.size(0), PAGE, dtype=torch.bool, device="cuda")
+        for i, n in enumerate(lens):
+            for j in range((n + 63) // 64):
+                if 0 <= table[i, j] < c.size(0):
+                    used[table[i, j].long(), : min(n - 64 * j, 64)] = True
+        c.transpose(1, 2)[~used] = float("nan")
+    for causal in (True, False):
+        _check(q, dirty, table, lens, 0.07, causal, clean=cache)
+        _check(q, dirty, table, lens, 0.07, causal, q_lens, clean=cache)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_nonfinite_values_of_many_rows(cuda, dtype):
+    gen = _gen(15)
+    for h, kvh, d in ((8, 1, 256), (8, 2, 128), (3, 1, 64)):
+        b, t = 1200 * 16 // (100 * h // kvh) // kvh, 100
+        cache, table = _pool(gen, b, 4, kvh, d, dtype)
+        q = torch.randn((b, t, h, d), device="cuda", generator=gen).to(dtype)
+        lens = _i32([200] * b)
+        want = w4a4.kv_attention(q, *cache, table, lens, 0.06)
+        for bad in (float("nan"), float("inf")):
+            dirty = cache[1].clone()
+            # keys 110 and 180 are seen by queries 10 and later, 80 and later (100 + i >= key)
+            dirty[table[0, 1].long(), 0, 110 - 64, 5] = bad
+            dirty[table[0, 2].long(), 0, 180 - 128, d - 1] = bad
+            got = w4a4.kv_attention(q, cache[0], dirty, table, lens, 0.06)
+            hit = torch.zeros_like(got, dtype=torch.bool)
+            hit[0, 10:, : h // kvh, 5] = hit[0, 80:, : h // kvh, d - 1] = True
+            assert not torch.isfinite(got[hit]).any() and torch.equal(got[~hit], want[~hit])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_nonfinite_values_reach_only_who_sees_them(cuda, dtype):
     gen = _gen(14)
     for h, kvh, d in ((8, 1, 256), (4, 2, 128), (2, 2, 64)):
