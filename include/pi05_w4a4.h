@@ -533,7 +533,7 @@ int pi05w4a4_int8_kv_attention(const void* q, const int64_t* q_strides, int32_t 
  * pi05w4a4_kv_append: writes tokens lens[b] .. lens[b] + counts[b] - 1 (counts null: all t) of every
  *   sequence; k, v [B, T, KVH, D] with strides as above.  Nothing else of the cache changes.  Tokens past
  *   table_pages * 64 are dropped.  lens is read only.  A row of a page may be written from one place of the
- *   table only.
+ *   table only.  k and v must not lie in the cache, nor k_cache and v_cache overlap.
  * pi05w4a4_qk_norm_rope_append: both in one launch: q_out, and the rotated keys and the values as they
  *   are into the cache (D as the cache takes it).  All T tokens of q are done.
  * pi05w4a4_kv_attention: out [B, T, H, D] = softmax(scaling q K^T) V over the tokens that query i of sequence b
@@ -543,7 +543,7 @@ int pi05w4a4_int8_kv_attention(const void* q, const int64_t* q_strides, int32_t 
  *   and infinities too; a NaN or infinity among the values that it sees makes its outputs in that
  *   dimension NaN or infinite.  lse, when not null, fp32 [B, T, H]: the natural log of the sum of
  *   exp(scaling q k) (-inf where none is seen).  Query head h reads KV head h / (H / KVH).  Needs
- * *   pi05w4a4_kv_attention_workspace_bytes(...) bytes (0 without a split, at most 2^28).  B * T * H <= 2^30.
+ *   pi05w4a4_kv_attention_workspace_bytes(...) bytes (0 without a split, at most 2^28).  B * T * H <= 2^30.
  *
  * pi05w4a4_lora_add: out[m, n] = y[m, n] + scale[id] * sum_r (sum_k x[m, k] a[id, g r0 + r, k]) b[id, n, r] with
  *   id = ids[m / per_id] and r0 = r, g the slice of column n: slice g has widths[g] columns (widths null: one

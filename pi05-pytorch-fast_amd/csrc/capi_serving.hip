@@ -61,12 +61,34 @@ void set_strides(int64_t* to, const int64_t* from) {
 
 }  // namespace
 
+// Whether `bytes` bytes from a and `more` from b share some.
+static bool ranges_overlap(const void* a, int64_t bytes, const void* b, int64_t more) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return bytes > 0 && more > 0 && x < y + more && y < x + bytes;
+}
+
+// A call that reads rows of the cache while it writes others would depend on the order of its waves.
+static int check_apart(const HeadRopeParams& p) {
+  const int64_t cache = static_cast<int64_t>(p.c.pages) * p.c.kvh * kKvPage * p.d * 2;
+  if (ranges_overlap(p.c.k, cache, p.c.v, cache)) return capi_fail(PI05W4A4_EINVAL, "k_cache and v_cache must not overlap");
+  for (int i = 0; i < 3; ++i) {
+    if (p.x[i] == nullptr) continue;
+    const int64_t* const st = p.stride[i];
+    const int64_t bytes = 2 * ((p.b - 1) * st[0] + (p.t - 1) * st[1] + (p.heads[i] - 1) * st[2] + p.d);
+    if (ranges_overlap(p.x[i], bytes, p.c.k, cache) || ranges_overlap(p.x[i], bytes, p.c.v, cache))
+      return capi_fail(PI05W4A4_EINVAL, "the new tokens must not lie in the cache");
+  }
+  return PI05W4A4_OK;
+}
+
 static int run_head_rope(HeadRopeParams& p, int32_t elem, void* stream, const char* what) {
   p.parts = head_rope_parts(p, device_cu_count());
   // A launch holds fewer than 2^32 threads: a wave for each part of a token.
   if (static_cast<int64_t>(p.b) * p.t * p.parts >= (1 << 26))
     return capi_fail(PI05W4A4_EINVAL, "%d x %d tokens of %d heads are more than one launch holds", p.b, p.t,
                      p.heads[0] + p.heads[1] + p.heads[2]);
+  if (p.c.lens != nullptr)
+    if (int rc = check_apart(p)) return rc;
   return capi_hip(launch_head_rope(p, elem, static_cast<hipStream_t>(stream)), what);
 }
 

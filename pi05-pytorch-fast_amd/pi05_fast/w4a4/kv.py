@@ -237,7 +237,8 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
     cached tokens, the first ``counts`` [B] of them (None: all T); the rest of a padded batch is
     not written.  Changes those rows of the cache and nothing else, and leaves ``lens`` as it is.
     Tokens past the table, or whose table entry names no page, are dropped.  Full pages can be
-    shared between sequences; a row may be written from one place of a call only."""
+    shared between sequences; a row may be written from one place of a call only.  k and v must not lie
+    in the cache."""
     if _direct(k, v, k_cache, v_cache, block_table, lens, counts):
         return _append_impl(k, v, k_cache, v_cache, block_table, lens, counts)
     return torch.ops.pi05_w4a4.kv_append(k, v, k_cache, v_cache, block_table, lens, counts)

@@ -509,6 +509,10 @@ def test_refusals(cuda):
     with pytest.raises(RuntimeError, match="multiple of the KV heads"):
         w4a4.kv_attention(torch.zeros((2, 1, 3, 64), dtype=torch.float16, device="cuda"), *w4a4.kv_cache(4, 2, 64, torch.float16, "cuda"),
                           table, lens, 0.1)
+    with pytest.raises(RuntimeError, match="must not lie in the cache"):
+        append(v=cache[0][:2, :, :1])
+    with pytest.raises(RuntimeError, match="must not overlap"):
+        append(cache=[cache[0], cache[0]])
     append(k=k[:, :0], v=k[:, :0])
     assert attend(q=q[:, :0]).shape == (2, 0, 2, 64)
     far = 1 << 32

@@ -161,6 +161,21 @@ def test_attention_refusals(lib, kw, text):
     assert _attend(lib, q=None, t=0) == 0 and _attend(lib, q=None, b=0) == 0
 
 
+def test_new_tokens_are_apart_from_the_cache(lib):
+    side = 2 * 64 * 64 * 2  # bytes of 2 pages of one head
+
+    def append(k, v, kc, vc, pages=2, ks=I3(64, 64, 64), b=1, t=4):
+        return lib.pi05w4a4_kv_append(vp(k), ks, vp(v), I3(64, 64, 64), 0, b, t, 1, 64, vp(kc), vp(vc), pages, P, 1, 1, P, None, None)
+
+    at = 1 << 20
+    for args in ((at, 1 << 16, at, 1 << 24), (at - 16, 1 << 16, at, 1 << 24), (1 << 16, at + side - 16, 1 << 24, at),
+                 (1 << 16, at, at, 1 << 24)):
+        assert append(*args) == 1 and "must not lie in the cache" in _err(lib)
+    assert append(at - 4096, 1 << 16, at, 1 << 24, ks=I3(0, 1024, 64), t=4) == 1 and "must not lie in the cache" in _err(lib)
+    for kc, vc in ((at, at), (at, at + side - 16), (at + 16, at)):
+        assert append(1 << 10, 1 << 11, kc, vc) == 1 and "must not overlap" in _err(lib)
+
+
 def test_launches_of_too_many_waves(lib):
     big = dict(b=4096, t=4096, kvh=32767)
     assert _append(lib, **big) == 1 and "one launch" in _err(lib)
