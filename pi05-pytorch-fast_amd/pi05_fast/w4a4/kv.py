@@ -19,10 +19,18 @@ from pi05_fast.w4a4 import extension as _ext
 from pi05_fast.w4a4.extension import (_check, _direct, _on_device, _ptr, _refuse_tangents, _stream, _workspace,
                                       load_int4_gemm)
 from pi05_fast.w4a4.int8 import ELEM
-from pi05_fast.w4a4.kv_int8 import HEAD_DIMS, MAX_BATCH, MAX_TOKENS, PAGE_TOKENS, _ints, _table
+from pi05_fast.w4a4.kv_int8 import HEAD_DIMS, MAX_BATCH, MAX_TOKENS, PAGE_TOKENS, _ints
 from pi05_fast.w4a4.rope import _check_rope, _heads, _meta, _plan, _strides, _weight
 
 MAX_KV_HEADS = 32767
+
+
+def _table_plan(table: torch.Tensor) -> tuple[int, int | None]:
+    """Columns and row stride of a block table for the library (None: to be copied)."""
+    rows, cols = table.shape
+    if cols > 1 and table.stride(1) != 1:
+        return cols, None
+    return cols, table.stride(0) if rows > 1 else cols
 
 
 def kv_cache(pages: int, kv_heads: int, head_dim: int, dtype: torch.dtype, device) -> tuple[torch.Tensor, torch.Tensor]:
@@ -73,7 +81,7 @@ def _check_append(what, k, v, k_cache, v_cache, table, lens, counts):
     _ints(what, "counts", counts, b, k.device)
     if b * t > MAX_TOKENS:  # here: the library takes them as 32 bits
         raise RuntimeError(f"{what}: at most {MAX_TOKENS} tokens a call, got {b} x {t}")
-    return (elem, b, t, kvh, d), pages, _strides(k), _strides(v)
+    return (elem, b, t, kvh, d), pages, _strides(k), _strides(v), *_table_plan(table)
 
 
 def _cache_pointers(what, k_cache, v_cache):
@@ -85,21 +93,25 @@ def _cache_pointers(what, k_cache, v_cache):
 
 def _append_impl(k, v, k_cache, v_cache, block_table, lens, counts):
     what = "kv_append"
-    shape, pages, ks, vs = _plan(
-        (what, _meta(k), _meta(v), _meta(k_cache), _meta(v_cache), _meta(block_table), _meta(lens), _meta(counts)),
+    shape, pages, ks, vs, cols, stride = _plan(
+        (what, k.dtype, k.device, k.shape, k.stride(), v.dtype, v.device, v.shape, v.stride(), k_cache.dtype, k_cache.device, k_cache.shape,
+         k_cache.stride(), v_cache.dtype, v_cache.device, v_cache.shape, v_cache.stride(), block_table.dtype, block_table.device,
+         block_table.shape, block_table.stride(), lens.dtype, lens.device, lens.shape, _meta(counts)),
         lambda: _check_append(what, k, v, k_cache, v_cache, block_table, lens, counts))
     kp, vp = _cache_pointers(what, k_cache, v_cache)
     if shape[1] == 0 or shape[2] == 0:
         return
     dev = k.device
-    table, stride = _table(block_table)
+    table = block_table
+    if stride is None:
+        table, stride = table.contiguous(), cols
     lens, counts = lens.contiguous(), None if counts is None else counts.contiguous()
     k, ks = _heads(k, ks)
     v, vs = _heads(v, vs)
     lib = _ext._lib if _ext._lib is not None else load_int4_gemm()
     with _on_device(dev):
         _check(lib.pi05w4a4_kv_append(k.data_ptr(), ks, v.data_ptr(), vs, *shape, kp, vp, pages, table.data_ptr(), stride,
-                                      table.size(1), lens.data_ptr(), _ptr(counts), _stream(dev)), "pi05w4a4_kv_append")
+                                      cols, lens.data_ptr(), _ptr(counts), _stream(dev)), "pi05w4a4_kv_append")
 
 
 def _check_rope_append(what, q, k, v, q_weight, k_weight, positions, inv_freq, k_cache, v_cache, table, lens, counts, axes):
@@ -109,22 +121,27 @@ def _check_rope_append(what, q, k, v, q_weight, k_weight, positions, inv_freq, k
     _, b, t, _, kvh, d = found[0]
     pages = _check_cache(what, q, k_cache, v_cache, table, lens, b, t, kvh, d)
     _ints(what, "counts", counts, b, q.device)
-    return *found, pages, _strides(v)
+    return *found, pages, _strides(v), *_table_plan(table)
 
 
 def _rope_append_impl(q, k, v, q_weight, k_weight, eps, positions, inv_freq, k_cache, v_cache, block_table, lens, counts,
                       unit_offset, interleaved, axes):
     what = "qk_norm_rope_append"
     axes = None if axes is None else tuple(axes)
-    shape, qs, ks, ps, count, amap, pages, vs = _plan(
-        (what, _meta(q), _meta(k), _meta(v), _meta(q_weight), _meta(k_weight), _meta(positions), _meta(inv_freq), _meta(k_cache),
-         _meta(v_cache), _meta(block_table), _meta(lens), _meta(counts), axes),
+    shape, qs, ks, ps, pos_bytes, count, amap, rot, pages, vs, cols, stride = _plan(
+        (what, axes, q.dtype, q.device, q.shape, q.stride(), k.dtype, k.device, k.shape, k.stride(), v.dtype, v.device, v.shape, v.stride(),
+         _meta(q_weight), _meta(k_weight), positions.dtype, positions.device, positions.shape, positions.stride(), inv_freq.dtype,
+         inv_freq.device, inv_freq.shape, k_cache.dtype, k_cache.device, k_cache.shape, k_cache.stride(), v_cache.dtype, v_cache.device,
+         v_cache.shape, v_cache.stride(), block_table.dtype, block_table.device, block_table.shape, block_table.stride(), lens.dtype,
+         lens.device, lens.shape, _meta(counts)),
         lambda: _check_rope_append(what, q, k, v, q_weight, k_weight, positions, inv_freq, k_cache, v_cache, block_table, lens,
                                    counts, axes))
     kp, vp = _cache_pointers(what, k_cache, v_cache)
     dev = q.device
     q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    table, stride = _table(block_table)
+    table = block_table
+    if stride is None:
+        table, stride = table.contiguous(), cols
     lens, counts = lens.contiguous(), None if counts is None else counts.contiguous()
     q, qs = _heads(q, qs)
     k, ks = _heads(k, ks)
@@ -133,10 +150,9 @@ def _rope_append_impl(q, k, v, q_weight, k_weight, eps, positions, inv_freq, k_c
     lib = _ext._lib if _ext._lib is not None else load_int4_gemm()
     with _on_device(dev):
         _check(lib.pi05w4a4_qk_norm_rope_append(q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, *shape, _ptr(q_weight),
-                                                _ptr(k_weight), eps, unit_offset, positions.data_ptr(), ps,
-                                                positions.element_size(), count, amap, inv_freq.data_ptr(), 2 * inv_freq.numel(),
-                                                interleaved, q_out.data_ptr(), kp, vp, pages, table.data_ptr(), stride,
-                                                table.size(1), lens.data_ptr(), _ptr(counts), _stream(dev)),
+                                                _ptr(k_weight), eps, unit_offset, positions.data_ptr(), ps, pos_bytes, count, amap,
+                                                inv_freq.data_ptr(), rot, interleaved, q_out.data_ptr(), kp, vp, pages,
+                                                table.data_ptr(), stride, cols, lens.data_ptr(), _ptr(counts), _stream(dev)),
                "pi05w4a4_qk_norm_rope_append")
     return q_out
 
@@ -160,13 +176,15 @@ def _check_attention(what, q, k_cache, v_cache, table, lens, q_lens):
     _ints(what, "q_lens", q_lens, b, q.device)
     with _on_device(q.device):
         need = int(load_int4_gemm().pi05w4a4_kv_attention_workspace_bytes(b, t, h, kvh, d, table.size(1)))
-    return (elem, b, t, h, kvh, d), pages, _strides(q), need
+    return (elem, b, t, h, kvh, d), pages, _strides(q), need, *_table_plan(table)
 
 
 def _attention_impl(q, k_cache, v_cache, block_table, lens, scaling, causal, q_lens, return_lse):
     what = "kv_attention"
-    shape, pages, qs, need = _plan(
-        (what, _meta(q), _meta(k_cache), _meta(v_cache), _meta(block_table), _meta(lens), _meta(q_lens)),
+    shape, pages, qs, need, cols, stride = _plan(
+        (what, q.dtype, q.device, q.shape, q.stride(), k_cache.dtype, k_cache.device, k_cache.shape, k_cache.stride(), v_cache.dtype,
+         v_cache.device, v_cache.shape, v_cache.stride(), block_table.dtype, block_table.device, block_table.shape, block_table.stride(),
+         lens.dtype, lens.device, lens.shape, _meta(q_lens)),
         lambda: _check_attention(what, q, k_cache, v_cache, block_table, lens, q_lens))
     kp, vp = _cache_pointers(what, k_cache, v_cache)
     dev = q.device
@@ -174,13 +192,15 @@ def _attention_impl(q, k_cache, v_cache, block_table, lens, scaling, causal, q_l
     lse = torch.empty(q.shape[:3], dtype=torch.float32, device=dev) if return_lse else None
     if shape[1] == 0 or shape[2] == 0:
         return out, lse
-    table, stride = _table(block_table)
+    table = block_table
+    if stride is None:
+        table, stride = table.contiguous(), cols
     lens, q_lens = lens.contiguous(), None if q_lens is None else q_lens.contiguous()
     q, qs = _heads(q, qs)
     lib = _ext._lib if _ext._lib is not None else load_int4_gemm()
     with _on_device(dev):
         ws = _workspace(dev, need) if need else None
-        _check(lib.pi05w4a4_kv_attention(q.data_ptr(), qs, *shape, kp, vp, pages, table.data_ptr(), stride, table.size(1),
+        _check(lib.pi05w4a4_kv_attention(q.data_ptr(), qs, *shape, kp, vp, pages, table.data_ptr(), stride, cols,
                                          lens.data_ptr(), _ptr(q_lens), scaling, causal, out.data_ptr(), _ptr(lse), _ptr(ws), need,
                                          _stream(dev)), "pi05w4a4_kv_attention")
     return out, lse

@@ -105,7 +105,8 @@ def _lora_impl(y, x, a, b, ids, scale, slices, in_place):
     what = "lora_add_" if in_place else "lora_add"
     slices = None if slices is None else tuple(slices)
     (m, k, n, r, adapters, per_id), ldy, ldx, widths, elem, need = _plan(
-        (what, _meta(y), _meta(x), _meta(a), _meta(b), _meta(ids), _meta(scale), slices),
+        (what, slices, y.dtype, y.device, y.shape, y.stride(), x.dtype, x.device, x.shape, x.stride(), a.dtype, a.device, a.shape, b.dtype,
+         b.device, b.shape, ids.dtype, ids.device, ids.shape, _meta(scale)),
         lambda: _check_lora(what, y, x, a, b, ids, scale, slices, in_place))
     dev = y.device
     if in_place:

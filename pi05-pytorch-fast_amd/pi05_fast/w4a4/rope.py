@@ -24,7 +24,7 @@ MAX_HEADS = 32767
 MAX_TOKENS = 1 << 24  # tokens of a call
 
 # What the checks of a call find depends on its tensors' types, devices, shapes and strides only: the arguments of
-# calls that passed them, by these.
+# calls that passed them, by these (one flat tuple, written out at each call: half the time of a tuple of tuples).
 _PLANS: dict[tuple, tuple] = {}
 
 
@@ -76,7 +76,7 @@ def _weight(w: torch.Tensor | None) -> torch.Tensor | None:
 
 def _check_rope(what, q, k, q_weight, k_weight, positions, inv_freq, axes):
     """The checks shared by the forms of the call, and what they find: (elem, b, t, h, kvh, d), the strides of q, k and the
-    positions, the number of axes and their map."""
+    positions and their bytes, the number of axes and their map, the rotated dimensions."""
     if not q.is_cuda:
         raise RuntimeError(f"{what} expects CUDA/HIP tensors")
     dev = q.device
@@ -107,7 +107,8 @@ def _check_rope(what, q, k, q_weight, k_weight, positions, inv_freq, axes):
     count = positions.size(0) if positions.dim() == 3 else 1
     amap = _axis_map(what, axes, pairs, count)
     ps = positions.stride() if positions.dim() == 3 else (0, *positions.stride())
-    return (elem, b, t, h, kvh, d), _strides(q), _strides(k), (ctypes.c_int64 * 3)(*ps), count, amap
+    return ((elem, b, t, h, kvh, d), _strides(q), _strides(k), (ctypes.c_int64 * 3)(*ps), positions.element_size(), count, amap,
+            2 * pairs)
 
 
 def _plan(key: tuple, make) -> tuple:
@@ -123,8 +124,9 @@ def _plan(key: tuple, make) -> tuple:
 def _rope_impl(q, k, q_weight, k_weight, eps, positions, inv_freq, unit_offset, interleaved, axes):
     what = "qk_norm_rope"
     axes = None if axes is None else tuple(axes)
-    shape, qs, ks, ps, count, amap = _plan(
-        (what, _meta(q), _meta(k), _meta(q_weight), _meta(k_weight), _meta(positions), _meta(inv_freq), axes),
+    shape, qs, ks, ps, pos_bytes, count, amap, rot = _plan(
+        (what, axes, q.dtype, q.device, q.shape, q.stride(), k.dtype, k.device, k.shape, k.stride(), _meta(q_weight), _meta(k_weight),
+         positions.dtype, positions.device, positions.shape, positions.stride(), inv_freq.dtype, inv_freq.device, inv_freq.shape),
         lambda: _check_rope(what, q, k, q_weight, k_weight, positions, inv_freq, axes))
     dev = q.device
     q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
@@ -135,9 +137,8 @@ def _rope_impl(q, k, q_weight, k_weight, eps, positions, inv_freq, unit_offset, 
     lib = _ext._lib if _ext._lib is not None else load_int4_gemm()
     with _on_device(dev):
         _check(lib.pi05w4a4_qk_norm_rope(q.data_ptr(), qs, k.data_ptr(), ks, *shape, _ptr(q_weight), _ptr(k_weight), eps,
-                                         unit_offset, positions.data_ptr(), ps, positions.element_size(), count, amap,
-                                         inv_freq.data_ptr(), 2 * inv_freq.numel(), interleaved, q_out.data_ptr(),
-                                         k_out.data_ptr(), _stream(dev)), "pi05w4a4_qk_norm_rope")
+                                         unit_offset, positions.data_ptr(), ps, pos_bytes, count, amap, inv_freq.data_ptr(), rot,
+                                         interleaved, q_out.data_ptr(), k_out.data_ptr(), _stream(dev)), "pi05w4a4_qk_norm_rope")
     return q_out, k_out
 
 
