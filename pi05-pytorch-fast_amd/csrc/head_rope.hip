@@ -12,8 +12,8 @@
 // D / 16 lanes hold a head, 16 elements each: of a rotated pair both halves, so that nothing crosses
 // lanes but the sum of squares.  A wave takes a token (or a part of its heads), each lane computes the sine and
 // cosine of every 64th pair, and the heads share them through LDS.
-// Bound by HBM where tokens are many: 4 x 1536 tokens of 32 + 8 heads of 128, 126 MB, 26.6 us, 4.7 TB/s, where the
-// bytes alone take 23.6 in this form; a single token by its loads' latency one behind the other, 4 us.
+// Bound by HBM where tokens are many: 4 x 1536 tokens of 32 + 8 heads of 128, 126 MB, 25.9 us, 4.9 TB/s, where the
+// bytes alone take 23.6 in this form (fewer registers for a third more waves, or weights loaded a head: no faster); a single token by its loads' latency one behind the other, 4 us.
 
 #include "quant_row.h"
 #include "serving_internal.h"

@@ -264,11 +264,11 @@ __device__ __forceinline__ void store_rows(const LoraParams& p, int64_t first, i
 }
 
 // A wave takes 16 rows and kCols columns of a slice, h and y (and the ids, on which only B waits) under way at
-// once; nothing is kept for a second row tile, as more waves hide more (B kept over the row tiles of a wave, with the
-// next tile under way: 191 us for 6208 x 32768 in place of 199, 51 for 2560 columns in place of 47).  Column j of tile
-// i is column NT j + i of the block: a lane ends with NT (eight, or four for large ranks) consecutive columns of four
+// once; nothing is kept for a second row tile: more waves hide as much, with less code (B kept over a wave's row tiles and
+// the next tile under way, in a form whose stores went through the L2: 191 us for 6208 x 32768 in place of 199, but 51
+// for 2560 columns in place of 47).  Column j of tile i is column NT j + i of the block: a lane ends with NT (eight, or four for large ranks) consecutive columns of four
 // rows, and 16 lanes read and write 256 or 128 consecutive bytes of a row.  Bound by y and out in HBM where rows are
-// many: 6208 x 32768 with rank 32, both launches 167 us, 5.1 TB/s.
+// many: 6208 x 32768 with rank 32, both launches 165 us, 5.1 TB/s.
 template <int KS>
 constexpr int kCols = KS <= 2 ? 128 : 64;
 

@@ -285,7 +285,7 @@ def kv_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
                  scaling: float, causal: bool = True, q_lens: torch.Tensor | None = None, return_lse: bool = False):
     """softmax(scaling q K^T) V of q [B, T, H, D] (the cache's type, rotated, any strides) over the
     cache: [B, T, H, D].  H is a multiple of KVH; query head h reads KV head h // (H / KVH).  Made for
-    decoded tokens, T = 1 or a few: every 16 rows of T * (H / KVH) read the cache once.  The work is planned
+    decoded tokens, T = 1 or a few: every 16 rows of T * (H / KVH), 64 where rows are many, read the cache once.  The work is planned
     for the table's width: pass a table held at capacity as ``block_table[:, :n]``, n the pages of
     the longest sequence.  Entries that name no page hide their 64 tokens.
 
