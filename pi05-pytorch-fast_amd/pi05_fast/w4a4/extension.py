@@ -1482,6 +1482,13 @@ def _refuse_tangents(*ts) -> None:
             raise RuntimeError("the pi05_w4a4 operators have no forward-mode derivatives, and an argument carries a tangent")
 
 
+def _refuse_gradients(what: str, *ts) -> None:
+    """For calls that write into an argument, which no backward pass would notice: refused rather than dropped."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
+        raise RuntimeError(f"{what} writes in place and has no derivatives, and an argument requires gradients: call it under "
+                           "torch.no_grad()")
+
+
 def _direct(*ts) -> bool:
     if _is_compiling() or _jit_tracing() is not None or _dispatch_modes() or _function_modes():
         return False

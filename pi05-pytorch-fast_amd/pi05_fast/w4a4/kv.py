@@ -16,8 +16,8 @@ from collections.abc import Sequence
 import torch
 
 from pi05_fast.w4a4 import extension as _ext
-from pi05_fast.w4a4.extension import (_check, _direct, _on_device, _ptr, _refuse_tangents, _stream, _workspace,
-                                      load_int4_gemm)
+from pi05_fast.w4a4.extension import (_check, _direct, _on_device, _ptr, _refuse_gradients, _refuse_tangents, _stream,
+                                      _workspace, load_int4_gemm)
 from pi05_fast.w4a4.int8 import ELEM
 from pi05_fast.w4a4.kv_int8 import HEAD_DIMS, MAX_BATCH, MAX_TOKENS, PAGE_TOKENS, _ints
 from pi05_fast.w4a4.rope import _check_rope, _heads, _meta, _plan, _strides, _weight
@@ -258,9 +258,10 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
     not written.  Changes those rows of the cache and nothing else, and leaves ``lens`` as it is.
     Tokens past the table, or whose table entry names no page, are dropped.  Full pages can be
     shared between sequences; a row may be written from one place of a call only.  k and v must not lie
-    in the cache."""
+    in the cache.  There are no derivatives: arguments that require gradients are refused."""
     if _direct(k, v, k_cache, v_cache, block_table, lens, counts):
         return _append_impl(k, v, k_cache, v_cache, block_table, lens, counts)
+    _refuse_gradients("kv_append", k, v, k_cache, v_cache)
     return torch.ops.pi05_w4a4.kv_append(k, v, k_cache, v_cache, block_table, lens, counts)
 
 
@@ -272,10 +273,12 @@ def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_wei
     """``qk_norm_rope`` of q and k and ``kv_append`` of the rotated keys and of v in one launch: returns
     the queries [B, T, H, D].  ``positions`` are the tokens' own (with several axes they are not the
     places in the cache, which follow from ``lens``).  All T tokens' queries are computed; keys and
-    values go into the cache up to ``counts``."""
+    values go into the cache up to ``counts``.  There are no derivatives: arguments that require
+    gradients are refused."""
     if _direct(q, k, v, q_weight, k_weight, positions, inv_freq, k_cache, v_cache, block_table, lens, counts):
         return _rope_append_impl(q, k, v, q_weight, k_weight, float(eps), positions, inv_freq, k_cache, v_cache, block_table, lens,
                                  counts, bool(unit_offset), bool(interleaved), axes)
+    _refuse_gradients("qk_norm_rope_append", q, k, v, q_weight, k_weight, inv_freq, k_cache, v_cache)
     return torch.ops.pi05_w4a4.qk_norm_rope_append(q, k, v, q_weight, k_weight, float(eps), positions, inv_freq, k_cache, v_cache,
                                                    block_table, lens, counts, bool(unit_offset), bool(interleaved),
                                                    None if axes is None else list(axes))

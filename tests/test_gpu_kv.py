@@ -523,6 +523,24 @@ def test_refusals(cuda):
         attend(table=table[:, :1].expand(2, far + 1))
 
 
+@pytest.mark.filterwarnings("ignore:There is a performance drop")
+def test_vmap(cuda):
+    """One call a sample, the same results; what writes in place is refused there."""
+    gen = _gen(26)
+    cache, table = _pool(gen, 3, 2, 1, 64, torch.float16)
+    q, k = (torch.randn((3, 2, n, 64), device="cuda", generator=gen).half() for n in (4, 1))
+    pos, freq, lens = torch.arange(6, device="cuda").view(3, 2), torch.rand(32, device="cuda", generator=gen), _i32([70, 128, 3])
+    got = torch.vmap(lambda q, k, p: w4a4.qk_norm_rope(q[None], k[None], k[0, 0], None, 1e-6, p[None], freq))(q, k, pos)
+    for i in range(3):
+        want = w4a4.qk_norm_rope(q[i:i + 1], k[i:i + 1], k[i, 0, 0], None, 1e-6, pos[i:i + 1], freq)
+        assert all(torch.equal(a[i], b) for a, b in zip(got, want))
+    got = torch.vmap(lambda q, t, n: w4a4.kv_attention(q[None], *cache, t[None], n[None], 0.1, return_lse=True))(q, table, lens)
+    want = w4a4.kv_attention(q, *cache, table, lens, 0.1, return_lse=True)
+    assert all(torch.equal(a[:, 0], b) for a, b in zip(got, want))
+    with pytest.raises(RuntimeError):
+        torch.vmap(lambda k, t, n: w4a4.kv_append(k[None], k[None], *cache, t[None], n[None]))(k, table, lens)
+
+
 def test_dispatched_route(cuda):
     gen = _gen(25)
     cache, table = _pool(gen, 2, 3, 1, 64, torch.float16)

@@ -247,6 +247,15 @@ def test_refusals(cuda):
         call(x=leaf).sum().backward()
 
 
+@pytest.mark.filterwarnings("ignore:There is a performance drop")
+def test_vmap(cuda):
+    y, x, a, b, scale = _whole(_gen(9), 6, 64, 48, 8, 2, 1, torch.float16)
+    y, x, ids = y.view(3, 2, 48), x.view(3, 2, 64), _ids([0, 1, -1])
+    assert torch.equal(torch.vmap(lambda y, x, i: w4a4.lora_add(y, x, a, b, i, scale))(y, x, ids), w4a4.lora_add(y, x, a, b, ids, scale))
+    with pytest.raises(RuntimeError):
+        torch.vmap(lambda y, x, i: w4a4.lora_add_(y, x, a, b, i, scale))(y, x, ids)
+
+
 def test_dispatched_route(cuda):
     y, x, a, b, scale = _whole(_gen(8), 5, 64, 48, 8, 2, 2, torch.float16)
     ids = _ids([0, 1, -1, 0, 1])

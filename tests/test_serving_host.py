@@ -80,6 +80,15 @@ def test_cpu_tensors_and_tangents_are_refused(name):
             call(lambda t: fw.make_dual(t, torch.ones_like(t)))
 
 
+@pytest.mark.parametrize("name", ["qk_norm_rope_append", "kv_append", "lora_add_"])
+def test_gradients_through_calls_in_place_are_refused(name):
+    call = _calls()[name]
+    with pytest.raises(RuntimeError, match="requires gradients"):
+        call(lambda t: t.clone().requires_grad_())
+    with torch.no_grad(), pytest.raises(RuntimeError, match="expects CUDA/HIP tensors"):
+        call(lambda t: t.clone().requires_grad_())
+
+
 def test_rope_axes():
     assert w4a4.rope_axes((2, 0, 3)) == (0, 0, 2, 2, 2)
     with pytest.raises(RuntimeError, match="head_dim"):
