@@ -323,6 +323,12 @@ extern "C" int pi05w4a4_lora_add(const void* y, int64_t ldy, const void* x, int6
   if (ldy < 0 || ldo < n) return capi_fail(PI05W4A4_EINVAL, "row strides must be >= 0, and those of the output >= N");
   if (rows_overlap(x, ldx, k, out, ldo, n, m)) return capi_fail(PI05W4A4_EINVAL, "x must not overlap the output");
   const LoraPlan plan = lora_plan(m, per_id, k, n, r, slices, adapters, device_cu_count());
+  p.m = m;
+  p.r = r;
+  p.slices = slices;
+  p.ksplit = plan.ksplit;
+  p.groups = plan.groups;
+  if (!lora_grid(p)) return capi_fail(PI05W4A4_EINVAL, "%lld rows of %d columns are more than one launch holds", (long long)m, n);
   const size_t need = adapters > 0 ? lora_workspace(m, r, slices, plan.ksplit) : 0;
   if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned(workspace, 16)))
     return capi_fail(PI05W4A4_EWORKSPACE, "lora_add needs a 16-byte aligned workspace of %zu bytes, got %zu", need, workspace_bytes);
@@ -334,17 +340,12 @@ extern "C" int pi05w4a4_lora_add(const void* y, int64_t ldy, const void* x, int6
   p.y = y;
   p.out = out;
   p.h = static_cast<float*>(workspace);
-  p.m = m;
   p.per_id = per_id;
   p.ldx = ldx;
   p.ldy = ldy;
   p.ldo = ldo;
   p.k = k;
   p.n = n;
-  p.r = r;
   p.adapters = adapters;
-  p.slices = slices;
-  p.ksplit = plan.ksplit;
-  p.groups = plan.groups;
   return capi_hip(launch_lora(p, elem, static_cast<hipStream_t>(stream)), "lora_add launch");
 }

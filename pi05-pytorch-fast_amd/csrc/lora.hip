@@ -496,24 +496,19 @@ void launch_down(const LoraParams& p, hipStream_t stream) {
 }
 
 template <typename T, int KS>
-void launch_up(LoraParams p, hipStream_t stream) {
-  p.runs = 0;
-  for (int s = 0; s < p.slices; ++s) p.runs += (p.width[s] + 4 * kCols<KS> - 1) / (4 * kCols<KS>);
+void launch_up(const LoraParams& p, hipStream_t stream) {
   const dim3 grid(static_cast<unsigned>((p.m + 15) / 16 * p.groups * p.runs));
   lora_up_kernel<T, KS><<<grid, 256, 0, stream>>>(p);
 }
 
 template <typename T, int NR>
-void launch_fused(LoraParams p, hipStream_t stream) {
-  constexpr int kRun = 8 * kCols<(NR + 1) / 2>;
-  p.runs = 0;
-  for (int s = 0; s < p.slices; ++s) p.runs += (p.width[s] + kRun - 1) / kRun;
+void launch_fused(const LoraParams& p, hipStream_t stream) {
   const dim3 grid(static_cast<unsigned>((p.m + 15) / 16 * p.groups * p.runs));
   lora_fused_kernel<T, NR><<<grid, 512, 0, stream>>>(p);
 }
 
 template <typename T>
-void launch(LoraParams p, hipStream_t stream) {
+void launch(const LoraParams& p, hipStream_t stream) {
   if (p.ksplit == 0) {
     if (p.r <= 16) launch_fused<T, 1>(p, stream);
     else if (p.r <= 32) launch_fused<T, 2>(p, stream);
@@ -521,7 +516,6 @@ void launch(LoraParams p, hipStream_t stream) {
     else launch_fused<T, 8>(p, stream);
     return;
   }
-  p.h_plane = lora_h_floats(p.m, p.r, p.slices);
   if (p.adapters > 0) launch_down<T>(p, stream);
   if (p.r <= 32) launch_up<T, 1>(p, stream);
   else if (p.r <= 64) launch_up<T, 2>(p, stream);
@@ -551,6 +545,15 @@ LoraPlan lora_plan(int64_t m, int64_t per_id, int32_t k, int32_t n, int32_t r, i
   const int64_t down = tiles * plan.groups * ((slices * r + 63) / 64);
   plan.ksplit = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({cus / down, (k + 511) / 512, 8})));
   return plan;
+}
+
+bool lora_grid(LoraParams& p) {
+  const int64_t waves = p.ksplit == 0 ? 8 : 4, columns = waves * (p.r <= 64 ? kCols<1> : kCols<4>);
+  int64_t runs = 0;
+  for (int s = 0; s < p.slices; ++s) runs += (p.width[s] + columns - 1) / columns;
+  p.runs = static_cast<int32_t>(runs);
+  p.h_plane = lora_h_floats(p.m, p.r, p.slices);
+  return (p.m + 15) / 16 * p.groups * runs * waves < (1 << 26);
 }
 
 hipError_t launch_lora(const LoraParams& p, int elem, hipStream_t stream) {

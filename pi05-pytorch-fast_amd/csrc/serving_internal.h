@@ -96,6 +96,8 @@ struct LoraPlan {
 };
 LoraPlan lora_plan(int64_t m, int64_t per_id, int32_t k, int32_t n, int32_t r, int32_t slices, int32_t adapters, int cus);
 int64_t lora_h_floats(int64_t m, int32_t r, int32_t slices);
+// What of a call follows from its plan (runs, h_plane); false: its waves are more than one launch holds.
+bool lora_grid(LoraParams& p);
 hipError_t launch_lora(const LoraParams& p, int elem, hipStream_t stream);
 
 }  // namespace w4a4

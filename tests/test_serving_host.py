@@ -185,6 +185,13 @@ def test_new_tokens_are_apart_from_the_cache(lib):
         assert append(1 << 10, 1 << 11, kc, vc) == 1 and "must not overlap" in _err(lib)
 
 
+def test_adapters_of_too_many_rows(lib):
+    far = vp(1 << 45)
+    assert _lora(lib, x=far, m=1 << 26, per=1 << 26, n=1 << 12, ldy=1 << 12, ldo=1 << 12, ws=None, wsb=0) == 1
+    assert "one launch" in _err(lib)
+    assert _lora(lib, x=far, m=1 << 26, per=1 << 26, n=1 << 9, ldy=1 << 9, ldo=1 << 9, ws=None, wsb=0) == 3  # the workspace
+
+
 def test_launches_of_too_many_waves(lib):
     big = dict(b=4096, t=4096, kvh=32767)
     assert _append(lib, **big) == 1 and "one launch" in _err(lib)
