@@ -551,8 +551,9 @@ int pi05w4a4_int8_kv_attention(const void* q, const int64_t* q_strides, int32_t 
  *   contiguous; scale [adapters], null for 1.  ids outside [0, adapters) name no adapter: out = y.  x has row
  *   stride ldx (% 8 == 0, 16-byte aligned), K % 8 == 0, K <= 2^20; y and out have row strides of any size and may
  *   be the same matrix, but must not overlap otherwise, nor x and out.
- *   r % 8 == 0, r <= 128; smaller ranks are padded with zeros.  fp32 with one rounding.  M <= 2^26, N <= 2^22, and
- *   M * N / 2048 (M * N / 1024 past rank 64) < 2^26.  Where x A^T is infinite, outputs may be NaN.
+ *   r % 8 == 0, r <= 128; smaller ranks are padded with zeros.  fp32 with one rounding.  M <= 2^26, N <= 2^22, and no
+ *   more waves than a launch holds (2^26; one is 16 rows of an adapter by 128 columns, 64 past rank 64).  Where x A^T is
+ *   infinite, outputs may be NaN.
  *   Needs pi05w4a4_lora_workspace_bytes(...) bytes.
  */
 int pi05w4a4_qk_norm_rope(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, int32_t elem,

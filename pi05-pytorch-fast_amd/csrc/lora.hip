@@ -11,10 +11,9 @@
 // parts whose products with B are summed (fp16: after a shift that brings a row's largest into the upper
 // range, so that no h overflows), so that nothing of h is lost beside the rounding of out.
 //
-// Rows need no order.  The adapters that occur in a tile of 16 rows are taken one by one: each is applied to the
-// whole tile and kept for its own rows, and the workgroups of a tile share them out.  A tile of one request
-// has one; 16 decoded tokens of 16 adapters have 16, whose weights have to be read anyway.  Rows without an
-// adapter keep y.
+// Rows need no order.  A tile is up to 16 rows of one adapter: 16 consecutive ones of a request of 64 or more, else those
+// of an adapter among 64 consecutive rows, which each workgroup finds by itself (191 rows of 14 adapters, 2048 x 3509: 9.6 us;
+// 17.2 with tiles of 16 consecutive rows, taken once for each of their adapters).  Rows without an adapter keep y.
 //
 // Operands are loaded with four neighbouring lanes on 64 consecutive bytes of a row and then handed to the
 // lanes that the matrix instruction wants them in: as it has them, 16 neighbouring lanes are 16 bytes of as many rows,
@@ -49,36 +48,82 @@ __device__ __forceinline__ vec8<T> to_operand(const vec8<T> v) {
   return __builtin_bit_cast(vec8<T>, x);
 }
 
-// h between the launches: blocks of 16 rows x 32 ranks of a slice, [K slice, row tile, slice, ranks / 32], as the lanes
-// of the second launch take them: lane 16 g + row has ranks 8 g .. + 7.
-__device__ __forceinline__ int64_t lora_h_index(const LoraParams& p, int64_t tile, int slice, int s) {
-  return ((tile * p.slices + slice) * ((p.r + 31) / 32) + s) * 512;
+// h between the launches: blocks of 16 rows x 32 ranks of a slice, [K slice, rows / 16, slice, ranks / 32]; a block has
+// ranks 8 g .. + 7 of its row i at 128 g + 8 i, as the lanes of the second launch take them.  Of a row and its block 0:
+__device__ __forceinline__ int64_t lora_h_row(const LoraParams& p, int row, int slice) {
+  return (static_cast<int64_t>(row >> 4) * p.slices + slice) * ((p.r + 31) / 32) * 512 + (row & 15) * 8;
 }
 
-__device__ __forceinline__ int lora_raw_id(const LoraParams& p, int64_t row) {
-  return p.ids[static_cast<uint32_t>(row) / static_cast<uint32_t>(p.per_id)];  // M and per_id <= 2^26
-}
-// -1: no adapter, -2: behind the last row.
-__device__ __forceinline__ int lora_id(const LoraParams& p, int raw, int64_t row) {
-  return row >= p.m ? -2 : raw < 0 || raw >= p.adapters ? -1 : raw;
-}
+constexpr int kWindow = 64;
 
-// Calls f(id) for every which-th of a tile's adapters, in the order of their first rows (-1 among them when `none`).
-// `id` is that of the tile's row lane % 16.  Uniform over the workgroup.
-template <typename F>
-__device__ __forceinline__ void each_adapter(int id, bool none, int which, int groups, F f) {
-  uint32_t left = static_cast<uint32_t>(__ballot(id >= (none ? -1 : 0))) & 0xffffu;
-  for (int n = 0; left != 0; ++n) {
-    const int now = __builtin_amdgcn_readlane(id, __builtin_ctz(left));
-    left &= ~static_cast<uint32_t>(__ballot(id == now));
-    if (n % groups == which) f(now);
+// The rows of a tile and their adapter (-1: none).
+template <bool GATHER>
+struct Tile {
+  int id;      // not GATHER: as it stands in ids, until known()
+  int n;       // rows
+  int row0;    // the first; GATHER: of the window
+  int place;   // GATHER: lane i < 16: row i, from row0
+  // The first use of the id that was loaded: false where the tile has nothing to do.
+  __device__ __forceinline__ bool known(const LoraParams& p, bool none) {
+    if constexpr (!GATHER) id = __builtin_amdgcn_readfirstlane(id < 0 || id >= p.adapters ? -1 : id);
+    return none || id >= 0;
+  }
+  // Row i of the tile, from row0; past the last one the last one again.
+  __device__ __forceinline__ int row(int i) const {
+    const int at = min(i, n - 1);
+    return GATHER ? __shfl(place, at, 64) : at;
+  }
+};
+
+// The which-th tile of unit (16 rows of a request, or a window); false: there is none.  Uniform over the workgroup.  none: rows
+// without an adapter have tiles too.  Rows of a request are known without their id, which nothing waits for here.
+template <bool GATHER>
+__device__ __forceinline__ bool find_tile(const LoraParams& p, int unit, int which, bool none, Tile<GATHER>& t) {
+  const int m = static_cast<int>(p.m), per_id = static_cast<int>(p.per_id);  // at most 2^26
+  if constexpr (!GATHER) {
+    const int request = unit / p.tiles, at = 16 * (unit - request * p.tiles);
+    t.row0 = request * per_id + at;
+    t.n = min(min(per_id - at, m - t.row0), 16);
+    if (t.n <= 0) return false;
+    t.id = p.ids[request];
+    return true;
+  } else {
+    const int lane = threadIdx.x & 63;
+    t.row0 = unit * kWindow;
+    const int raw = p.ids[min(t.row0 + lane, m - 1) / per_id];
+    const int id = t.row0 + lane >= m ? -2 : raw < 0 || raw >= p.adapters ? -1 : raw;
+    const int least = none ? -1 : 0;
+    uint64_t same;
+    int at;  // of the tile among the adapter's
+    if (p.leaders) {  // the one whose first row is row `which`
+      t.id = __builtin_amdgcn_readlane(id, which);
+      same = __ballot(id == t.id);
+      at = __builtin_popcountll(same & ((uint64_t{1} << which) - 1));
+      if (t.id < least || at % 16 != 0) return false;
+      at /= 16;
+    } else {  // counted over the adapters in the order of their first rows
+      uint64_t left = __ballot(id >= least);
+      for (at = which;; at -= (__builtin_popcountll(same) + 15) / 16) {
+        if (left == 0) return false;
+        t.id = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
+        same = __ballot(id == t.id);
+        if (16 * at < __builtin_popcountll(same)) break;
+        left &= ~same;
+      }
+    }
+    t.n = min(__builtin_popcountll(same) - 16 * at, 16);
+    // Each row goes to the lane of its place in the tile; the others' to lane 63, where nobody looks.
+    const int rank = __builtin_popcountll(same & ((uint64_t{1} << lane) - 1)) - 16 * at;
+    const bool mine = id == t.id && rank >= 0 && rank < 16;
+    t.place = __builtin_amdgcn_ds_permute(4 * (mine ? rank : 63), lane);
+    return true;
   }
 }
 
 // Rows 16 NR y .. of A, K slice z; the slice's chunks of 32 elements are dealt to the waves in runs.
-// Bound by the arrival of x and A (A from the L2 for all row tiles but the first): kAhead chunks of both are
+// Bound by the arrival of x and A (A from the L2 for all tiles of an adapter but the first): kAhead chunks of both are
 // under way at once.  6208 x 2048 with 64 rows of A: 17 us.
-template <typename T, int NR>
+template <typename T, int NR, bool GATHER>
 __global__ __launch_bounds__(512) void lora_down_kernel(LoraParams p) {
   constexpr int W = 8, kAhead = 4;
   __shared__ __align__(16) v4f part[W][NR][64];
@@ -86,10 +131,8 @@ __global__ __launch_bounds__(512) void lora_down_kernel(LoraParams p) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, col = lane & 15;
   const int lr = lane >> 2, lc = lane & 3;  // row and chunk that the lane loads
-  const int tile = blockIdx.x / p.groups;
-  const int64_t first = 16LL * tile;
-  const int64_t row = first + col;
-  const int my_id = lora_id(p, lora_raw_id(p, min(row, p.m - 1)), row);
+  Tile<GATHER> tile;
+  if (!find_tile(p, blockIdx.x / p.groups, blockIdx.x % p.groups, false, tile) || !tile.known(p, false)) return;
   const int total = p.slices * p.r;  // rows of an adapter's A
   const int rank0 = blockIdx.y * 16 * NR;
   const int chunks = (p.k + 31) / 32;
@@ -99,62 +142,58 @@ __global__ __launch_bounds__(512) void lora_down_kernel(LoraParams p) {
   const int w0 = min(c0 + wave * per_wave, c1), w1 = min(w0 + per_wave, c1);
   const int whole = min(w1, p.k / 32);  // chunks that K fills
 
-  const T* const xp = static_cast<const T*>(p.x) + min(first + lr, p.m - 1) * p.ldx + 8 * lc;
-  each_adapter(my_id, false, blockIdx.x % p.groups, p.groups, [&](int id) {
-    const T* ap[NR];
+  const T* const xp = static_cast<const T*>(p.x) + tile.row0 * p.ldx + tile.row(lr) * p.ldx + 8 * lc;
+  const T* ap[NR];
 #pragma unroll
-    for (int i = 0; i < NR; ++i)  // rows past the last one: the last one again, not stored
-      ap[i] = static_cast<const T*>(p.a) + (static_cast<int64_t>(id) * total + min(rank0 + 16 * i + lr, total - 1)) * p.k + 8 * lc;
-    v4f acc[NR];
+  for (int i = 0; i < NR; ++i)  // rows past the last one: the last one again, not stored
+    ap[i] = static_cast<const T*>(p.a) + (static_cast<int64_t>(tile.id) * total + min(rank0 + 16 * i + lr, total - 1)) * p.k + 8 * lc;
+  v4f acc[NR];
 #pragma unroll
-    for (int i = 0; i < NR; ++i) acc[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-    auto add = [&](const vec8<T> x, const vec8<T> (&a)[NR]) {
-      const vec8<T> u = to_operand<T>(x);
+  for (int i = 0; i < NR; ++i) acc[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+  auto add = [&](const vec8<T> x, const vec8<T> (&a)[NR]) {
+    const vec8<T> u = to_operand<T>(x);
 #pragma unroll
-      for (int i = 0; i < NR; ++i) acc[i] = mfma(u, to_operand<T>(a[i]), acc[i]);
-    };
-    auto load = [&](vec8<T>& x, vec8<T> (&a)[NR], int k) {
-      x = *reinterpret_cast<const vec8<T>*>(xp + k);
+    for (int i = 0; i < NR; ++i) acc[i] = mfma(u, to_operand<T>(a[i]), acc[i]);
+  };
+  auto load = [&](vec8<T>& x, vec8<T> (&a)[NR], int k) {
+    x = *reinterpret_cast<const vec8<T>*>(xp + k);
 #pragma unroll
-      for (int i = 0; i < NR; ++i) a[i] = *reinterpret_cast<const vec8<T>*>(ap[i] + k);
-    };
-    int c = w0;
-    for (; c + kAhead <= whole; c += kAhead) {
-      vec8<T> x[kAhead], a[kAhead][NR];
+    for (int i = 0; i < NR; ++i) a[i] = *reinterpret_cast<const vec8<T>*>(ap[i] + k);
+  };
+  int c = w0;
+  for (; c + kAhead <= whole; c += kAhead) {
+    vec8<T> x[kAhead], a[kAhead][NR];
 #pragma unroll
-      for (int j = 0; j < kAhead; ++j) load(x[j], a[j], 32 * (c + j));
+    for (int j = 0; j < kAhead; ++j) load(x[j], a[j], 32 * (c + j));
 #pragma unroll
-      for (int j = 0; j < kAhead; ++j) add(x[j], a[j]);
+    for (int j = 0; j < kAhead; ++j) add(x[j], a[j]);
+  }
+  for (; c < w1; ++c) {  // the last ones, and one that K does not fill
+    vec8<T> x, a[NR];
+    const bool in = 32 * c + 8 * lc < p.k;
+    load(x, a, in ? 32 * c : -8 * lc);  // elsewhere the row's first elements
+    if (!in) {
+      x = vec8<T>{};
+#pragma unroll
+      for (int i = 0; i < NR; ++i) a[i] = vec8<T>{};
     }
-    for (; c < w1; ++c) {  // the last ones, and one that K does not fill
-      vec8<T> x, a[NR];
-      const bool in = 32 * c + 8 * lc < p.k;
-      load(x, a, in ? 32 * c : -8 * lc);  // elsewhere the row's first elements
-      if (!in) {
-        x = vec8<T>{};
+    add(x, a);
+  }
 #pragma unroll
-        for (int i = 0; i < NR; ++i) a[i] = vec8<T>{};
-      }
-      add(x, a);
+  for (int i = 0; i < NR; ++i) part[wave][i][lane] = acc[i];
+  __syncthreads();
+  for (int i = wave; i < NR; i += W) {
+    v4f s = part[0][i][lane];
+#pragma unroll
+    for (int w = 1; w < W; ++w) s += part[w][i][lane];
+    const int rank = rank0 + 16 * i + col, slice = rank / p.r, of = rank % p.r;
+    float* const hp = p.h + blockIdx.z * p.h_plane + of / 8 * 128 + of % 8;  // blocks of 32 ranks follow one another
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int row = tile.row0 + tile.row(4 * g + r);
+      if (4 * g + r < tile.n && rank < total) hp[lora_h_row(p, row, slice)] = s[r];
     }
-#pragma unroll
-    for (int i = 0; i < NR; ++i) part[wave][i][lane] = acc[i];
-    __syncthreads();
-    for (int i = wave; i < NR; i += W) {
-      v4f s = part[0][i][lane];
-#pragma unroll
-      for (int w = 1; w < W; ++w) s += part[w][i][lane];
-      const int rank = rank0 + 16 * i + col;
-      float* const hp = p.h + blockIdx.z * p.h_plane + lora_h_index(p, tile, rank / p.r, rank % p.r / 32) +
-                        (rank % p.r % 32 / 8) * 128 + rank % p.r % 8;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int of = __shfl(my_id, 4 * g + r, 64);  // row 4 g + r of the tile
-        if (of == id && rank < total) hp[(4 * g + r) * 8] = s[r];
-      }
-    }
-    __syncthreads();
-  });
+  }
 }
 
 // The lane's row of h, ranks 32 s + 8 g .. + 7, as two 16-bit parts; returns the factor that takes the products back.
@@ -218,18 +257,16 @@ __device__ __forceinline__ void times_b(const LoraParams& p, const vec8<T> (&w)[
   }
 }
 
-// y of the lane: rows 4 g + r of the tile (past the last one: the last one again), columns nc .. + NT - 1.
+// y of the lane: columns nc .. + NT - 1 of its four rows.
 template <typename T, int NT>
 using vecn = T __attribute__((ext_vector_type(NT)));
 template <typename T, int NT>
 using vecn_h = T __attribute__((ext_vector_type(NT), aligned(2)));  // at any element
 template <typename T, int NT>
-__device__ __forceinline__ void load_y(const LoraParams& p, int64_t first, int nc, int end, bool whole, vecn<T, NT> (&y)[4]) {
-  const int g = (threadIdx.x & 63) >> 4;
-  const int last = static_cast<int>(min(p.m - 1 - first, static_cast<int64_t>(15)));
+__device__ __forceinline__ void load_y(const LoraParams& p, int row0, const int (&row)[4], int nc, int end, bool whole, vecn<T, NT> (&y)[4]) {
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
-    const T* const yp = static_cast<const T*>(p.y) + first * p.ldy + min(4 * g + r, last) * p.ldy + nc;
+    const T* const yp = static_cast<const T*>(p.y) + row0 * p.ldy + row[r] * p.ldy + nc;
     if (whole) {
       y[r] = *reinterpret_cast<const vecn_h<T, NT>*>(yp);
     } else {
@@ -239,20 +276,19 @@ __device__ __forceinline__ void load_y(const LoraParams& p, int64_t first, int n
   }
 }
 
-// The rows of adapter id (-1: as they were).
+// The lane's first n rows (id -1: as they were).
 template <typename T, int NT>
-__device__ __forceinline__ void store_rows(const LoraParams& p, int64_t first, int nc, int end, bool whole, int id, const int (&of)[4],
+__device__ __forceinline__ void store_rows(const LoraParams& p, int row0, const int (&row)[4], int n, int nc, int end, bool whole, int id,
                                            const float (&back)[4], float scale, const v4f (&acc)[NT], const vecn<T, NT> (&y)[4]) {
-  const int g = (threadIdx.x & 63) >> 4;
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
-    if (of[r] != id) continue;
+    if (r >= n) continue;
     vecn<T, NT> z = y[r];
     if (id >= 0) {
 #pragma unroll
       for (int e = 0; e < NT; ++e) z[e] = static_cast<T>(fmaf(acc[e][r] * back[r], scale, static_cast<float>(z[e])));
     }
-    T* const op = static_cast<T*>(p.out) + first * p.ldo + (4 * g + r) * p.ldo + nc;
+    T* const op = static_cast<T*>(p.out) + row0 * p.ldo + row[r] * p.ldo + nc;
     if (whole) {
       __builtin_nontemporal_store(z, reinterpret_cast<vecn_h<T, NT>*>(op));  // past the L2, which B and h need
     } else {
@@ -273,17 +309,16 @@ template <int KS>
 constexpr int kCols = KS <= 2 ? 128 : 64;
 
 // KS: ranks / 32.
-template <typename T, int KS>
+template <typename T, int KS, bool GATHER>
 __global__ __launch_bounds__(256, KS == 1 ? 4 : 2) void lora_up_kernel(LoraParams p) {
   constexpr int C = kCols<KS>, NT = C / 16;  // a lane's consecutive columns
   constexpr int ZA = KS == 1 ? 4 : 1;        // K slices of h that are loaded at once
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, col = lane & 15;
-  // The workgroup's four blocks within a slice, its rows, and its part of their adapters.
+  // The workgroup's four blocks within a slice, and its rows.
   int run = blockIdx.x % p.runs, slice = 0, n0 = 0;
   const int rest = blockIdx.x / p.runs;
-  const int which = rest % p.groups, tile = rest / p.groups;
   for (; slice < p.slices; ++slice) {
     const int runs = (p.width[slice] + 4 * C - 1) / (4 * C);
     if (run < runs) break;
@@ -297,96 +332,90 @@ __global__ __launch_bounds__(256, KS == 1 ? 4 : 2) void lora_up_kernel(LoraParam
   const bool whole = n0 + C <= end;  // uniform
   const bool in_place = p.out == p.y && p.ldo == p.ldy;
 
-  // The ids, h (ranks 32 s + 8 g .. + 7 of row `col`) and y (columns nc .. + NT - 1 of rows 4 g + r).  Rows past the last
-  // one are the last one again.
-  const int64_t first = 16LL * tile;
-  const int last = static_cast<int>(min(p.m - 1 - first, static_cast<int64_t>(15)));
-  const int raw = lora_raw_id(p, first + min(col, last));
-  v4f part[ZA][KS][2];
-  if (p.adapters > 0) {
+  Tile<GATHER> tile;
+  if (!find_tile(p, rest / p.groups, rest % p.groups, !in_place, tile)) return;
+  int row[4];
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      const float* const hp = p.h + lora_h_index(p, tile, slice, s) + lane * 8;
-#pragma unroll
-      for (int z = 0; z < ZA; ++z)
-        if (z < p.ksplit) {
-          part[z][s][0] = *reinterpret_cast<const v4f*>(hp + z * p.h_plane);
-          part[z][s][1] = *reinterpret_cast<const v4f*>(hp + z * p.h_plane + 4);
-        }
-    }
-  }
+  for (int r = 0; r < 4; ++r) row[r] = tile.row(4 * g + r);
+  float back[4]{};
+  v4f acc[NT]{};
   vecn<T, NT> y[4];
-  load_y<T, NT>(p, first, nc, end, whole, y);
+  if (p.adapters == 0) {
+    load_y<T, NT>(p, tile.row0, row, nc, end, whole, y);
+    if (!in_place) store_rows<T, NT>(p, tile.row0, row, tile.n - 4 * g, nc, end, whole, -1, back, 0.0f, acc, y);
+    return;
+  }
+  // Under way at once: h (ranks 32 s + 8 g .. + 7 of row `col`), y (columns nc .. + NT - 1 of rows 4 g + r), and B as soon as
+  // the id is here.
+  const int64_t h_row = lora_h_row(p, tile.row0 + tile.row(col), slice) + 128 * g;
+  v4f part[ZA][KS][2];
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    const float* const hp = p.h + h_row + min(s, (p.r + 31) / 32 - 1) * 512;
+#pragma unroll
+    for (int z = 0; z < ZA; ++z)
+      if (z < p.ksplit) {
+        part[z][s][0] = *reinterpret_cast<const v4f*>(hp + z * p.h_plane);
+        part[z][s][1] = *reinterpret_cast<const v4f*>(hp + z * p.h_plane + 4);
+      }
+  }
+  load_y<T, NT>(p, tile.row0, row, nc, end, whole, y);
+  if (!tile.known(p, !in_place)) return;
+  const int id = max(tile.id, 0);  // of a tile without an adapter: not used
+  const float scale = p.scale != nullptr ? p.scale[id] : 1.0f;
+  vec8<T> w[NT][KS];
+  load_b<T, NT, KS>(p, id, n0, end, w);
 
-  const int my_id = lora_id(p, raw, first + col);
   vec8<T> hi[KS], lo[KS];
-  float unshift;
-  {
-    float f[KS][8];
+  float f[KS][8];
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
+  for (int s = 0; s < KS; ++s) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) f[s][e] = p.adapters > 0 ? part[0][s][e >> 2][e & 3] : 0.0f;
+    for (int e = 0; e < 8; ++e) f[s][e] = part[0][s][e >> 2][e & 3];
 #pragma unroll
-      for (int z = 1; z < ZA; ++z)
-        if (z < p.ksplit) {
+    for (int z = 1; z < ZA; ++z)
+      if (z < p.ksplit) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) f[s][e] += part[z][s][e >> 2][e & 3];
-        }
-      for (int z = ZA; z < p.ksplit; ++z) {
-        const float* const hp = p.h + lora_h_index(p, tile, slice, s) + lane * 8 + z * p.h_plane;
-        const v4f a = *reinterpret_cast<const v4f*>(hp), b = *reinterpret_cast<const v4f*>(hp + 4);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          f[s][e] += a[e];
-          f[s][4 + e] += b[e];
-        }
+        for (int e = 0; e < 8; ++e) f[s][e] += part[z][s][e >> 2][e & 3];
       }
-      if (32 * s + 8 * g >= p.r) {  // past the last rank: anything
+    for (int z = ZA; z < p.ksplit; ++z) {
+      const float* const hp = p.h + h_row + min(s, (p.r + 31) / 32 - 1) * 512 + z * p.h_plane;
+      const v4f a = *reinterpret_cast<const v4f*>(hp), b = *reinterpret_cast<const v4f*>(hp + 4);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[s][e] = 0.0f;
+      for (int e = 0; e < 4; ++e) {
+        f[s][e] += a[e];
+        f[s][4 + e] += b[e];
       }
     }
-    unshift = split_h<T, KS>(f, hi, lo);
-  }
-  // What the lane ends with are rows 4 g + r, whose adapters and factors are in other lanes.
-  float back[4];
-  int of[4];
+    if (32 * s + 8 * g >= p.r) {  // past the last rank: anything
 #pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    back[r] = __shfl(unshift, 4 * g + r, 64);
-    of[r] = __shfl(my_id, 4 * g + r, 64);
-  }
-  each_adapter(my_id, !in_place, which, p.groups, [&](int id) {
-    float scale = 0.0f;
-    v4f acc[NT]{};
-    if (id >= 0) {
-      scale = p.scale != nullptr ? p.scale[id] : 1.0f;
-      vec8<T> w[NT][KS];
-      load_b<T, NT, KS>(p, id, n0, end, w);
-      times_b<T, NT, KS>(p, w, hi, lo, acc);
+      for (int e = 0; e < 8; ++e) f[s][e] = 0.0f;
     }
-    store_rows<T, NT>(p, first, nc, end, whole, id, of, back, scale, acc, y);
-  });
+  }
+  const float unshift = split_h<T, KS>(f, hi, lo);
+  // What the lane ends with are rows 4 g + r, whose factors are in other lanes.
+#pragma unroll
+  for (int r = 0; r < 4; ++r) back[r] = __shfl(unshift, 4 * g + r, 64);
+  times_b<T, NT, KS>(p, w, hi, lo, acc);
+  store_rows<T, NT>(p, tile.row0, row, tile.n - 4 * g, nc, end, whole, tile.id, back, scale, acc, y);
 }
 
 // Both products in one launch, for few rows: a workgroup computes h of its tile, adapter and slice itself (its eight
 // waves each an eighth of K, joined in LDS) while B and y are under way, and its waves take a block of kCols columns each.
 // Bound by the arrival of A at one CU.  One row into 2560 columns in three slices: 6.0 us, two launches 7.7; 64 rows of
-// 64 adapters into 2048: 8.3, 9.8.
-template <typename T, int NR>
+// 64 adapters into 2048: 7.0.
+template <typename T, int NR, bool GATHER>
 __global__ __launch_bounds__(512) void lora_fused_kernel(LoraParams p) {
   constexpr int W = 8, KS = (NR + 1) / 2, C = kCols<KS>, NT = C / 16;
   constexpr int kAhead = NR <= 2 ? 8 : 16 / NR;
   __shared__ __align__(16) v4f part[W][NR][64];
-  __shared__ __align__(16) float hs[KS * 512];  // as lora_h_index has a tile's block
+  __shared__ __align__(16) float hs[KS * 512];  // as a block of h
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, col = lane & 15;
   const int lr = lane >> 2, lc = lane & 3;  // row and chunk that the lane loads
   int run = blockIdx.x % p.runs, slice = 0, n0 = 0;
   const int rest = blockIdx.x / p.runs;
-  const int which = rest % p.groups, tile = rest / p.groups;
   for (; slice < p.slices; ++slice) {
     const int runs = (p.width[slice] + W * C - 1) / (W * C);
     if (run < runs) break;
@@ -399,169 +428,177 @@ __global__ __launch_bounds__(512) void lora_fused_kernel(LoraParams p) {
   const int nc = n0 + NT * col;
   const bool whole = n0 + C <= end;  // uniform
   const bool in_place = p.out == p.y && p.ldo == p.ldy;
-  const int64_t first = 16LL * tile;
-  const int my_id = lora_id(p, lora_raw_id(p, min(first + col, p.m - 1)), first + col);
-  vecn<T, NT> y[4];
-  if (columns) load_y<T, NT>(p, first, nc, end, whole, y);
-  int of[4];
+  Tile<GATHER> tile;
+  if (!find_tile(p, rest / p.groups, rest % p.groups, !in_place, tile)) return;
+  int row[4];
 #pragma unroll
-  for (int r = 0; r < 4; ++r) of[r] = __shfl(my_id, 4 * g + r, 64);
+  for (int r = 0; r < 4; ++r) row[r] = tile.row(4 * g + r);
+  vecn<T, NT> y[4];
+  if (columns) load_y<T, NT>(p, tile.row0, row, nc, end, whole, y);
 
   const int chunks = (p.k + 31) / 32, per_wave = (chunks + W - 1) / W;
   const int w0 = min(wave * per_wave, chunks), w1 = min(w0 + per_wave, chunks);
   const int full = min(w1, p.k / 32);  // chunks that K fills
-  const T* const xp = static_cast<const T*>(p.x) + min(first + lr, p.m - 1) * p.ldx + 8 * lc;
-  each_adapter(my_id, !in_place, which, p.groups, [&](int id) {
-    float scale = 0.0f, back[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    v4f out[NT]{};
-    if (id >= 0) {  // uniform
-      scale = p.scale != nullptr ? p.scale[id] : 1.0f;
-      vec8<T> w[NT][KS];
-      if (columns) load_b<T, NT, KS>(p, id, n0, end, w);
-      const T* ap[NR];
+  const T* const xp = static_cast<const T*>(p.x) + tile.row0 * p.ldx + tile.row(lr) * p.ldx + 8 * lc;
+  float scale = 0.0f, back[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  v4f out[NT]{};
+  if (!tile.known(p, !in_place)) return;
+  const int id = tile.id;
+  if (id >= 0) {  // uniform
+    scale = p.scale != nullptr ? p.scale[id] : 1.0f;
+    vec8<T> w[NT][KS];
+    if (columns) load_b<T, NT, KS>(p, id, n0, end, w);
+    const T* ap[NR];
 #pragma unroll
-      for (int i = 0; i < NR; ++i)  // ranks past the last one: the last one again, not used
-        ap[i] = static_cast<const T*>(p.a) + ((static_cast<int64_t>(id) * p.slices + slice) * p.r + min(16 * i + lr, p.r - 1)) * p.k + 8 * lc;
-      v4f acc[NR]{};
-      auto add = [&](const vec8<T> x, const vec8<T> (&a)[NR]) {
-        const vec8<T> u = to_operand<T>(x);
+    for (int i = 0; i < NR; ++i)  // ranks past the last one: the last one again, not used
+      ap[i] = static_cast<const T*>(p.a) + ((static_cast<int64_t>(id) * p.slices + slice) * p.r + min(16 * i + lr, p.r - 1)) * p.k + 8 * lc;
+    v4f acc[NR]{};
+    auto add = [&](const vec8<T> x, const vec8<T> (&a)[NR]) {
+      const vec8<T> u = to_operand<T>(x);
 #pragma unroll
-        for (int i = 0; i < NR; ++i) acc[i] = mfma(u, to_operand<T>(a[i]), acc[i]);
-      };
-      auto load = [&](vec8<T>& x, vec8<T> (&a)[NR], int k) {
-        x = *reinterpret_cast<const vec8<T>*>(xp + k);
+      for (int i = 0; i < NR; ++i) acc[i] = mfma(u, to_operand<T>(a[i]), acc[i]);
+    };
+    auto load = [&](vec8<T>& x, vec8<T> (&a)[NR], int k) {
+      x = *reinterpret_cast<const vec8<T>*>(xp + k);
 #pragma unroll
-        for (int i = 0; i < NR; ++i) a[i] = *reinterpret_cast<const vec8<T>*>(ap[i] + k);
-      };
-      int c = w0;
-      for (; c + kAhead <= full; c += kAhead) {
-        vec8<T> x[kAhead], a[kAhead][NR];
+      for (int i = 0; i < NR; ++i) a[i] = *reinterpret_cast<const vec8<T>*>(ap[i] + k);
+    };
+    int c = w0;
+    for (; c + kAhead <= full; c += kAhead) {
+      vec8<T> x[kAhead], a[kAhead][NR];
 #pragma unroll
-        for (int j = 0; j < kAhead; ++j) load(x[j], a[j], 32 * (c + j));
+      for (int j = 0; j < kAhead; ++j) load(x[j], a[j], 32 * (c + j));
 #pragma unroll
-        for (int j = 0; j < kAhead; ++j) add(x[j], a[j]);
-      }
-      for (; c < w1; ++c) {  // the last ones, and one that K does not fill
-        vec8<T> x, a[NR];
-        const bool in = 32 * c + 8 * lc < p.k;
-        load(x, a, in ? 32 * c : -8 * lc);  // elsewhere the row's first elements
-        if (!in) {
-          x = vec8<T>{};
-#pragma unroll
-          for (int i = 0; i < NR; ++i) a[i] = vec8<T>{};
-        }
-        add(x, a);
-      }
-#pragma unroll
-      for (int i = 0; i < NR; ++i) part[wave][i][lane] = acc[i];
-      __syncthreads();
-      if (wave < NR) {
-        v4f s = part[0][wave][lane];
-#pragma unroll
-        for (int j = 1; j < W; ++j) s += part[j][wave][lane];
-        const int rank = 16 * wave + col;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) hs[rank / 32 * 512 + rank % 32 / 8 * 128 + (4 * g + r) * 8 + rank % 8] = s[r];
-      }
-      __syncthreads();
-      if (columns) {
-        float f[KS][8];
-        vec8<T> hi[KS], lo[KS];
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-          const v4f a = *reinterpret_cast<const v4f*>(hs + s * 512 + lane * 8), b = *reinterpret_cast<const v4f*>(hs + s * 512 + lane * 8 + 4);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) f[s][e] = 32 * s + 8 * g >= p.r ? 0.0f : e < 4 ? a[e & 3] : b[e & 3];
-        }
-        const float unshift = split_h<T, KS>(f, hi, lo);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) back[r] = __shfl(unshift, 4 * g + r, 64);
-        times_b<T, NT, KS>(p, w, hi, lo, out);
-      }
+      for (int j = 0; j < kAhead; ++j) add(x[j], a[j]);
     }
-    if (columns) store_rows<T, NT>(p, first, nc, end, whole, id, of, back, scale, out, y);
-  });
+    for (; c < w1; ++c) {  // the last ones, and one that K does not fill
+      vec8<T> x, a[NR];
+      const bool in = 32 * c + 8 * lc < p.k;
+      load(x, a, in ? 32 * c : -8 * lc);  // elsewhere the row's first elements
+      if (!in) {
+        x = vec8<T>{};
+#pragma unroll
+        for (int i = 0; i < NR; ++i) a[i] = vec8<T>{};
+      }
+      add(x, a);
+    }
+#pragma unroll
+    for (int i = 0; i < NR; ++i) part[wave][i][lane] = acc[i];
+    __syncthreads();
+    if (wave < NR) {
+      v4f s = part[0][wave][lane];
+#pragma unroll
+      for (int j = 1; j < W; ++j) s += part[j][wave][lane];
+      const int rank = 16 * wave + col;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) hs[rank / 32 * 512 + rank % 32 / 8 * 128 + (4 * g + r) * 8 + rank % 8] = s[r];
+    }
+    __syncthreads();
+    if (columns) {
+      float f[KS][8];
+      vec8<T> hi[KS], lo[KS];
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        const v4f a = *reinterpret_cast<const v4f*>(hs + s * 512 + lane * 8), b = *reinterpret_cast<const v4f*>(hs + s * 512 + lane * 8 + 4);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[s][e] = 32 * s + 8 * g >= p.r ? 0.0f : e < 4 ? a[e & 3] : b[e & 3];
+      }
+      const float unshift = split_h<T, KS>(f, hi, lo);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) back[r] = __shfl(unshift, 4 * g + r, 64);
+      times_b<T, NT, KS>(p, w, hi, lo, out);
+    }
+  }
+  if (columns) store_rows<T, NT>(p, tile.row0, row, tile.n - 4 * g, nc, end, whole, id, back, scale, out, y);
 }
 
-template <typename T>
+template <typename T, bool GATHER>
 void launch_down(const LoraParams& p, hipStream_t stream) {
-  const unsigned tiles = static_cast<unsigned>((p.m + 15) / 16 * p.groups);
+  const unsigned tiles = static_cast<unsigned>(p.units) * p.groups;
   const int total = p.slices * p.r;
   if (total <= 16)
-    lora_down_kernel<T, 1><<<dim3(tiles, 1, p.ksplit), 512, 0, stream>>>(p);
+    lora_down_kernel<T, 1, GATHER><<<dim3(tiles, 1, p.ksplit), 512, 0, stream>>>(p);
   else if (total <= 32)
-    lora_down_kernel<T, 2><<<dim3(tiles, 1, p.ksplit), 512, 0, stream>>>(p);
+    lora_down_kernel<T, 2, GATHER><<<dim3(tiles, 1, p.ksplit), 512, 0, stream>>>(p);
   else
-    lora_down_kernel<T, 4><<<dim3(tiles, (total + 63) / 64, p.ksplit), 512, 0, stream>>>(p);
+    lora_down_kernel<T, 4, GATHER><<<dim3(tiles, (total + 63) / 64, p.ksplit), 512, 0, stream>>>(p);
 }
 
-template <typename T, int KS>
-void launch_up(const LoraParams& p, hipStream_t stream) {
-  const dim3 grid(static_cast<unsigned>((p.m + 15) / 16 * p.groups * p.runs));
-  lora_up_kernel<T, KS><<<grid, 256, 0, stream>>>(p);
-}
-
-template <typename T, int NR>
-void launch_fused(const LoraParams& p, hipStream_t stream) {
-  const dim3 grid(static_cast<unsigned>((p.m + 15) / 16 * p.groups * p.runs));
-  lora_fused_kernel<T, NR><<<grid, 512, 0, stream>>>(p);
-}
-
-template <typename T>
+template <typename T, bool GATHER>
 void launch(const LoraParams& p, hipStream_t stream) {
+  const dim3 grid(static_cast<unsigned>(p.units) * p.groups * p.runs);
   if (p.ksplit == 0) {
-    if (p.r <= 16) launch_fused<T, 1>(p, stream);
-    else if (p.r <= 32) launch_fused<T, 2>(p, stream);
-    else if (p.r <= 64) launch_fused<T, 4>(p, stream);
-    else launch_fused<T, 8>(p, stream);
+    if (p.r <= 16) lora_fused_kernel<T, 1, GATHER><<<grid, 512, 0, stream>>>(p);
+    else if (p.r <= 32) lora_fused_kernel<T, 2, GATHER><<<grid, 512, 0, stream>>>(p);
+    else if (p.r <= 64) lora_fused_kernel<T, 4, GATHER><<<grid, 512, 0, stream>>>(p);
+    else lora_fused_kernel<T, 8, GATHER><<<grid, 512, 0, stream>>>(p);
     return;
   }
-  if (p.adapters > 0) launch_down<T>(p, stream);
-  if (p.r <= 32) launch_up<T, 1>(p, stream);
-  else if (p.r <= 64) launch_up<T, 2>(p, stream);
-  else launch_up<T, 4>(p, stream);
+  if (p.adapters > 0) launch_down<T, GATHER>(p, stream);
+  if (p.r <= 32) lora_up_kernel<T, 1, GATHER><<<grid, 256, 0, stream>>>(p);
+  else if (p.r <= 64) lora_up_kernel<T, 2, GATHER><<<grid, 256, 0, stream>>>(p);
+  else lora_up_kernel<T, 4, GATHER><<<grid, 256, 0, stream>>>(p);
 }
 
 }  // namespace
 
 int64_t lora_h_floats(int64_t m, int32_t r, int32_t slices) { return (m + 15) / 16 * slices * ((r + 31) / 32) * 512; }
 
-// A tile's adapters go to as many workgroups as it can have adapters, where tiles are few.  One launch (ksplit 0) where its
-// workgroups have a CU each and the ranks that each reads again are at most 128 KB (one / two launches, us: 64 KB 6.0 / 7.7,
-// 256 KB (K = 4096, rank 32) 9.7 / 8.6, 512 KB 15.7 / 9.0; 256 rows of 64 adapters, 1024 workgroups, 27.6 / 21.1).  Else K slices
-// for as many workgroups as CUs.
+// Tiles of consecutive rows where requests have 64 or more (or there is one).  Else windows: as many workgroups as a window
+// can have tiles, found by counting; past 32 one for each row, the first row of a tile its workgroup's, which costs
+// nothing to find.  One launch (ksplit 0) where its workgroups have a CU each and the ranks that each reads again
+// are at most 128 KB (one / two launches, us: 64 KB 6.0 / 7.7, 256 KB (K = 4096, rank 32) 9.7 / 8.6, 512 KB 15.7 / 9.0).
+// Else K slices for as many workgroups as CUs, and of 8192 or more for six a CU (12139 rows of 16384, rank 24: in 1 / 2 / 4
+// slices 162 / 132 / 131 us, 6208 rows, rank 64: 138 / 114 / 118; with K = 2048 the sums cost more, 6208 x 32768
+// in two slices, 64 rows of A: 164.5 / 163.8 / 179).
 LoraPlan lora_plan(int64_t m, int64_t per_id, int32_t k, int32_t n, int32_t r, int32_t slices, int32_t adapters, int cus) {
-  LoraPlan plan;
-  const int64_t tiles = (m + 15) / 16;
-  const int64_t most = std::min<int64_t>({16, 15 / per_id + 2, adapters + 1});
-  plan.groups = per_id >= 16 ? 1 : static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(most, 2 * cus / tiles)));
+  LoraPlan plan{};
+  plan.gather = per_id < kWindow && per_id < m;
+  if (plan.gather) {
+    const int64_t rows = std::min<int64_t>(m, kWindow);
+    const int64_t kinds = std::min<int64_t>({rows, (rows - 1) / per_id + 2, static_cast<int64_t>(adapters) + 1});
+    const int64_t tiles = std::min((rows + 15 * kinds) / 16, rows);
+    plan.leaders = tiles > 32;
+    plan.units = static_cast<int32_t>((m + kWindow - 1) / kWindow);
+    plan.groups = static_cast<int32_t>(plan.leaders ? rows : tiles);
+  } else {
+    plan.tiles = static_cast<int32_t>((std::min(per_id, m) + 15) / 16);
+    plan.units = static_cast<int32_t>((m + per_id - 1) / per_id * plan.tiles);
+    plan.groups = 1;
+  }
+  const int64_t all = static_cast<int64_t>(plan.units) * plan.groups;
   int64_t ranks = 16;
   while (ranks < r) ranks *= 2;
   const int64_t run = ranks <= 64 ? 1024 : 512;  // columns of a workgroup
-  if (ranks * k * 2 <= (128 << 10) && tiles * plan.groups * ((n + run - 1) / run + slices - 1) <= cus) {
-    plan.ksplit = 0;
-    return plan;
-  }
-  const int64_t down = tiles * plan.groups * ((slices * r + 63) / 64);
-  plan.ksplit = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({cus / down, (k + 511) / 512, 8})));
+  if (ranks * k * 2 <= (128 << 10) && all * ((n + run - 1) / run + slices - 1) <= cus) return plan;
+  const int64_t down = all * ((slices * r + 63) / 64);
+  const int64_t fill = std::min<int64_t>({cus / down, (k + 511) / 512, 8}), even = std::min<int64_t>(k / 8192, (6 * cus + down - 1) / down);
+  plan.ksplit = static_cast<int32_t>(std::max<int64_t>({1, fill, even}));
   return plan;
 }
 
-bool lora_grid(LoraParams& p) {
+bool lora_grid(LoraParams& p, const LoraPlan& plan) {
+  p.ksplit = plan.ksplit;
+  p.groups = plan.groups;
+  p.units = plan.units;
+  p.tiles = plan.tiles;
+  p.gather = plan.gather;
+  p.leaders = plan.leaders;
   const int64_t waves = p.ksplit == 0 ? 8 : 4, columns = waves * (p.r <= 64 ? kCols<1> : kCols<4>);
   int64_t runs = 0;
   for (int s = 0; s < p.slices; ++s) runs += (p.width[s] + columns - 1) / columns;
   p.runs = static_cast<int32_t>(runs);
   p.h_plane = lora_h_floats(p.m, p.r, p.slices);
-  return (p.m + 15) / 16 * p.groups * runs * waves < (1 << 26);
+  const int64_t all = static_cast<int64_t>(p.units) * p.groups;
+  return all * runs * waves < (1 << 26) && all * 8 < (1 << 26);
 }
 
 hipError_t launch_lora(const LoraParams& p, int elem, hipStream_t stream) {
   if (p.m <= 0 || p.n <= 0) return hipSuccess;
   if (elem == kFp16)
-    launch<_Float16>(p, stream);
+    p.gather ? launch<_Float16, true>(p, stream) : launch<_Float16, false>(p, stream);
   else
-    launch<__bf16>(p, stream);
+    p.gather ? launch<__bf16, true>(p, stream) : launch<__bf16, false>(p, stream);
   return hipGetLastError();
 }
 

@@ -86,18 +86,22 @@ struct LoraParams {
   int32_t k, n, r, adapters, slices;
   int32_t width[kLoraSlices];  // columns of each slice
   int32_t ksplit;      // K slices of the first launch; 0: both products in one
-  int32_t groups;      // workgroups that share a row tile's adapters
+  int32_t units;       // 16-row tiles of requests, or windows of rows
+  int32_t groups;      // workgroups of a window: its tiles at most
+  int32_t tiles;       // of a request
+  int32_t gather;      // windows
+  int32_t leaders;     // a workgroup for each row of a window
   int32_t runs;        // of a workgroup's columns, over the slices
   int64_t h_plane;     // floats of a K slice in h
 };
 struct LoraPlan {
-  int ksplit;
-  int groups;
+  int32_t ksplit, units, groups, tiles;
+  bool gather, leaders;
 };
 LoraPlan lora_plan(int64_t m, int64_t per_id, int32_t k, int32_t n, int32_t r, int32_t slices, int32_t adapters, int cus);
 int64_t lora_h_floats(int64_t m, int32_t r, int32_t slices);
-// What of a call follows from its plan (runs, h_plane); false: its waves are more than one launch holds.
-bool lora_grid(LoraParams& p);
+// What of a call follows from its plan; false: its waves are more than one launch holds.
+bool lora_grid(LoraParams& p, const LoraPlan& plan);
 hipError_t launch_lora(const LoraParams& p, int elem, hipStream_t stream);
 
 }  // namespace w4a4

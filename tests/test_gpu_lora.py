@@ -13,6 +13,7 @@ import pytest
 import torch
 
 from pi05_fast import w4a4
+from pi05_fast.w4a4 import extension as ext
 
 pytestmark = pytest.mark.gpu
 TYPES = [torch.float16, torch.bfloat16]
@@ -114,6 +115,50 @@ def test_requests_of_many_tokens(cuda):
     assert torch.equal(w4a4.lora_add(y, x, a, b, flat.view(4, 50), scale), want)
     one = _exact(y.view(200, 96), x.view(200, 256), a, b, torch.full_like(flat, 2), scale, [96]).view(4, 50, 96)
     assert torch.equal(w4a4.lora_add(y, x, a, b, _ids(2), scale), one)
+
+
+@pytest.mark.parametrize("adapters", [1, 3, 70])
+@pytest.mark.parametrize("per_id", [1, 2, 5, 16, 31, 63, 64, 65, 100, 130])
+def test_requests_of_any_length(cuda, per_id, adapters):
+    """Rows of an adapter together or apart, fewer and more than a tile, and rows of NaN beside them."""
+    requests = 200 // per_id + 2
+    m = requests * per_id
+    gen = _gen(per_id + adapters)
+    y, x, a, b, scale = _whole(gen, m, 72, 40, 8, adapters, 1, torch.bfloat16)
+    bad = torch.zeros(m, dtype=torch.bool, device="cuda")
+    bad[::7] = True
+    for ids in (torch.randint(-1, adapters + 1, (requests,), device="cuda", generator=gen), torch.arange(requests, device="cuda") % 3 - 1):
+        ids = ids.to(torch.int32)
+        rows = ids.repeat_interleave(per_id)
+        want = _exact(y, x, a, b, rows, scale, [40])
+        xs = x.masked_fill(bad[:, None], float("nan")).view(requests, per_id, 72)
+        got = w4a4.lora_add(y.view(requests, per_id, 40), xs, a, b, ids, scale).view(m, 40)
+        named = (rows >= 0) & (rows < adapters)
+        assert torch.equal(got[~bad | ~named], want[~bad | ~named]) and torch.isnan(got[bad & named]).all()
+        z = y.clone().view(requests, per_id, 40)
+        w4a4.lora_add_(z, xs, a, b, ids, scale)
+        assert torch.equal(z.view(m, 40).nan_to_num(0), got.nan_to_num(0))
+
+
+def test_rows_short_of_a_request(cuda):
+    """At the C entry the last id may have fewer rows than the others."""
+    lib = ext.load_int4_gemm()
+    for m, per_id in ((150, 64), (37, 20), (129, 128), (5, 9)):
+        y, x, a, b, scale = _whole(_gen(m), m, 64, 48, 16, 3, 1, torch.float16)
+        ids = torch.arange((m + per_id - 1) // per_id, device="cuda").to(torch.int32) % 3
+        out, ws = torch.empty_like(y), torch.empty(1 << 20, dtype=torch.uint8, device="cuda")
+        assert lib.pi05w4a4_lora_workspace_bytes(m, per_id, 64, 48, 16, 1, 3) <= ws.numel()
+        rc = lib.pi05w4a4_lora_add(y.data_ptr(), 48, x.data_ptr(), 64, m, 64, a.data_ptr(), b.data_ptr(), scale.data_ptr(), 3, 16, ids.data_ptr(),
+                                   per_id, 48, 1, None, 0, out.data_ptr(), 48, ws.data_ptr(), ws.numel(), torch.cuda.current_stream().cuda_stream)
+        assert rc == 0 and torch.equal(out, _exact(y, x, a, b, ids.repeat_interleave(per_id)[:m], scale, [48]))
+
+
+def test_many_rows_of_a_long_k(cuda):
+    """K in slices although every CU has rows."""
+    y, x, a, b, scale = _whole(_gen(10), 5000, 16384, 64, 24, 2, 1, torch.float16)
+    ids = torch.arange(50, device="cuda").to(torch.int32) % 3
+    want = _exact(y, x, a, b, ids.repeat_interleave(100), scale, [64])
+    assert torch.equal(w4a4.lora_add(y.view(50, 100, 64), x.view(50, 100, 16384), a, b, ids, scale).view(5000, 64), want)
 
 
 def test_strides(cuda):
