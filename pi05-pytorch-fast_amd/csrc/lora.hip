@@ -312,7 +312,7 @@ constexpr int kCols = KS <= 2 ? 128 : 64;
 template <typename T, int KS, bool GATHER>
 __global__ __launch_bounds__(256, KS == 1 ? 4 : 2) void lora_up_kernel(LoraParams p) {
   constexpr int C = kCols<KS>, NT = C / 16;  // a lane's consecutive columns
-  constexpr int ZA = KS == 1 ? 4 : 1;        // K slices of h that are loaded at once
+  constexpr int ZA = KS == 1 ? 4 : 2;        // K slices of h that are loaded at once
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, col = lane & 15;
@@ -349,16 +349,19 @@ __global__ __launch_bounds__(256, KS == 1 ? 4 : 2) void lora_up_kernel(LoraParam
   // the id is here.
   const int64_t h_row = lora_h_row(p, tile.row0 + tile.row(col), slice) + 128 * g;
   v4f part[ZA][KS][2];
-#pragma unroll
-  for (int s = 0; s < KS; ++s) {
-    const float* const hp = p.h + h_row + min(s, (p.r + 31) / 32 - 1) * 512;
+  auto load_h = [&](int z0) {
 #pragma unroll
     for (int z = 0; z < ZA; ++z)
-      if (z < p.ksplit) {
-        part[z][s][0] = *reinterpret_cast<const v4f*>(hp + z * p.h_plane);
-        part[z][s][1] = *reinterpret_cast<const v4f*>(hp + z * p.h_plane + 4);
+      if (z0 + z < p.ksplit) {
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          const float* const hp = p.h + h_row + min(s, (p.r + 31) / 32 - 1) * 512 + (z0 + z) * p.h_plane;
+          part[z][s][0] = *reinterpret_cast<const v4f*>(hp);
+          part[z][s][1] = *reinterpret_cast<const v4f*>(hp + 4);
+        }
       }
-  }
+  };
+  load_h(0);
   load_y<T, NT>(p, tile.row0, row, nc, end, whole, y);
   if (!tile.known(p, !in_place)) return;
   const int id = max(tile.id, 0);  // of a tile without an adapter: not used
@@ -369,29 +372,27 @@ __global__ __launch_bounds__(256, KS == 1 ? 4 : 2) void lora_up_kernel(LoraParam
   vec8<T> hi[KS], lo[KS];
   float f[KS][8];
 #pragma unroll
-  for (int s = 0; s < KS; ++s) {
+  for (int s = 0; s < KS; ++s)
 #pragma unroll
     for (int e = 0; e < 8; ++e) f[s][e] = part[0][s][e >> 2][e & 3];
+  for (int z0 = 0;; load_h(z0)) {
 #pragma unroll
-    for (int z = 1; z < ZA; ++z)
-      if (z < p.ksplit) {
+    for (int z = 0; z < ZA; ++z)
+      if (z0 + z > 0 && z0 + z < p.ksplit) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[s][e] += part[z][s][e >> 2][e & 3];
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) f[s][e] += part[z][s][e >> 2][e & 3];
       }
-    for (int z = ZA; z < p.ksplit; ++z) {
-      const float* const hp = p.h + h_row + min(s, (p.r + 31) / 32 - 1) * 512 + z * p.h_plane;
-      const v4f a = *reinterpret_cast<const v4f*>(hp), b = *reinterpret_cast<const v4f*>(hp + 4);
+    z0 += ZA;
+    if (z0 >= p.ksplit) break;
+  }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        f[s][e] += a[e];
-        f[s][4 + e] += b[e];
-      }
-    }
+  for (int s = 0; s < KS; ++s)
     if (32 * s + 8 * g >= p.r) {  // past the last rank: anything
 #pragma unroll
       for (int e = 0; e < 8; ++e) f[s][e] = 0.0f;
     }
-  }
   const float unshift = split_h<T, KS>(f, hi, lo);
   // What the lane ends with are rows 4 g + r, whose factors are in other lanes.
 #pragma unroll
