@@ -304,15 +304,15 @@ __device__ __forceinline__ void store_rows(const LoraParams& p, int row0, const 
 // the next tile under way, in a form whose stores went through the L2: 191 us for 6208 x 32768 in place of 199, but 51
 // for 2560 columns in place of 47).  Column j of tile i is column NT j + i of the block: a lane ends with NT (eight, or four for large ranks) consecutive columns of four
 // rows, and 16 lanes read and write 256 or 128 consecutive bytes of a row.  Bound by y and out in HBM where rows are
-// many: 6208 x 32768 with rank 32, both launches 165 us, 5.1 TB/s.
+// many: 6208 x 32768 with rank 32, both launches 161 us, 5.3 TB/s.
 template <int KS>
 constexpr int kCols = KS <= 2 ? 128 : 64;
 
 // KS: ranks / 32.
 template <typename T, int KS, bool GATHER>
-__global__ __launch_bounds__(256, KS == 1 ? 4 : 2) void lora_up_kernel(LoraParams p) {
+__global__ __launch_bounds__(256, KS == 1 ? 4 : 3) void lora_up_kernel(LoraParams p) {
   constexpr int C = kCols<KS>, NT = C / 16;  // a lane's consecutive columns
-  constexpr int ZA = KS == 1 ? 4 : 2;        // K slices of h that are loaded at once
+  constexpr int ZA = 4 / KS;                 // K slices of h that are loaded at once
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, col = lane & 15;
@@ -549,9 +549,9 @@ int64_t lora_h_floats(int64_t m, int32_t r, int32_t slices) { return (m + 15) / 
 // can have tiles, found by counting; past 32 one for each row, the first row of a tile its workgroup's, which costs
 // nothing to find.  One launch (ksplit 0) where its workgroups have a CU each and the ranks that each reads again
 // are at most 128 KB (one / two launches, us: 64 KB 6.0 / 7.7, 256 KB (K = 4096, rank 32) 9.7 / 8.6, 512 KB 15.7 / 9.0).
-// Else K slices for as many workgroups as CUs, and of 8192 or more for six a CU (12139 rows of 16384, rank 24: in 1 / 2 / 4
-// slices 162 / 132 / 131 us, 6208 rows, rank 64: 138 / 114 / 118; with K = 2048 the sums cost more, 6208 x 32768
-// in two slices, 64 rows of A: 164.5 / 163.8 / 179).
+// Else K slices for two workgroups a CU (1963 x 4096 with 96 rows of A, 260 workgroups: 32.9 us, in two slices 30.2), and of 8192 or
+// more for six (12139 rows of 16384, rank 24: in 1 / 2 / 4 slices 162 / 132 / 131 us, 6208 rows, rank 64: 138 / 114 /
+// 118); with K = 2048 more slices cost more than they give (6208 x 32768, 64 rows of A: 164.5 / 163.8 / 179).
 LoraPlan lora_plan(int64_t m, int64_t per_id, int32_t k, int32_t n, int32_t r, int32_t slices, int32_t adapters, int cus) {
   LoraPlan plan{};
   plan.gather = per_id < kWindow && per_id < m;
@@ -573,7 +573,7 @@ LoraPlan lora_plan(int64_t m, int64_t per_id, int32_t k, int32_t n, int32_t r, i
   const int64_t run = ranks <= 64 ? 1024 : 512;  // columns of a workgroup
   if (ranks * k * 2 <= (128 << 10) && all * ((n + run - 1) / run + slices - 1) <= cus) return plan;
   const int64_t down = all * ((slices * r + 63) / 64);
-  const int64_t fill = std::min<int64_t>({cus / down, (k + 511) / 512, 8}), even = std::min<int64_t>(k / 8192, (6 * cus + down - 1) / down);
+  const int64_t fill = std::min<int64_t>({(2 * cus + down - 1) / down, (k + 511) / 512, 8}), even = std::min<int64_t>(k / 8192, (6 * cus + down - 1) / down);
   plan.ksplit = static_cast<int32_t>(std::max<int64_t>({1, fill, even}));
   return plan;
 }
