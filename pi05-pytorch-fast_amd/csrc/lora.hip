@@ -132,12 +132,14 @@ __global__ __launch_bounds__(512) void lora_down_kernel(LoraParams p) {
   const int g = lane >> 4, col = lane & 15;
   const int lr = lane >> 2, lc = lane & 3;  // row and chunk that the lane loads
   Tile<GATHER> tile;
-  if (!find_tile(p, blockIdx.x / p.groups, blockIdx.x % p.groups, false, tile) || !tile.known(p, false)) return;
+  // The K slices are the fastest: workgroups whose numbers are equal mod 8 share an XCD, whose L2 then holds its slices of A.
+  const int place = blockIdx.x / p.ksplit, kslice = blockIdx.x - place * p.ksplit;
+  if (!find_tile(p, place / p.groups, place % p.groups, false, tile) || !tile.known(p, false)) return;
   const int total = p.slices * p.r;  // rows of an adapter's A
   const int rank0 = blockIdx.y * 16 * NR;
   const int chunks = (p.k + 31) / 32;
   const int per_slice = (chunks + p.ksplit - 1) / p.ksplit;
-  const int c0 = blockIdx.z * per_slice, c1 = min(c0 + per_slice, chunks);
+  const int c0 = kslice * per_slice, c1 = min(c0 + per_slice, chunks);
   const int per_wave = (per_slice + W - 1) / W;
   const int w0 = min(c0 + wave * per_wave, c1), w1 = min(w0 + per_wave, c1);
   const int whole = min(w1, p.k / 32);  // chunks that K fills
@@ -187,7 +189,7 @@ __global__ __launch_bounds__(512) void lora_down_kernel(LoraParams p) {
 #pragma unroll
     for (int w = 1; w < W; ++w) s += part[w][i][lane];
     const int rank = rank0 + 16 * i + col, slice = rank / p.r, of = rank % p.r;
-    float* const hp = p.h + blockIdx.z * p.h_plane + of / 8 * 128 + of % 8;  // blocks of 32 ranks follow one another
+    float* const hp = p.h + kslice * p.h_plane + of / 8 * 128 + of % 8;  // blocks of 32 ranks follow one another
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int row = tile.row0 + tile.row(4 * g + r);
@@ -515,14 +517,14 @@ __global__ __launch_bounds__(512) void lora_fused_kernel(LoraParams p) {
 
 template <typename T, bool GATHER>
 void launch_down(const LoraParams& p, hipStream_t stream) {
-  const unsigned tiles = static_cast<unsigned>(p.units) * p.groups;
+  const unsigned tiles = static_cast<unsigned>(p.units) * p.groups * p.ksplit;
   const int total = p.slices * p.r;
   if (total <= 16)
-    lora_down_kernel<T, 1, GATHER><<<dim3(tiles, 1, p.ksplit), 512, 0, stream>>>(p);
+    lora_down_kernel<T, 1, GATHER><<<tiles, 512, 0, stream>>>(p);
   else if (total <= 32)
-    lora_down_kernel<T, 2, GATHER><<<dim3(tiles, 1, p.ksplit), 512, 0, stream>>>(p);
+    lora_down_kernel<T, 2, GATHER><<<tiles, 512, 0, stream>>>(p);
   else
-    lora_down_kernel<T, 4, GATHER><<<dim3(tiles, (total + 63) / 64, p.ksplit), 512, 0, stream>>>(p);
+    lora_down_kernel<T, 4, GATHER><<<dim3(tiles, (total + 63) / 64), 512, 0, stream>>>(p);
 }
 
 template <typename T, bool GATHER>
@@ -549,9 +551,11 @@ int64_t lora_h_floats(int64_t m, int32_t r, int32_t slices) { return (m + 15) / 
 // can have tiles, found by counting; past 32 one for each row, the first row of a tile its workgroup's, which costs
 // nothing to find.  One launch (ksplit 0) where its workgroups have a CU each and the ranks that each reads again
 // are at most 128 KB (one / two launches, us: 64 KB 6.0 / 7.7, 256 KB (K = 4096, rank 32) 9.7 / 8.6, 512 KB 15.7 / 9.0).
-// Else K slices for two workgroups a CU (1963 x 4096 with 96 rows of A, 260 workgroups: 32.9 us, in two slices 30.2), and of 8192 or
-// more for six (12139 rows of 16384, rank 24: in 1 / 2 / 4 slices 162 / 132 / 131 us, 6208 rows, rank 64: 138 / 114 /
-// 118); with K = 2048 more slices cost more than they give (6208 x 32768, 64 rows of A: 164.5 / 163.8 / 179).
+// Else K slices for two workgroups a CU (1963 x 4096 with 96 rows of A, 260 workgroups: 32.9 us, in two slices 26.4).  More where A
+// is more than an L2 holds, so that each XCD has some of the slices (us in 1 / 2 / 4 / 8: 1197 x 16384 with 256 rows
+// of three adapters 137 / 91 / 79 / 77, 3553 x 16384 with 96 of 14 206 / 183 / 173 / 150, 2920 x 16384 with 64 of five
+// 181 / 150 / 132 / 138), else of a long K for six workgroups a CU (12139 x 16384 with 24 of one 164 / 131 / 130 / 132).  With
+// K = 2048 they cost more than they give (6208 x 32768 columns, 64 rows of A: 163 / 160 / 172 / 195).
 LoraPlan lora_plan(int64_t m, int64_t per_id, int32_t k, int32_t n, int32_t r, int32_t slices, int32_t adapters, int cus) {
   LoraPlan plan{};
   plan.gather = per_id < kWindow && per_id < m;
@@ -573,8 +577,10 @@ LoraPlan lora_plan(int64_t m, int64_t per_id, int32_t k, int32_t n, int32_t r, i
   const int64_t run = ranks <= 64 ? 1024 : 512;  // columns of a workgroup
   if (ranks * k * 2 <= (128 << 10) && all * ((n + run - 1) / run + slices - 1) <= cus) return plan;
   const int64_t down = all * ((slices * r + 63) / 64);
-  const int64_t fill = std::min<int64_t>({(2 * cus + down - 1) / down, (k + 511) / 512, 8}), even = std::min<int64_t>(k / 8192, (6 * cus + down - 1) / down);
-  plan.ksplit = static_cast<int32_t>(std::max<int64_t>({1, fill, even}));
+  const int64_t fill = std::min<int64_t>({(2 * cus + down - 1) / down, (k + 511) / 512, 8});
+  const int64_t more = static_cast<int64_t>(adapters) * slices * r * k * 2 > (4 << 20) ? std::min<int64_t>(k / 2048, 8)
+                                                                                      : std::min<int64_t>(k / 8192, (6 * cus + down - 1) / down);
+  plan.ksplit = static_cast<int32_t>(std::max<int64_t>({1, fill, more}));
   return plan;
 }
 
@@ -591,7 +597,7 @@ bool lora_grid(LoraParams& p, const LoraPlan& plan) {
   p.runs = static_cast<int32_t>(runs);
   p.h_plane = lora_h_floats(p.m, p.r, p.slices);
   const int64_t all = static_cast<int64_t>(p.units) * p.groups;
-  return all * runs * waves < (1 << 26) && all * 8 < (1 << 26);
+  return all * runs * waves < (1 << 26) && all * std::max(p.ksplit, 1) * 8 < (1 << 26);
 }
 
 hipError_t launch_lora(const LoraParams& p, int elem, hipStream_t stream) {
