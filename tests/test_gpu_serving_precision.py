@@ -1,0 +1,57 @@
+"""How many bits of an fp32 weight the 16-bit serving operators' second products keep, seen where large terms cancel.
+
+Attention.  Of three keys the second cancels the first and the third what its rounding left, so that the output is
+below 2^-14 of the terms and its own rounding does not hide theirs.  A logit is one product, exact, of at
+most 1.  In units of 2^-24: the exponent s = log2(e) z is 0.4 off by the constant and 1 by its rounding, less the
+reference (at most 7 in size) 4, together 5.4 ln 2 = 3.8 of the weight; exp2 2; two parts of fp16 4, three of bf16
+nothing; two additions of three products, truncated at worst, 4.  The sum of the weights scales the small output
+only.
+
+Adapters.  The two ranks of a row are whole numbers of up to 24 bits (fp16: 22), made by two products, and all but
+cancel: every sum is exact in fp32, so that the result is compared bit for bit.
+"""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from pi05_fast import w4a4
+
+pytestmark = pytest.mark.gpu
+TYPES = [torch.float16, torch.bfloat16]
+
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def cancelling(gen, b, d, dtype, device="cuda"):
+    """z [B, 3], v [B, 3, D] in the type, the weighted sum of v and the size of its terms."""
+    z = (torch.rand((b, 3), device=device, generator=gen) * 2 - 1).to(dtype).double()
+    p = torch.softmax(z, -1)[..., None]
+    v = torch.zeros((b, 3, d), dtype=torch.float64, device=device)
+    v[:, 0] = (torch.randn((b, d), device=device, generator=gen) * 64).to(dtype).double()
+    v[:, 1] = (-p[:, 0] * v[:, 0] / p[:, 1]).to(dtype).double()
+    v[:, 2] = (-(p[:, :2] * v[:, :2]).sum(1) / p[:, 2]).to(dtype).double()
+    return z, v, (p * v).sum(1), (p * v.abs()).sum(1)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("b,t,h,kvh,d", [(200, 1, 1, 1, 256), (200, 1, 4, 1, 128), (200, 1, 2, 2, 64), (60, 3, 1, 1, 256), (60, 5, 2, 1, 128),
+                                         (60, 9, 1, 1, 64), (70, 64, 8, 1, 256), (70, 70, 8, 1, 128), (70, 90, 8, 1, 64)])
+def test_attention_weights(cuda, b, t, h, kvh, d, dtype):
+    gen = _gen(b + t + d)
+    z, v, want, size = cancelling(gen, b, d, dtype)
+    cache = w4a4.kv_cache(b, kvh, d, dtype, "cuda")
+    cache[0][:, :, :3, 0] = z.to(dtype)[:, None]
+    cache[1][:, :, :3] = v.to(dtype)[:, None]
+    q = torch.zeros((b, t, h, d), dtype=dtype, device="cuda")
+    q[..., 0] = 1
+    table = torch.arange(b, device="cuda", dtype=torch.int32)[:, None]
+    lens = torch.full((b,), 3, dtype=torch.int32, device="cuda")
+    got = w4a4.kv_attention(q, *cache, table, lens, 1.0, causal=False).double()
+    units = 10.0 if dtype == torch.bfloat16 else 14.0
+    tol = units * 2.0**-24 * size + torch.finfo(dtype).eps / 2 * 1.001 * want.abs() + 2.0**-25
+    over = ((got - want[:, None, None]).abs() / tol[:, None, None]).max().item()
+    assert over <= 1, over
