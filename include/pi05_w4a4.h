@@ -542,7 +542,8 @@ int pi05w4a4_int8_kv_attention(const void* q, const int64_t* q_strides, int32_t 
  *   queries as well.  A query that sees none gets zeros.  What a query does not see has no effect on it, NaN
  *   and infinities too; a NaN or infinity among the values that it sees makes its outputs in that
  *   dimension NaN or infinite.  lse, when not null, fp32 [B, T, H]: the natural log of the sum of
- *   exp(scaling q k) (-inf where none is seen).  Query head h reads KV head h / (H / KVH).  Needs
+ *   exp(scaling q k) (-inf where none is seen).  fp32 with one rounding, but that weights enter the product with the
+ *   values to 2^-22 (and 2^-32 of the row's largest) in fp16, to 2^-24 in bf16.  Query head h reads KV head h / (H / KVH).  Needs
  *   pi05w4a4_kv_attention_workspace_bytes(...) bytes (0 without a split, at most 2^28).  B * T * H <= 2^30.
  *
  * pi05w4a4_lora_add: out[m, n] = y[m, n] + scale[id] * sum_r (sum_k x[m, k] a[id, g r0 + r, k]) b[id, n, r] with
@@ -551,8 +552,9 @@ int pi05w4a4_int8_kv_attention(const void* q, const int64_t* q_strides, int32_t 
  *   contiguous; scale [adapters], null for 1.  ids outside [0, adapters) name no adapter: out = y.  x has row
  *   stride ldx (% 8 == 0, 16-byte aligned), K % 8 == 0, K <= 2^20; y and out have row strides of any size and may
  *   be the same matrix, but must not overlap otherwise, nor x and out.
- *   r % 8 == 0, r <= 128; smaller ranks are padded with zeros.  fp32 with one rounding.  M <= 2^26, N <= 2^22, and no
- *   more waves than a launch holds (2^26; one is 16 rows of an adapter by 128 columns, 64 past rank 64).  Where x A^T is
+ *   r % 8 == 0, r <= 128; smaller ranks are padded with zeros.  fp32 with one rounding, but that x a^T enters the
+ *   second product to 2^-22 in fp16 (to 2^-24 in bf16).  M <= 2^26, N <= 2^22, and no
+ *   more waves than a launch holds (2^26; one is 16 rows of an adapter by 128 columns, 64 past rank 64).  Where x a^T or b is
  *   infinite, outputs may be NaN.
  *   Needs pi05w4a4_lora_workspace_bytes(...) bytes.
  */

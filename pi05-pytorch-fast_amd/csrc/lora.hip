@@ -7,9 +7,10 @@
 //
 // lora_down_kernel: 16 rows x up to 64 rows of A, the K slice of a workgroup over its eight waves, joined
 // in LDS; fp32 sums of each K slice to the workspace.
-// lora_up_kernel: 16 rows x 128 columns a wave.  h is the sum of the K slices in fp32, split into two 16-bit
-// parts whose products with B are summed (fp16: after a shift that brings a row's largest into the upper
-// range, so that no h overflows), so that nothing of h is lost beside the rounding of out.
+// lora_up_kernel: 16 rows x 128 columns a wave.  h is the sum of the K slices in fp32, split into 16-bit parts
+// whose products with B are summed: three of bf16, which hold all of it, or two of fp16, which hold it to 2^-22 and
+// 2^-38 of its row's largest (after a shift that brings that one into the upper range, so that no h overflows).  bf16 in
+// two / three parts, us: 6208 x 32768 of rank 32 159.4 / 160.1, of rank 64 198 / 209, 6208 x 2560 of rank 128 72.6 / 74.0.
 //
 // Rows need no order.  A tile is up to 16 rows of one adapter: 16 consecutive ones of a request of 64 or more, else those
 // of an adapter among 64 consecutive rows, which each workgroup finds by itself (191 rows of 14 adapters, 2048 x 3509: 9.6 us;
@@ -198,10 +199,16 @@ __global__ __launch_bounds__(512) void lora_down_kernel(LoraParams p) {
   }
 }
 
-// The lane's row of h, ranks 32 s + 8 g .. + 7, as two 16-bit parts; returns the factor that takes the products back.
+// 16-bit parts of h.
+template <typename T>
+constexpr int kParts = 2;
+template <>
+constexpr int kParts<__bf16> = 3;
+
+// Brings the lane's row of h, ranks 32 s + 8 g .. + 7, into the range of its parts; returns the factor that takes the products back.
 template <typename T, int KS>
-__device__ __forceinline__ float split_h(const float (&f)[KS][8], vec8<T> (&hi)[KS], vec8<T> (&lo)[KS]) {
-  float shift = 1.0f, unshift = 1.0f;
+__device__ __forceinline__ float shift_h(float (&f)[KS][8]) {
+  float unshift = 1.0f;
   if constexpr (static_cast<float>(static_cast<T>(65536.0f)) > 1e30f) {  // fp16
     float top = 0.0f;
 #pragma unroll
@@ -212,20 +219,17 @@ __device__ __forceinline__ float split_h(const float (&f)[KS][8], vec8<T> (&hi)[
     top = fmaxf(top, __shfl_xor(top, 32, 64));
     // The row's largest to 2^13 .. 2^14; nothing to do for rows of zeros, infinities or NaN.
     const int e = static_cast<int>(__float_as_uint(top) >> 23) - 127;
+    float shift = 1.0f;
     if (top > 0.0f && e < 128) {
       const int by = max(min(13 - e, 126), -126);
       shift = __uint_as_float(static_cast<uint32_t>(127 + by) << 23);
       unshift = __uint_as_float(static_cast<uint32_t>(127 - by) << 23);
     }
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[s][e] *= shift;
   }
-#pragma unroll
-  for (int s = 0; s < KS; ++s)
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float v = f[s][e] * shift;
-      hi[s][e] = static_cast<T>(v);
-      lo[s][e] = static_cast<T>(v - static_cast<float>(hi[s][e]));
-    }
   return unshift;
 }
 
@@ -243,18 +247,28 @@ __device__ __forceinline__ void load_b(const LoraParams& p, int id, int n0, int 
 }
 
 template <typename T, int NT, int KS>
-__device__ __forceinline__ void times_b(const LoraParams& p, const vec8<T> (&w)[NT][KS], const vec8<T> (&hi)[KS],
-                                        const vec8<T> (&lo)[KS], v4f (&acc)[NT]) {
+__device__ __forceinline__ void times_b(const LoraParams& p, const vec8<T> (&w)[NT][KS], const float (&f)[KS][8], v4f (&acc)[NT]) {
   const int g = (threadIdx.x & 63) >> 4;
 #pragma unroll
-  for (int i = 0; i < NT; ++i) {
-    acc[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int i = 0; i < NT; ++i) acc[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
+  for (int s = 0; s < KS; ++s) {
+    vec8<T> h[kParts<T>];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      float v = f[s][e];
+#pragma unroll
+      for (int j = 0; j < kParts<T>; ++j) {
+        h[j][e] = static_cast<T>(v);
+        v -= static_cast<float>(h[j][e]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
       vec8<T> u = to_operand<T>(w[i][s]);
       if (32 * s + 8 * g >= p.r) u = vec8<T>{};
-      acc[i] = mfma(hi[s], u, acc[i]);
-      acc[i] = mfma(lo[s], u, acc[i]);
+#pragma unroll
+      for (int j = 0; j < kParts<T>; ++j) acc[i] = mfma(h[j], u, acc[i]);
     }
   }
 }
@@ -371,7 +385,6 @@ __global__ __launch_bounds__(256, KS == 1 ? 4 : 3) void lora_up_kernel(LoraParam
   vec8<T> w[NT][KS];
   load_b<T, NT, KS>(p, id, n0, end, w);
 
-  vec8<T> hi[KS], lo[KS];
   float f[KS][8];
 #pragma unroll
   for (int s = 0; s < KS; ++s)
@@ -395,11 +408,11 @@ __global__ __launch_bounds__(256, KS == 1 ? 4 : 3) void lora_up_kernel(LoraParam
 #pragma unroll
       for (int e = 0; e < 8; ++e) f[s][e] = 0.0f;
     }
-  const float unshift = split_h<T, KS>(f, hi, lo);
+  const float unshift = shift_h<T, KS>(f);
   // What the lane ends with are rows 4 g + r, whose factors are in other lanes.
 #pragma unroll
   for (int r = 0; r < 4; ++r) back[r] = __shfl(unshift, 4 * g + r, 64);
-  times_b<T, NT, KS>(p, w, hi, lo, acc);
+  times_b<T, NT, KS>(p, w, f, acc);
   store_rows<T, NT>(p, tile.row0, row, tile.n - 4 * g, nc, end, whole, tile.id, back, scale, acc, y);
 }
 
@@ -499,17 +512,16 @@ __global__ __launch_bounds__(512) void lora_fused_kernel(LoraParams p) {
     __syncthreads();
     if (columns) {
       float f[KS][8];
-      vec8<T> hi[KS], lo[KS];
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
         const v4f a = *reinterpret_cast<const v4f*>(hs + s * 512 + lane * 8), b = *reinterpret_cast<const v4f*>(hs + s * 512 + lane * 8 + 4);
 #pragma unroll
         for (int e = 0; e < 8; ++e) f[s][e] = 32 * s + 8 * g >= p.r ? 0.0f : e < 4 ? a[e & 3] : b[e & 3];
       }
-      const float unshift = split_h<T, KS>(f, hi, lo);
+      const float unshift = shift_h<T, KS>(f);
 #pragma unroll
       for (int r = 0; r < 4; ++r) back[r] = __shfl(unshift, 4 * g + r, 64);
-      times_b<T, NT, KS>(p, w, hi, lo, out);
+      times_b<T, NT, KS>(p, w, f, out);
     }
   }
   if (columns) store_rows<T, NT>(p, tile.row0, row, tile.n - 4 * g, nc, end, whole, id, back, scale, out, y);

@@ -168,7 +168,7 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
     8), a [adapters, R, K], b [adapters, N, R] (R a multiple of 8 of at most 128; smaller ranks are
     padded with zeros), ids int32 of the first dimensions of the rows ([B] for one adapter a request, or
     one for each row), scale fp32 [adapters] (None: 1).  Ids outside [0, adapters) name no adapter: those
-    rows are y.  Sums are fp32, with one rounding.
+    rows are y.  Sums are fp32, with one rounding; the first one's enter the second product to 2^-22 in fp16, whole in bf16.
 
     ``slices`` (up to four widths, their sum N) are the parts of a joined projection, which have first
     factors of their own: a is then [adapters, len(slices) * R, K], part g's rows g R .. g R + R - 1, and

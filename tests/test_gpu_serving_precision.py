@@ -55,3 +55,41 @@ def test_attention_weights(cuda, b, t, h, kvh, d, dtype):
     tol = units * 2.0**-24 * size + torch.finfo(dtype).eps / 2 * 1.001 * want.abs() + 2.0**-25
     over = ((got - want[:, None, None]).abs() / tol[:, None, None]).max().item()
     assert over <= 1, over
+
+
+def _far_sums(gen, m, k, dtype):
+    """x [M, K] and, for one adapter a row, the first factors of two ranks [M, K] with whole sums of up to 24 (fp16: 22) bits
+    that are less than 100 apart; the sums."""
+    bits, parts = (8, 3) if dtype == torch.bfloat16 else (11, 2)
+    top = 1 << (bits * parts)
+    h0 = torch.randint(top // 2, top - 200, (m,), device="cuda", generator=gen)
+    h1 = h0 + torch.randint(-100, 101, (m,), device="cuda", generator=gen)
+    at = torch.randperm(k, device="cuda", generator=gen)[:parts]
+    x = torch.zeros((m, k), device="cuda")
+    a = torch.zeros((m, 2, k), device="cuda")
+    for i in range(parts):
+        x[:, at[i]] = float(1 << (bits * i))
+        for j, h in enumerate((h0, h1)):
+            a[:, j, at[i]] = ((h >> (bits * i)) & ((1 << bits) - 1)).float()
+    return x.to(dtype), a.to(dtype), h0 - h1
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("per_id", [1, 5, 70])
+@pytest.mark.parametrize("r,k,n", [(8, 64, 40), (24, 104, 130), (64, 128, 300), (128, 64, 96), (8, 16384, 64), (24, 4096, 257), (64, 2048, 130),
+                                   (128, 2048, 70)])
+def test_sums_of_adapters(cuda, r, k, n, per_id, dtype):
+    """In one launch (the first four) and in two."""
+    gen = _gen(r + k + n + per_id)
+    count = 9
+    x, two, apart = _far_sums(gen, count, k, dtype)
+    a = torch.zeros((count, r, k), dtype=dtype, device="cuda")
+    b = torch.zeros((count, n, r), dtype=dtype, device="cuda")
+    i, j = (0, r - 1) if per_id == 1 else (r // 2, r // 2 + 1)
+    a[:, i], a[:, j], b[:, :, i], b[:, :, j] = two[:, 0], two[:, 1], 1, -1
+    ids = torch.randperm(count, device="cuda", generator=gen)
+    rows = ids.repeat_interleave(per_id)
+    y = torch.randint(-100, 101, (count * per_id, n), device="cuda", generator=gen).to(dtype)
+    want = (y.float() + apart[rows, None]).to(dtype)
+    got = w4a4.lora_add(y.view(count, per_id, n), x[rows].view(count, per_id, k), a, b, ids.to(torch.int32))
+    assert torch.equal(got.view(-1, n), want)
