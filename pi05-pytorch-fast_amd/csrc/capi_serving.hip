@@ -259,6 +259,8 @@ extern "C" int pi05w4a4_kv_attention(const void* q, const int64_t* q_strides, in
   p.lse = lse;
   p.ws = static_cast<float*>(workspace);
   p.scaling = scaling;
+  p.down = kv_attn16_down(elem, table_pages);
+  p.up = 1.0f / p.down;
   p.causal = causal != 0;
   p.b = b;
   p.t = t;

@@ -55,6 +55,7 @@ struct KvAttn16Params {
   float* lse;             // [B, T, H] or null
   float* ws;              // partial results when nsplit > 1
   float scaling;
+  float down, up;         // factor of the softmax weights and its inverse, powers of two (fp16: 1)
   int32_t causal;
   int32_t b, t, h;
   int32_t nsplit;         // runs of pages of a sequence
@@ -67,6 +68,7 @@ struct KvAttn16Plan {
   bool wide;
 };
 KvAttn16Plan kv_attn16_plan(int64_t b, int64_t t, int32_t h, int32_t kvh, int32_t d, int64_t table_pages, int cus);
+float kv_attn16_down(int elem, int64_t table_pages);
 size_t kv_attn16_workspace(int64_t b, int64_t t, int32_t h, int32_t d, int nsplit);
 hipError_t launch_kv_attn16(const KvAttn16Params& p, int elem, hipStream_t stream);
 

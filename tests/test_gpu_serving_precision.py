@@ -93,3 +93,20 @@ def test_sums_of_adapters(cuda, r, k, n, per_id, dtype):
     want = (y.float() + apart[rows, None]).to(dtype)
     got = w4a4.lora_add(y.view(count, per_id, n), x[rows].view(count, per_id, k), a, b, ids.to(torch.int32))
     assert torch.equal(got.view(-1, n), want)
+
+
+@pytest.mark.parametrize("b,t,h,kvh,d,pages", [(3, 1, 8, 1, 256, 3), (2, 1, 4, 1, 128, 40), (40, 1, 4, 2, 64, 2), (3, 9, 4, 1, 256, 3),
+                                               (3, 20, 2, 1, 64, 4), (6, 110, 8, 1, 256, 5), (12, 97, 8, 2, 128, 5), (70, 70, 3, 1, 64, 5)])
+def test_values_at_the_end_of_the_range(cuda, b, t, h, kvh, d, pages):
+    """bf16 values of nearly fp32's largest number, of one sign and of both: their mean is as large at most."""
+    from test_gpu_kv import _check, _pool
+
+    gen = _gen(b + t + d)
+    cache, table = _pool(gen, b, pages, kvh, d, torch.bfloat16)
+    q = (torch.randn((b, t, h, d), device="cuda", generator=gen) * 3).bfloat16()
+    lens = torch.randint(1, pages * 64 + 1, (b,), device="cuda", generator=gen).tolist()
+    lens[0] = pages * 64
+    for v in (torch.full_like(cache[1], torch.finfo(torch.bfloat16).max), (torch.rand(cache[1].shape, device="cuda", generator=gen) * 3.3e38).bfloat16(),
+              cache[1].sign() * 3e38):
+        _check(q, [cache[0], v.bfloat16()], table, lens, d**-0.5, causal=False)
+        _check(q, [cache[0], v.bfloat16()], table, lens, d**-0.5)
