@@ -1464,13 +1464,16 @@ _register_custom_op()
 # several per decoder layer) when nothing needs it: plain tensors, no autograd graph to
 # record, no Dynamo trace, no torch.jit.trace (whose graph only sees dispatched ops), no
 # dispatch or function mode, no function transform (vmap calls the dispatched op once a
-# sample).  The direct and the dispatched route run the same implementation.
+# sample).  The direct and the dispatched route run the same implementation; a call that
+# writes into arguments counts that as a change of them (``_changed``), as the dispatcher
+# does, so that a backward pass which saved one raises.
 _is_compiling = torch.compiler.is_compiling
 _jit_tracing = torch._C._get_tracing_state
 _dispatch_modes = torch._C._len_torch_dispatch_stack
 _function_modes = torch._C._is_torch_function_mode_enabled
 _transforms = torch._C._functorch.peek_interpreter_stack
 _PLAIN = (torch.Tensor, torch.nn.Parameter)
+_changed = torch.autograd.graph.increment_version
 
 
 def _refuse_tangents(*ts) -> None:

@@ -16,7 +16,7 @@ from collections.abc import Sequence
 import torch
 
 from pi05_fast.w4a4 import extension as _ext
-from pi05_fast.w4a4.extension import (_check, _direct, _on_device, _ptr, _refuse_gradients, _refuse_tangents, _stream,
+from pi05_fast.w4a4.extension import (_changed, _check, _direct, _on_device, _ptr, _refuse_gradients, _refuse_tangents, _stream,
                                       _workspace, load_int4_gemm)
 from pi05_fast.w4a4.int8 import ELEM
 from pi05_fast.w4a4.kv_int8 import HEAD_DIMS, MAX_BATCH, MAX_TOKENS, PAGE_TOKENS, _ints
@@ -260,7 +260,8 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
     shared between sequences; a row may be written from one place of a call only.  k and v must not lie
     in the cache.  There are no derivatives: arguments that require gradients are refused."""
     if _direct(k, v, k_cache, v_cache, block_table, lens, counts):
-        return _append_impl(k, v, k_cache, v_cache, block_table, lens, counts)
+        _append_impl(k, v, k_cache, v_cache, block_table, lens, counts)
+        return _changed((k_cache, v_cache))
     _refuse_gradients("kv_append", k, v, k_cache, v_cache)
     return torch.ops.pi05_w4a4.kv_append(k, v, k_cache, v_cache, block_table, lens, counts)
 
@@ -276,8 +277,10 @@ def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_wei
     values go into the cache up to ``counts``.  There are no derivatives: arguments that require
     gradients are refused."""
     if _direct(q, k, v, q_weight, k_weight, positions, inv_freq, k_cache, v_cache, block_table, lens, counts):
-        return _rope_append_impl(q, k, v, q_weight, k_weight, float(eps), positions, inv_freq, k_cache, v_cache, block_table, lens,
-                                 counts, bool(unit_offset), bool(interleaved), axes)
+        q_out = _rope_append_impl(q, k, v, q_weight, k_weight, float(eps), positions, inv_freq, k_cache, v_cache, block_table, lens,
+                                  counts, bool(unit_offset), bool(interleaved), axes)
+        _changed((k_cache, v_cache))
+        return q_out
     _refuse_gradients("qk_norm_rope_append", q, k, v, q_weight, k_weight, inv_freq, k_cache, v_cache)
     return torch.ops.pi05_w4a4.qk_norm_rope_append(q, k, v, q_weight, k_weight, float(eps), positions, inv_freq, k_cache, v_cache,
                                                    block_table, lens, counts, bool(unit_offset), bool(interleaved),

@@ -22,7 +22,7 @@ import ctypes
 import torch
 
 from pi05_fast.w4a4 import extension as _ext
-from pi05_fast.w4a4.extension import (_check, _direct, _on_device, _ptr, _refuse_tangents, _stream, _workspace,
+from pi05_fast.w4a4.extension import (_changed, _check, _direct, _on_device, _ptr, _refuse_tangents, _stream, _workspace,
                                       load_int4_gemm)
 from pi05_fast.w4a4.int8 import ELEM
 
@@ -220,7 +220,8 @@ def int8_kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_ca
     dropped.  A call may write a page from one place only: full pages can be shared between
     sequences, and stand in a table twice, a page that still fills cannot."""
     if _direct(k, v, k_cache, v_cache, k_scale, v_scale, block_table, lens, counts):
-        return _append_impl(k, v, k_cache, v_cache, k_scale, v_scale, block_table, lens, counts)
+        _append_impl(k, v, k_cache, v_cache, k_scale, v_scale, block_table, lens, counts)
+        return _changed((k_cache, v_cache, k_scale, v_scale))
     return torch.ops.pi05_w4a4.int8_kv_append(k, v, k_cache, v_cache, k_scale, v_scale, block_table, lens, counts)
 
 

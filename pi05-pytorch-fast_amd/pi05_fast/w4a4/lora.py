@@ -13,7 +13,7 @@ from collections.abc import Sequence
 import torch
 
 from pi05_fast.w4a4 import extension as _ext
-from pi05_fast.w4a4.extension import (_check, _direct, _on_device, _ptr, _refuse_gradients, _refuse_tangents, _stream,
+from pi05_fast.w4a4.extension import (_changed, _check, _direct, _on_device, _ptr, _refuse_gradients, _refuse_tangents, _stream,
                                       _workspace, load_int4_gemm)
 from pi05_fast.w4a4.int8 import ELEM
 from pi05_fast.w4a4.rope import _meta, _plan
@@ -183,7 +183,9 @@ def lora_add_(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor
     """``lora_add`` into y, which may be a part of a wider output (rows at one stride), and y.  Rows without an
     adapter are not touched.  An x in the same memory is copied first.  Arguments that require gradients are refused."""
     if _direct(y, x, a, b, ids, scale):
-        return _lora_impl(y, x, a, b, ids, scale, slices, True)
+        _lora_impl(y, x, a, b, ids, scale, slices, True)
+        _changed(y)
+        return y
     _refuse_gradients("lora_add_", y, x, a, b, scale)
     torch.ops.pi05_w4a4.lora_add_(y, x, a, b, ids, scale, None if slices is None else list(slices))
     return y
