@@ -556,7 +556,8 @@ int pi05w4a4_int8_kv_attention(const void* q, const int64_t* q_strides, int32_t 
  *   second product to 2^-22 in fp16 (to 2^-24 in bf16).  M <= 2^26, N <= 2^22, and no
  *   more waves than a launch holds (2^26; one is 16 rows of an adapter by 128 columns, 64 past rank 64).  Where x a^T or b is
  *   infinite, outputs may be NaN.
- *   Needs pi05w4a4_lora_workspace_bytes(...) bytes.
+ *   Needs pi05w4a4_lora_workspace_bytes(...) bytes: none for few rows, else the fp32 sums x a^T, slices * r rounded up to
+ *   32 a row, for each part of K that is summed by itself (several parts: at most 2^28 bytes together).
  */
 int pi05w4a4_qk_norm_rope(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, int32_t elem,
                           int32_t b, int32_t t, int32_t h, int32_t kvh, int32_t d, const void* q_weight,

@@ -559,6 +559,8 @@ void launch(const LoraParams& p, hipStream_t stream) {
 
 int64_t lora_h_floats(int64_t m, int32_t r, int32_t slices) { return (m + 15) / 16 * slices * ((r + 31) / 32) * 512; }
 
+constexpr int64_t kMaxPartial = int64_t{1} << 28;
+
 // Tiles of consecutive rows where requests have 64 or more (or there is one).  Else windows: as many workgroups as a window
 // can have tiles, found by counting; past 32 one for each row, the first row of a tile its workgroup's, which costs
 // nothing to find.  One launch (ksplit 0) where its workgroups have a CU each and the ranks that each reads again
@@ -567,7 +569,11 @@ int64_t lora_h_floats(int64_t m, int32_t r, int32_t slices) { return (m + 15) / 
 // is more than an L2 holds, so that each XCD has some of the slices (us in 1 / 2 / 4 / 8: 1197 x 16384 with 256 rows
 // of three adapters 137 / 91 / 79 / 77, 3553 x 16384 with 96 of 14 206 / 183 / 173 / 150, 2920 x 16384 with 64 of five
 // 181 / 150 / 132 / 138), else of a long K for six workgroups a CU (12139 x 16384 with 24 of one 164 / 131 / 130 / 132).  With
-// K = 2048 they cost more than they give (6208 x 32768 columns, 64 rows of A: 163 / 160 / 172 / 195).
+// K = 2048 they cost more than they give (6208 x 32768 columns, 64 rows of A: 163 / 160 / 172 / 195).  Where rows alone
+// give four workgroups a CU, two at most, for every wave of the second launch reads all planes of h (16384 x 16384 with 64
+// of five 277 / 246 / 259 / 272, 65536 x 16384 with 32 of eight 1301 / 1279 / 1377 / 1539, 4096 x 4096 with 384 of eight 95 / 89
+// / 90 / 119), past eight those of a long K only (65536 x 4096 with 64 of 16 443 / 466 / 527 / 685); and no planes of more than
+// kMaxPartial together.
 LoraPlan lora_plan(int64_t m, int64_t per_id, int32_t k, int32_t n, int32_t r, int32_t slices, int32_t adapters, int cus) {
   LoraPlan plan{};
   plan.gather = per_id < kWindow && per_id < m;
@@ -590,9 +596,11 @@ LoraPlan lora_plan(int64_t m, int64_t per_id, int32_t k, int32_t n, int32_t r, i
   if (ranks * k * 2 <= (128 << 10) && all * ((n + run - 1) / run + slices - 1) <= cus) return plan;
   const int64_t down = all * ((slices * r + 63) / 64);
   const int64_t fill = std::min<int64_t>({(2 * cus + down - 1) / down, (k + 511) / 512, 8});
-  const int64_t more = static_cast<int64_t>(adapters) * slices * r * k * 2 > (4 << 20) ? std::min<int64_t>(k / 2048, 8)
+  const int64_t far = down < 4 * cus ? std::min<int64_t>(k / 2048, 8) : std::min<int64_t>(k / (down < 8 * cus ? 2048 : 8192), 2);
+  const int64_t more = static_cast<int64_t>(adapters) * slices * r * k * 2 > (4 << 20) ? far
                                                                                       : std::min<int64_t>(k / 8192, (6 * cus + down - 1) / down);
-  plan.ksplit = static_cast<int32_t>(std::max<int64_t>({1, fill, more}));
+  const int64_t most = kMaxPartial / (4 * lora_h_floats(m, r, slices));
+  plan.ksplit = static_cast<int32_t>(std::max<int64_t>(1, std::min(std::max(fill, more), most)));
   return plan;
 }
 
