@@ -553,9 +553,9 @@ int pi05w4a4_int8_kv_attention(const void* q, const int64_t* q_strides, int32_t 
  *   stride ldx (% 8 == 0, 16-byte aligned), K % 8 == 0, K <= 2^20; y and out have row strides of any size and may
  *   be the same matrix, but must not overlap otherwise, nor x and out.
  *   r % 8 == 0, r <= 128; smaller ranks are padded with zeros.  fp32 with one rounding, but that x a^T enters the
- *   second product to 2^-22 in fp16 (to 2^-24 in bf16).  M <= 2^26, N <= 2^22, and no
- *   more waves than a launch holds (2^26; one is 16 rows of an adapter by 128 columns, 64 past rank 64).  Where x a^T or b is
- *   infinite, outputs may be NaN.
+ *   second product to 2^-22 in fp16 (to 2^-24 in bf16).  M <= 2^26, N <= 2^22, and fewer than
+ *   2^26 tiles of 16 rows by 128 columns (64 past rank 64; a slice's columns count as whole groups of four tiles).
+ *   Where x a^T or b is infinite, outputs may be NaN.
  *   Needs pi05w4a4_lora_workspace_bytes(...) bytes: none for few rows, else the fp32 sums x a^T, slices * r rounded up to
  *   32 a row, for each part of K that is summed by itself (several parts: at most 2^28 bytes together).
  */

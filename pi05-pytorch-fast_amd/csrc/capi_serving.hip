@@ -329,7 +329,7 @@ extern "C" int pi05w4a4_lora_add(const void* y, int64_t ldy, const void* x, int6
   p.r = r;
   p.slices = slices;
   p.per_id = per_id;
-  if (!lora_grid(p, plan)) return capi_fail(PI05W4A4_EINVAL, "%lld rows of %d columns are more than one launch holds", (long long)m, n);
+  if (!lora_grid(p, plan)) return capi_fail(PI05W4A4_EINVAL, "tiles of %lld rows by %d columns are more waves than one launch holds", (long long)m, n);
   const size_t need = adapters > 0 ? lora_workspace(m, r, slices, plan.ksplit) : 0;
   if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned(workspace, 16)))
     return capi_fail(PI05W4A4_EWORKSPACE, "lora_add needs a 16-byte aligned workspace of %zu bytes, got %zu", need, workspace_bytes);

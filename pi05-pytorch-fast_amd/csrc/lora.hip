@@ -135,7 +135,7 @@ __global__ __launch_bounds__(512) void lora_down_kernel(LoraParams p) {
   Tile<GATHER> tile;
   // The K slices are the fastest: workgroups whose numbers are equal mod 8 share an XCD, whose L2 then holds its slices of A.
   const int place = blockIdx.x / p.ksplit, kslice = blockIdx.x - place * p.ksplit;
-  if (!find_tile(p, place / p.groups, place % p.groups, false, tile) || !tile.known(p, false)) return;
+  if (!find_tile(p, p.unit0 + place / p.groups, place % p.groups, false, tile) || !tile.known(p, false)) return;
   const int total = p.slices * p.r;  // rows of an adapter's A
   const int rank0 = blockIdx.y * 16 * NR;
   const int chunks = (p.k + 31) / 32;
@@ -349,7 +349,7 @@ __global__ __launch_bounds__(256, KS == 1 ? 4 : 3) void lora_up_kernel(LoraParam
   const bool in_place = p.out == p.y && p.ldo == p.ldy;
 
   Tile<GATHER> tile;
-  if (!find_tile(p, rest / p.groups, rest % p.groups, !in_place, tile)) return;
+  if (!find_tile(p, p.unit0 + rest / p.groups, rest % p.groups, !in_place, tile)) return;
   int row[4];
 #pragma unroll
   for (int r = 0; r < 4; ++r) row[r] = tile.row(4 * g + r);
@@ -445,7 +445,7 @@ __global__ __launch_bounds__(512) void lora_fused_kernel(LoraParams p) {
   const bool whole = n0 + C <= end;  // uniform
   const bool in_place = p.out == p.y && p.ldo == p.ldy;
   Tile<GATHER> tile;
-  if (!find_tile(p, rest / p.groups, rest % p.groups, !in_place, tile)) return;
+  if (!find_tile(p, p.unit0 + rest / p.groups, rest % p.groups, !in_place, tile)) return;
   int row[4];
 #pragma unroll
   for (int r = 0; r < 4; ++r) row[r] = tile.row(4 * g + r);
@@ -528,8 +528,8 @@ __global__ __launch_bounds__(512) void lora_fused_kernel(LoraParams p) {
 }
 
 template <typename T, bool GATHER>
-void launch_down(const LoraParams& p, hipStream_t stream) {
-  const unsigned tiles = static_cast<unsigned>(p.units) * p.groups * p.ksplit;
+void launch_down(const LoraParams& p, int units, hipStream_t stream) {
+  const unsigned tiles = static_cast<unsigned>(units) * p.groups * p.ksplit;
   const int total = p.slices * p.r;
   if (total <= 16)
     lora_down_kernel<T, 1, GATHER><<<tiles, 512, 0, stream>>>(p);
@@ -540,8 +540,8 @@ void launch_down(const LoraParams& p, hipStream_t stream) {
 }
 
 template <typename T, bool GATHER>
-void launch(const LoraParams& p, hipStream_t stream) {
-  const dim3 grid(static_cast<unsigned>(p.units) * p.groups * p.runs);
+void launch_units(const LoraParams& p, int units, hipStream_t stream) {
+  const dim3 grid(static_cast<unsigned>(units) * p.groups * p.runs);
   if (p.ksplit == 0) {
     if (p.r <= 16) lora_fused_kernel<T, 1, GATHER><<<grid, 512, 0, stream>>>(p);
     else if (p.r <= 32) lora_fused_kernel<T, 2, GATHER><<<grid, 512, 0, stream>>>(p);
@@ -549,10 +549,25 @@ void launch(const LoraParams& p, hipStream_t stream) {
     else lora_fused_kernel<T, 8, GATHER><<<grid, 512, 0, stream>>>(p);
     return;
   }
-  if (p.adapters > 0) launch_down<T, GATHER>(p, stream);
+  if (p.adapters > 0) launch_down<T, GATHER>(p, units, stream);
   if (p.r <= 32) lora_up_kernel<T, 1, GATHER><<<grid, 256, 0, stream>>>(p);
   else if (p.r <= 64) lora_up_kernel<T, 2, GATHER><<<grid, 256, 0, stream>>>(p);
   else lora_up_kernel<T, 4, GATHER><<<grid, 256, 0, stream>>>(p);
+}
+
+// A launch holds fewer than 2^32 threads.
+constexpr int64_t kMaxWaves = 1 << 26;
+
+// As many units at a time as a launch holds: all of them, but for windows of many adapters over very many rows, whose
+// workgroups are up to 16 times those of whole tiles (a window's are 2^21 waves at most).
+template <typename T, bool GATHER>
+void launch(LoraParams p, hipStream_t stream) {
+  const int64_t waves = p.groups * std::max<int64_t>(p.runs * (p.ksplit == 0 ? 8 : 4), p.ksplit * 8);
+  const int64_t fit = (kMaxWaves - 1) / waves;
+  for (int64_t at = 0; at < p.units; at += fit) {
+    p.unit0 = static_cast<int32_t>(at);
+    launch_units<T, GATHER>(p, static_cast<int>(std::min<int64_t>(fit, p.units - at)), stream);
+  }
 }
 
 }  // namespace
@@ -616,8 +631,7 @@ bool lora_grid(LoraParams& p, const LoraPlan& plan) {
   for (int s = 0; s < p.slices; ++s) runs += (p.width[s] + columns - 1) / columns;
   p.runs = static_cast<int32_t>(runs);
   p.h_plane = lora_h_floats(p.m, p.r, p.slices);
-  const int64_t all = static_cast<int64_t>(p.units) * p.groups;
-  return all * runs * waves < (1 << 26) && all * std::max(p.ksplit, 1) * 8 < (1 << 26);
+  return (p.m + 15) / 16 * runs * waves < kMaxWaves;
 }
 
 hipError_t launch_lora(const LoraParams& p, int elem, hipStream_t stream) {

@@ -89,6 +89,7 @@ struct LoraParams {
   int32_t width[kLoraSlices];  // columns of each slice
   int32_t ksplit;      // K slices of the first launch; 0: both products in one
   int32_t units;       // 16-row tiles of requests, or windows of rows
+  int32_t unit0;       // the first one of a launch
   int32_t groups;      // workgroups of a window: its tiles at most
   int32_t tiles;       // of a request
   int32_t gather;      // windows
@@ -102,7 +103,7 @@ struct LoraPlan {
 };
 LoraPlan lora_plan(int64_t m, int64_t per_id, int32_t k, int32_t n, int32_t r, int32_t slices, int32_t adapters, int cus);
 int64_t lora_h_floats(int64_t m, int32_t r, int32_t slices);
-// What of a call follows from its plan; false: its waves are more than one launch holds.
+// What of a call follows from its plan; false: whole tiles of its rows are more waves than one launch holds.
 bool lora_grid(LoraParams& p, const LoraPlan& plan);
 hipError_t launch_lora(const LoraParams& p, int elem, hipStream_t stream);
 

@@ -34,3 +34,19 @@ def test_sums_of_many_rows(lib, m, per_id, k, r, slices, adapters):
 @pytest.mark.parametrize("k,r,slices,adapters", [(16384, 128, 4, 4), (16384, 8, 4, 300), (1 << 20, 128, 1, 2)])
 def test_sums_of_few_rows(lib, m, k, r, slices, adapters):
     assert lib.pi05w4a4_lora_workspace_bytes(m, 1, k, 2560, r, slices, adapters) <= 1 << 27
+
+
+def _lora(lib, m, per_id, n, r=16, adapters=64, y=vp(1 << 45), x=vp(1 << 46), ldx=64, out=vp(1 << 44), ldy=None, ldo=None, ws=None):
+    return lib.pi05w4a4_lora_add(y, n if ldy is None else ldy, x, ldx, m, 64, vp(4096), vp(4096), None, adapters, r, vp(4096), per_id, n, 1, None, 0, out,
+                                 n if ldo is None else ldo, ws, 0, None)
+
+
+@pytest.mark.parametrize("m,per_id,n,r", [(1 << 19, 1, 1 << 14, 16), (1 << 18, 1, (1 << 14) + 8, 72), (1 << 22, 3, 1 << 10, 16), (1 << 26, 65, 512, 16)])
+def test_adapters_by_rows_have_the_limit_of_whole_tiles(lib, m, per_id, n, r):
+    """Windows of many adapters, and requests that end inside a tile, need more workgroups than rows / 16: several launches."""
+    assert _lora(lib, m, per_id, n, r) == 3 and b"workspace" in lib.pi05w4a4_last_error()
+
+
+@pytest.mark.parametrize("m,per_id,n,r", [(1 << 26, 1, 1 << 12, 16), (1 << 26, 3, (1 << 11) + 1, 8), (1 << 20, 1, 1 << 17, 72), (1 << 26, 1 << 26, 1 << 12, 16)])
+def test_more_tiles_than_a_launch_holds(lib, m, per_id, n, r):
+    assert _lora(lib, m, per_id, n, r) == 1 and b"one launch" in lib.pi05w4a4_last_error()
