@@ -522,10 +522,11 @@ int pi05w4a4_int8_kv_attention(const void* q, const int64_t* q_strides, int32_t 
  *     f = x * g / sqrt(mean_d(x^2) + eps), g = 1 + w (unit_offset) or w, or f = x where the weight is null;
  *     pair j < rot / 2 is dimensions (j, j + rot / 2), or (2j, 2j + 1) when interleaved, and turns by
  *     pos * inv_freq[j]: (f1 c - f2 s, f2 c + f1 s); dimensions from rot on stay f.
- *   A call of more than 2^26 waves, each three times 1024 / D heads of a token, is refused.  rot % 16 == 0 (0: no
- *   rotation).  Positions are [axes, B, T] of int32 or int64 (pos_bytes 4 or 8), with strides
- *   {axis, batch, token} in elements; axis_of_pair (host, rot / 2 bytes; null: all 0) names the axis of each
- *   pair, at most 4 axes.  fp32 with one rounding; angles are reduced in 64 bits.
+ *   A wave takes up to three rounds of 1024 / D heads of a token (D rounded up to a power of two), fewer where tokens
+ *   are few; a call of more than 2^26 - 4 waves is refused.  rot % 16 == 0 (0: no rotation).  Positions are
+ *   [axes, B, T] of int32 or int64 (pos_bytes 4 or 8), with strides {axis, batch, token} in elements; axis_of_pair
+ *   (host, rot / 2 bytes; null: all 0) names the axis of each pair, at most 4 axes.  fp32 with one rounding; angles
+ *   are reduced in 64 bits.
  *
  * KV cache: pages of 64 tokens, k_cache and v_cache [pages, KVH, 64, D]; D is 64, 128 or 256.  Token i of sequence
  *   b is row i % 64 of page table[b * table_stride + i / 64].  Table entries outside [0, pages) name no

@@ -83,8 +83,8 @@ static int check_apart(const HeadRopeParams& p) {
 
 static int run_head_rope(HeadRopeParams& p, int32_t elem, void* stream, const char* what) {
   p.parts = head_rope_parts(p, device_cu_count());
-  // A launch holds fewer than 2^32 threads: a wave for each part of a token.
-  if (static_cast<int64_t>(p.b) * p.t * p.parts >= (1 << 26))
+  // A launch holds fewer than 2^32 threads: a wave for each part of a token, four a workgroup.
+  if (static_cast<int64_t>(p.b) * p.t * p.parts > (1 << 26) - 4)
     return capi_fail(PI05W4A4_EINVAL, "%d x %d tokens of %d heads are more than one launch holds", p.b, p.t,
                      p.heads[0] + p.heads[1] + p.heads[2]);
   if (p.c.lens != nullptr)

@@ -50,3 +50,12 @@ def test_adapters_by_rows_have_the_limit_of_whole_tiles(lib, m, per_id, n, r):
 @pytest.mark.parametrize("m,per_id,n,r", [(1 << 26, 1, 1 << 12, 16), (1 << 26, 3, (1 << 11) + 1, 8), (1 << 20, 1, 1 << 17, 72), (1 << 26, 1 << 26, 1 << 12, 16)])
 def test_more_tiles_than_a_launch_holds(lib, m, per_id, n, r):
     assert _lora(lib, m, per_id, n, r) == 1 and b"one launch" in lib.pi05w4a4_last_error()
+
+
+def test_heads_of_just_too_many_waves(lib):
+    """8191 tokens in 8193 parts are 2^26 - 1 waves: in workgroups of four, 2^32 threads."""
+    i3 = ctypes.c_int64 * 3
+    q, pos, out = vp(1 << 20), vp(4096), vp(1 << 21)
+    rc = lib.pi05w4a4_qk_norm_rope(q, i3(512, 512, 512), q, i3(512, 512, 512), 0, 1, 8191, 32767, 16389, 512, None, None, 1e-6, 1, pos,
+                                   i3(0, 1, 1), 4, 1, None, pos, 512, 0, out, out, None)
+    assert rc == 1 and b"one launch" in lib.pi05w4a4_last_error()
