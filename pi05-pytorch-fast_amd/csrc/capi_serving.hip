@@ -324,6 +324,8 @@ extern "C" int pi05w4a4_lora_add(const void* y, int64_t ldy, const void* x, int6
   if (ldx < 0 || ldx % 8 != 0) return capi_fail(PI05W4A4_EINVAL, "the row stride of x must be a multiple of 8 elements, got %lld", (long long)ldx);
   if (ldy < 0 || ldo < n) return capi_fail(PI05W4A4_EINVAL, "row strides must be >= 0, and those of the output >= N");
   if (rows_overlap(x, ldx, k, out, ldo, n, m)) return capi_fail(PI05W4A4_EINVAL, "x must not overlap the output");
+  if (!(y == out && (ldy == ldo || m == 1)) && rows_overlap(y, ldy, n, out, ldo, n, m))
+    return capi_fail(PI05W4A4_EINVAL, "y must be the output or not overlap it");
   const LoraPlan plan = lora_plan(m, per_id, k, n, r, slices, adapters, device_cu_count());
   p.m = m;
   p.r = r;

@@ -59,3 +59,16 @@ def test_heads_of_just_too_many_waves(lib):
     rc = lib.pi05w4a4_qk_norm_rope(q, i3(512, 512, 512), q, i3(512, 512, 512), 0, 1, 8191, 32767, 16389, 512, None, None, 1e-6, 1, pos,
                                    i3(0, 1, 1), 4, 1, None, pos, 512, 0, out, out, None)
     assert rc == 1 and b"one launch" in lib.pi05w4a4_last_error()
+
+
+@pytest.mark.parametrize("m,ldy,ldo,at,refused", [
+    (2, 32, 32, 0, False), (1, 40, 32, 0, False),  # the output itself
+    (2, 40, 32, 0, True), (2, 32, 40, 0, True), (2, 0, 32, 0, True), (1, 32, 32, 2, True), (2, 32, 32, -2, True), (3, 80, 80, 62, True),
+    (3, 80, 80, 64, False), (3, 80, 80, -64, False), (3, 80, 80, 160 - 62, True), (2, 32, 32, 128, False), (2, 32, 32, 126, True), (2, 64, 32, -192, False),
+])
+def test_adapters_read_y_before_they_write_it(lib, m, ldy, ldo, at, refused):
+    """y is the output's rows, or apart from them; beside them in wider rows it is apart, and the call fails for its workspace only."""
+    rc = lib.pi05w4a4_lora_add(vp((1 << 20) + at), ldy, vp(1 << 24), 16384, m, 16384, vp(4096), vp(4096), None, 2, 8, vp(4096), 1, 32, 1, None, 0,
+                               vp(1 << 20), ldo, None, 0, None)
+    text = lib.pi05w4a4_last_error()
+    assert (rc == 1 and b"y must be" in text) if refused else rc == 3
