@@ -3,8 +3,9 @@
 The cache is a pool of pages of 64 tokens, keys and values [pages, KVH, 64, D] in fp16 or bf16.  Token i
 of sequence b is row i % 64 of page ``block_table[b, i // 64]`` (int32; entries outside the pool name
 no page): the tables and lengths are those of the 8-bit cache (``kv_int8``), whose half of the
-bytes cost the keys' and values' bits.  ``kv_append`` writes keys that are rotated already, as
-``prefix_attention`` returns its key states; ``qk_norm_rope_append`` norms and rotates on the way;
+bytes cost the keys' and values' bits.  ``kv_append`` writes keys that are rotated already, such as the
+key states [B, KVH, S, 256] of ``prefix_attention``: ``kv_append(keys.transpose(1, 2), v.unflatten(-1, (KVH, 256)), ..)``,
+views both; ``qk_norm_rope_append`` norms and rotates on the way;
 ``kv_attention`` attends decoded tokens over the cache, one a sequence or a few (action tokens behind a
 prefix, drafts).  Lengths live on the device and are the caller's to advance.
 """
