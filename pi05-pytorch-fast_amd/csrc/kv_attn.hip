@@ -11,9 +11,9 @@
 // tile e of a chunk of 16 VE dimensions then holds dimensions VE i + e, and a lane ends with 4 VE
 // consecutive ones.
 //
-// Few rows are bound by the cache's bytes: 64 sequences of up to 8192 tokens, D = 256, 400 MB, 81.6 us, 4.9 TB/s, where a
+// Few rows are bound by the cache's bytes: 64 sequences of up to 8192 tokens, D = 256, 400 MB, 81.8 us, 4.9 TB/s, where a
 // copy reaches 5.2; one sequence of 776 tokens by the latency of its loads one behind the other (lengths and
-// table, keys and values, the join), 8.9 us.  Many rows have a kernel of their own below.
+// table, keys and values, the join), 9.2 us.  Many rows have a kernel of their own below.
 //
 // Weights go into the products as a sum of 16-bit parts, each with its own product: the matrix pipe has the
 // time (the cache's bytes bound).  Three parts of bf16 hold all 24 bits of an fp32 weight, two of fp16 hold
@@ -429,8 +429,9 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void kv_attn16_kernel(KvA
 // The same for many rows: a workgroup takes 64 of a KV head, and a run of pages that reach LDS by direct loads, one
 // ahead.  Waves w and w + 4 take rows 16 w .. of it, and the page's first and second half.  Where 16 rows a workgroup
 // read every key for themselves, at the rate of the L2, this is bound by LDS (64 KB in and 256 KB out a page of
-// D = 256: 1.1 of its 1.6 us) and by the matrix products beside it: 32 x 50 tokens of 8 heads of 256 over 826 28.5 us
-// (16 rows a workgroup: 53), 64 x 64 54 (109), 8 x 776 over 776 68 (134), 440 TFLOP/s.
+// D = 256: 1.1 of its 1.6 us) and by the matrix products beside it: 32 x 50 tokens of 8 heads of 256 over 826 29.8 us
+// (16 rows a workgroup: 54), 64 x 64 54 (110), 8 x 776 over 776 69 (135), 430 TFLOP/s; bf16, whose weights take a third
+// product, 32.8 (58), 60 (118), 75 (143).
 //
 // Values are read from LDS a dimension a lane, so that they need no turning.  A key's 16-byte chunks stand in the order
 // chunk ^ f(key), f by the bits of the key that differ among the rows of a read, so that it meets every bank alike
@@ -652,9 +653,9 @@ constexpr size_t kMaxPartial = size_t{1} << 28;
 // bytes at 5.5 TB/s, which fewer workgroups than CUs do not reach; for more than one run the join, whose loads past
 // the sixteenth run follow one another, and partial results at 3.5 TB/s.
 // 16 rows a workgroup, us in 1 / 2 / 4 / 8 / 16 / 32 runs: D = 256, one sequence of 8192 keys 109 / - / - / - / 16.3 / 17.0, 16 of
-// 2048 32.5 / 23.1 / 17.3 / 14.6 / 15.0 (12) / -, 64 of 8192 - / 108 / 82 / 85 / 94 / -, 8 x 50 tokens over 826 17.4 / 26; D = 128, 8
+// 2048 32.5 / 23.1 / 17.3 / 14.6 / 15.0 (12) / -, 64 of 8192 - / 108 / 82 / 85 / 94 / -, 8 x 50 tokens over 826 18.9 / 28.7; D = 128, 8
 // KV heads, 8 of 1024 13.3 / 12.3 / 11.5 / 12.8 / - / -; D = 64, 8 KV heads, 4 of 4096 25.4 / 18.3 / 13.3 / 11.8 / 13.1 / 17.4.
-// 64 rows, us in 1 / 2 / 3 / 4 / 6 runs: D = 256, 8 x 50 tokens over 826 26.4 / 23.0 / 22.5 / 22.9 / 29.4; 8 KV heads of 128 with
+// 64 rows, us in 1 / 2 / 3 / 4 / 6 runs: D = 256, 8 x 50 tokens over 826 31.2 / 27.0 / 25.9 / 26.0 / 32.3; 8 KV heads of 128 with
 // 64 rows, 16 of 2048 37.4 / 31.5 / 39.0 / 38.0 / 44.8, of 64 26.7 / 21.7 / 22.9 / 22.1 / 25.0.
 // Runs of one page take two waves (one sequence of 776 keys, 13 runs, 1 / 2 / 4 waves: 9.6 / 9.8 / 11.2).
 KvAttn16Plan kv_attn16_plan(int64_t b, int64_t t, int32_t h, int32_t kvh, int32_t d, int64_t table_pages, int cus) {

@@ -300,7 +300,7 @@ def kv_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
     padding) of ``lens`` [B] cached ones, whose keys the cache holds already.  When ``causal``, query i
     sees the first lens - q_len + i + 1 tokens, else all of them.  A length past the table (64 tokens an
     entry) counts as the table's, for the place of the queries too.  A query that sees no token, a
-    padding row among them, gets zeros.  What a query does not see has no effect on it, whatever it
+    padding row among them, gets zeros, and so does one whose scores are all minus infinity.  What a query does not see has no effect on it, whatever it
     holds; a NaN or infinity among the values it sees makes its output in that dimension NaN or infinite.  With
     ``return_lse``, also the natural log of the sum of exp(scaling q k), fp32 [B, T, H] (-inf where none
     is seen), with which attention over further keys can be joined."""
